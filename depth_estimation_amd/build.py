@@ -44,6 +44,9 @@ def build(force: bool = False, verbose: bool = True) -> Path:
     if not force and not stale():
         return LIB
     common = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-ffp-contract=off", "-fno-slp-vectorize",
+              # the packed fp32 instructions hipcc forms by itself have given wrong results on gfx950
+              # boards now and then: plain ones only
+              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
               "-fPIC", "-fvisibility=hidden", "-DDW_BUILD", f"-I{ROOT / 'include'}", f"-I{CSRC}"]
     objdir = ROOT / "build" / "obj"
     objdir.mkdir(parents=True, exist_ok=True)
