@@ -29,6 +29,21 @@ class DwDesc(C.Structure):
                 ("S", C.c_int32), ("F", C.c_int32), ("flags", C.c_int32)]
 
 
+DW_DTYPE_F32, DW_DTYPE_BF16, DW_DTYPE_F16 = 0, 1, 2
+DW_DIST_INDEX64 = 1
+DW_DIST_LAST = 2
+DW_DIST_RENORMALISE = 4
+DW_DIST_TEACHER_BF16 = 8
+DW_DIST_TEACHER_F16 = 16
+DW_DIST_MAX_ENTRIES = 64
+
+
+class DwDistDesc(C.Structure):
+    _fields_ = [("outer", C.c_int64), ("classes", C.c_int64), ("inner", C.c_int64),
+                ("entry_stride", C.c_int64 * 3), ("scale", C.c_float), ("dtype", C.c_int32),
+                ("entries", C.c_int32), ("flags", C.c_int32)]
+
+
 class DepthwarpError(RuntimeError):
     pass
 
@@ -37,6 +52,7 @@ _lib = None
 
 _VP = C.c_void_p
 _PP = C.POINTER(C.c_void_p)
+_DD = C.POINTER(DwDistDesc)
 _SIGNATURES = {
     "dw_version": (C.c_int, []),
     "dw_strerror": (C.c_char_p, [C.c_int]),
@@ -77,6 +93,12 @@ _SIGNATURES = {
     "dw_lidar_workspace_bytes": (C.c_size_t, [C.c_int32] * 4),
     "dw_lidar_project": (C.c_int, [C.c_int32] * 4 + [_VP, _VP, _VP, C.c_int32, _VP, _VP, _VP, _VP, C.c_size_t,
                                                       _VP]),
+    "dw_log_probs_workspace_bytes": (C.c_int64, [_DD]),
+    "dw_log_probs_fwd": (C.c_int, [_DD] + [_VP] * 8 + [C.c_size_t, _VP]),
+    "dw_log_probs_bwd": (C.c_int, [_DD] + [_VP] * 8),
+    "dw_distill_workspace_bytes": (C.c_int64, [_DD]),
+    "dw_distill_fwd": (C.c_int, [_DD] + [_VP] * 6 + [C.c_size_t, _VP]),
+    "dw_distill_bwd": (C.c_int, [_DD] + [_VP] * 7),
     "dw_cost_volume_fwd": (C.c_int, [C.c_int32] * 5 + [_VP] * 7),
     "dw_cost_volume_bwd": (C.c_int, [C.c_int32] * 5 + [_VP] * 7),
 }

@@ -18,7 +18,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libdepthwarp.so"
-SOURCES = ["photometric.hip", "compute_loss.hip", "modules.hip", "soft_argmin.hip", "cost_volume.hip", "lidar.hip", "abi.hip"]
+SOURCES = ["photometric.hip", "compute_loss.hip", "modules.hip", "soft_argmin.hip", "cost_volume.hip", "lidar.hip",
+           "distribution.hip", "abi.hip"]
 # per-source options: the tile kernel runs 1 % faster with the scheduler's max-ILP strategy
 # (measured), the soft-argmin backward kernel much slower, so the option is not global
 EXTRA_FLAGS = {"photometric.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]}

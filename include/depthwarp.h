@@ -371,6 +371,73 @@ DW_API int dw_lidar_project(int32_t B, int32_t n_max, int32_t H, int32_t W, cons
                             double* pts_im, int32_t* n_valid, double* depth, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Distributions over classes (disparity bins of a volume, or any other soft-max
+ * axis): scoring and distillation.  Absent from the reference; they stand next
+ * to its disparity regression (/root/reference/model/model.py:417-429, 454-456).
+ *
+ * Logits are (outer, classes, inner) contiguous; with DW_DIST_LAST the classes
+ * of a row lie together: (outer, inner, classes).  Rows are numbered outer *
+ * inner + inner index.  z = scale * x (scale -1 turns costs into logits, 1/T is
+ * a temperature), p = softmax(z) over the classes of a row.  Sums and outputs
+ * are float32 for every element type.
+ *   A class at -inf (z) has probability 0; a row of nothing else has entropy 0,
+ *   log-probability -inf and gradient 0.  A row with NaN or z = +inf gives NaN
+ *   (its top classes are ordered all the same: NaN first).
+ *   Rows behind the last, and bytes between rows, are neither read nor written.
+ * ------------------------------------------------------------------------- */
+typedef struct dw_dist_desc {
+  int64_t outer, classes, inner; /* 1 <= classes <= 2^28; outer or inner may be 0: nothing to do */
+  int64_t entry_stride[3];       /* distillation: element strides of the teacher's list along outer, entry, inner */
+  float scale;                   /* finite, not 0 */
+  int32_t dtype;                 /* of the logits and their gradient: DW_DTYPE_* */
+  int32_t entries;               /* top classes wanted (0..64, at most classes) / entries of the teacher's list (1..64) */
+  int32_t flags;                 /* DW_DIST_* */
+} dw_dist_desc;
+
+#define DW_DTYPE_F32 0
+#define DW_DTYPE_BF16 1
+#define DW_DTYPE_F16 2
+
+#define DW_DIST_INDEX64 1       /* index / teacher_index is int64 (else int32) */
+#define DW_DIST_LAST 2          /* the classes of a row lie together */
+#define DW_DIST_RENORMALISE 4   /* distillation: soft-max over the listed entries, no further class */
+#define DW_DIST_TEACHER_BF16 8  /* the teacher's values are bfloat16 (else float32) */
+#define DW_DIST_TEACHER_F16 16  /* ... float16 */
+
+/* Log-probability of a given class, entropy, and the classes of largest z.
+ *   index          (rows) or NULL; a value outside [0, classes): no class given, log_prob 0
+ *   log_prob       (rows) out, or NULL          entropy  (rows) out, or NULL
+ *   top_log_prob, top_index   (outer, entries, inner) out, with DW_DIST_LAST (rows, entries);
+ *                  descending, ties by lowest index; NULL with entries = 0
+ *   stats          (rows, 2) out for the backward pass, or NULL
+ * dw_log_probs_workspace_bytes: bytes (0: no workspace needed), or a negative DW_ERR_* code.
+ * Backward: grad_logits from grad_log_prob and / or grad_entropy ((rows), either may be
+ * NULL); a row whose gradients are all 0 (or whose class is not given) gets zeros
+ * whatever its logits are.  `entropy` is needed with grad_entropy. */
+DW_API int64_t dw_log_probs_workspace_bytes(const dw_dist_desc* d);
+DW_API int dw_log_probs_fwd(const dw_dist_desc* d, const void* logits, const void* index, float* log_prob,
+                            float* entropy, float* top_log_prob, int32_t* top_index, float* stats,
+                            void* workspace, size_t workspace_bytes, void* stream);
+DW_API int dw_log_probs_bwd(const dw_dist_desc* d, const void* logits, const void* index, const float* stats,
+                            const float* entropy, const float* grad_log_prob, const float* grad_entropy,
+                            void* grad_logits, void* stream);
+
+/* Kullback-Leibler divergence of the logits from a teacher known by its top entries: classes i_e with
+ * log-probabilities l_e.  An entry with an index outside [0, classes) is padding, whatever its value.
+ *   q_e = exp l_e; everything unlisted is one more class: r = max(0, 1 - sum q) against the unlisted
+ *   classes' probability P;  loss = sum q (l - log p_i) + r (log r - log P)
+ *   (no such term where nothing unlisted has a finite z).
+ *   DW_DIST_RENORMALISE: q = softmax over the listed l (log-probabilities or logits), r = 0.
+ * A class listed twice counts with both its entries.  A row without entries has loss and gradient 0.
+ *   loss (rows) out; stats (rows, 4) out for the backward pass, or NULL
+ * Backward: with Q = sum q + r, listed  dx = g scale (p Q - q), unlisted dx = g scale p (Q - r / P). */
+DW_API int64_t dw_distill_workspace_bytes(const dw_dist_desc* d);
+DW_API int dw_distill_fwd(const dw_dist_desc* d, const void* logits, const void* teacher, const void* teacher_index,
+                          float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+DW_API int dw_distill_bwd(const dw_dist_desc* d, const void* logits, const void* teacher, const void* teacher_index,
+                          const float* stats, const float* grad_loss, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,153 @@
+"""Distributions over classes without a GPU: the float64 oracle against autograd, differences and closed
+forms; refusals of the Python entry points and of the C ABI (nothing is launched)."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from depth_estimation_amd import _lib
+from oracle import distribution as ref
+
+INF = float("inf")
+
+
+def _rows(n, V, seed=0, spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(n, V, generator=g, dtype=torch.float64) * spread, g
+
+
+# --------------------------------------------------------------------------- the oracle itself
+
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.5])
+def test_oracle_log_probs_is_log_softmax_and_its_gradient_is_autograds(scale):
+    x, g = _rows(7, 19)
+    idx = torch.tensor([0, 18, 5, -1, 19, 3, 3])
+    gl, gh = torch.randn(7, generator=g, dtype=torch.float64), torch.randn(7, generator=g, dtype=torch.float64)
+    out = ref.log_probs(x, idx, scale, top=4)
+    xr = x.clone().requires_grad_(True)
+    logp = F.log_softmax(xr * scale, -1)
+    lp = torch.where((idx >= 0) & (idx < 19), logp.gather(-1, idx.clamp(0, 18)[:, None])[:, 0], 0.0)
+    ent = torch.distributions.Categorical(logits=xr * scale).entropy()
+    assert torch.allclose(out["log_prob"], lp) and torch.allclose(out["entropy"], ent)
+    top = logp.detach().topk(4, -1)
+    assert torch.equal(out["top_index"].long(), top.indices) and torch.allclose(out["top_log_prob"], top.values)
+    want, = torch.autograd.grad([lp, ent], [xr], [gl, gh])
+    assert torch.allclose(ref.log_probs_grad(x, idx, scale, gl, gh), want, atol=1e-12)
+
+
+@pytest.mark.parametrize("renormalise", [False, True])
+@pytest.mark.parametrize("scale", [1.0, -0.7])
+def test_oracle_distill_gradient_against_differences(scale, renormalise):
+    x, g = _rows(5, 11, seed=3)
+    idx = torch.tensor([[0, 4, 7], [10, 10, 2], [3, -1, 5], [-1, -1, 11], [6, 1, 0]])   # twice, padding, none
+    val = F.log_softmax(torch.randn(5, 4, generator=g, dtype=torch.float64), -1)[:, :3]
+    out = ref.distill(x, val, idx, scale, renormalise)
+    eps = 1e-5
+    for j in range(11):
+        d = torch.zeros(5, 11, dtype=torch.float64)
+        d[:, j] = eps
+        num = (ref.distill(x + d, val, idx, scale, renormalise)["loss"]
+               - ref.distill(x - d, val, idx, scale, renormalise)["loss"]) / (2 * eps)
+        assert torch.allclose(out["grad"][:, j], num, atol=1e-8), j
+    assert out["loss"][3] == 0 and (out["grad"][3] == 0).all()
+
+
+def test_oracle_distill_of_a_full_list_is_the_divergence_and_vanishes_for_equal_distributions():
+    x, g = _rows(4, 6, seed=5)
+    t = torch.randn(4, 6, generator=g, dtype=torch.float64)
+    idx = torch.arange(6).expand(4, 6)
+    out = ref.distill(x, F.log_softmax(t, -1), idx)
+    want = F.kl_div(F.log_softmax(x, -1), F.log_softmax(t, -1), log_target=True, reduction="none").sum(-1)
+    assert torch.allclose(out["loss"], want)
+    same = ref.distill(x, F.log_softmax(x, -1)[:, :3], idx[:, :3])
+    assert same["loss"].abs().max() < 1e-12 and same["grad"].abs().max() < 1e-12
+
+
+def test_oracle_masked_and_empty_rows():
+    x, _ = _rows(3, 5, seed=1)
+    x[0] = -INF
+    x[1, 1:] = -INF
+    idx = torch.tensor([2, 0, 4])
+    out = ref.log_probs(x, idx, 1.0, top=5)
+    assert out["log_prob"][0] == -INF and out["entropy"][0] == 0 and out["top_index"][0].tolist() == [0, 1, 2, 3, 4]
+    assert out["log_prob"][1] == 0 and out["entropy"][1] == 0
+    one = torch.ones(3, dtype=torch.float64)
+    g = ref.log_probs_grad(x, idx, 1.0, one, one)
+    assert g.isfinite().all() and (g[0] == 0).all()
+    lowest = torch.full((1, 8), torch.finfo(torch.float32).min)
+    assert abs(float(ref.log_probs(lowest, torch.tensor([3]))["entropy"]) - math.log(8)) < 1e-12
+
+
+# ----------------------------------------------------------------------------------- refusals
+
+def _desc(outer=2, classes=8, inner=1, scale=1.0, dtype=0, entries=2, flags=0):
+    import ctypes
+    return ctypes.byref(_lib.DwDistDesc(outer, classes, inner, (2, 1, 1), scale, dtype, entries, flags))
+
+
+BAD = [(dict(classes=0), -2), (dict(classes=(1 << 28) + 1), -2), (dict(outer=-1), -2), (dict(inner=-1), -2),
+       (dict(entries=-1), -2), (dict(entries=65), -2), (dict(dtype=3), -5), (dict(dtype=-1), -5), (dict(flags=64), -5),
+       (dict(scale=0.0), -5), (dict(scale=INF), -5), (dict(scale=float("nan")), -5),
+       (dict(outer=1 << 41), -2), (dict(outer=1 << 39, inner=1 << 39), -2), (dict(outer=1 << 30, classes=1 << 27), -2)]
+
+
+@pytest.mark.parametrize("kw,code", BAD)
+def test_abi_refuses_bad_problems_before_touching_a_pointer(kw, code):
+    lib = _lib.lib()
+    d = _desc(**kw)
+    assert lib.dw_log_probs_workspace_bytes(d) == code
+    assert lib.dw_log_probs_fwd(d, None, None, None, None, None, None, None, None, 0, None) == code
+    assert lib.dw_log_probs_bwd(d, None, None, None, None, None, None, None, None) == code
+    assert lib.dw_distill_workspace_bytes(d) == code
+    assert lib.dw_distill_fwd(d, None, None, None, None, None, None, 0, None) == code
+    assert lib.dw_distill_bwd(d, None, None, None, None, None, None, None) == code
+
+
+def test_abi_refuses_null_pointers_small_workspaces_and_misfit_lists():
+    lib = _lib.lib()
+    x = 256   # stands for a device pointer: nothing is launched
+    assert lib.dw_log_probs_workspace_bytes(None) == -1 and lib.dw_distill_workspace_bytes(None) == -1
+    d = _desc()
+    assert lib.dw_log_probs_fwd(d, None, x, x, x, x, x, x, None, 0, None) == -1
+    assert lib.dw_log_probs_fwd(d, x, None, x, x, x, x, x, None, 0, None) == -1      # log_prob without an index
+    assert lib.dw_log_probs_fwd(d, x, x, x, x, None, x, x, None, 0, None) == -1      # entries without their outputs
+    assert lib.dw_log_probs_bwd(d, x, x, None, x, x, x, x, None) == -1
+    assert lib.dw_log_probs_bwd(d, x, x, x, None, x, x, x, None) == -1               # entropy's gradient needs the entropy
+    assert lib.dw_log_probs_bwd(d, x, None, x, x, x, None, x, None) == -1
+    assert lib.dw_distill_fwd(d, x, x, None, x, x, None, 0, None) == -1
+    assert lib.dw_distill_bwd(d, x, x, x, None, x, x, None) == -1
+    assert lib.dw_log_probs_workspace_bytes(_desc(classes=1, entries=2)) == -2       # more top classes than classes
+    assert lib.dw_log_probs_workspace_bytes(_desc(flags=4)) == -5                    # a flag of the other operator
+    assert lib.dw_distill_workspace_bytes(_desc(entries=0)) == -2
+    assert lib.dw_distill_workspace_bytes(_desc(flags=8 | 16)) == -5
+    one_long_row = _desc(outer=1, classes=1 << 20, entries=4)
+    n = lib.dw_log_probs_workspace_bytes(one_long_row)
+    assert n > 0 and n % 256 == 0
+    assert lib.dw_log_probs_fwd(one_long_row, x, x, x, x, x, x, x, None, n, None) == -1
+    assert lib.dw_log_probs_fwd(one_long_row, x, x, x, x, x, x, x, x, n - 1, None) == -3
+    assert lib.dw_log_probs_fwd(one_long_row, x, x, x, x, x, x, x, x + 8, n, None) == -3
+    assert lib.dw_distill_workspace_bytes(one_long_row) > 0
+    assert lib.dw_distill_fwd(one_long_row, x, x, x, x, x, x, 0, None) == -3
+    # nothing to do: no pointer is needed
+    assert lib.dw_log_probs_fwd(_desc(outer=0), None, None, None, None, None, None, None, None, 0, None) == 0
+    assert lib.dw_distill_bwd(_desc(inner=0), None, None, None, None, None, None, None) == 0
+
+
+def test_header_and_binding_agree():
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "include", "depthwarp.h")).read()
+    for name, value in re.findall(r"#define\s+(DW_(?:DIST|DTYPE)_\w+)\s+(\d+)", text):
+        assert getattr(_lib, name) == int(value)
+    import ctypes
+    assert ctypes.sizeof(_lib.DwDistDesc) == 64
+
+
+def test_python_refuses_cpu_tensors():
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    with pytest.raises(_lib.DepthwarpError):
+        log_probs(torch.zeros(2, 4), torch.zeros(2, dtype=torch.long))
+    with pytest.raises(_lib.DepthwarpError):
+        distill_loss(torch.zeros(2, 4), torch.zeros(2, 2), torch.zeros(2, 2, dtype=torch.long))

@@ -1,0 +1,691 @@
+"""Log-probabilities and distillation over classes against the float64 oracle, at the sizes, masks, layouts
+and types where they can go wrong.
+
+Tolerances (u = 2^-24, half a step of float32).  t = (x - max) c is off by 3 u |t| (difference, product,
+constant), 2^t by another 2 u.  A sum of L positive terms, one after the other, is off by at most L u
+relative and by about sqrt(L) u where the roundings are independent; 6 sqrt(L) + 40 covers sums of up to
+4096 terms with the joins that follow.  So with T = max |z - max z| over the classes that carry weight
+(those with z > max - 40: e^-40 is far below u, but log-probabilities of single classes go by their
+own t) a log-probability is off by at most u (6 sqrt(L) + 40 + 4 |t|).  The entropy adds the roundings of
+w = sum e t, whose terms all have one sign: u (6 sqrt(L) + 40 + 4 T) (1 + H).  A gradient gets the same
+factor on each of the parts it is made of, plus half a step of its own type and the type's smallest step."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _factor(V):
+    return U * (6 * math.sqrt(min(V, 4096)) + 40)
+
+
+def _make(layout, shape, dtype, seed=0, spread=2.0, scale=1.0):
+    """Logits on the CPU in `dtype`, class axis 1; the kernels get them in the layout's memory order."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(shape, generator=g) * spread).to(dtype)
+    return x, g
+
+
+def _gpu(x, layout):
+    y = x.cuda()
+    if layout == "last":
+        y = y.movedim(1, -1).contiguous().movedim(-1, 1)
+    return y
+
+
+def _last(x):   # class axis last, as the oracle wants it
+    return x.movedim(1, -1).contiguous()
+
+
+def _close(got, want, tol, what):
+    got, want = got.detach().cpu().double(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    same = (got == want) | (got.isnan() & want.isnan())
+    bad = ~same & ~((got - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:4], want[bad][:4], (got - want).abs()[bad][:4])
+
+
+def _step(dtype):   # half a step relative, and half the smallest step
+    f = torch.finfo(dtype)
+    return f.eps / 2, max(f.smallest_normal * f.eps / 2, 2.0 ** -126)
+
+
+def _check_log_probs(x, idx, layout, scale, top, with_grad=True, seed=1):
+    from depth_estimation_amd.distribution import log_probs
+    from oracle import distribution as ref
+    V = x.shape[1]
+    xg = _gpu(x, layout).requires_grad_(with_grad)
+    out = log_probs(xg, idx.cuda(), scale=scale, top=top)
+    xl = _last(x)
+    want = ref.log_probs(xl, idx, scale, top)
+    f = _factor(V)
+    z = xl.double() * scale
+    t = (z - z.amax(-1, keepdim=True)).nan_to_num(0, 0, 0).clamp_min(-1e30).abs()
+    near = torch.where(t < 40, t, 0.0).amax(-1)
+    t_at = t.gather(-1, idx.clamp(0, V - 1).long()[..., None])[..., 0]
+    _close(out.log_prob, want["log_prob"], f + 4 * U * t_at, "log_prob")
+    tol_h = (f + 4 * U * near) * (1 + want["entropy"])
+    _close(out.entropy, want["entropy"], tol_h, "entropy")
+    assert torch.equal(_last(out.top_index.cpu()), want["top_index"])
+    t_top = t.gather(-1, want["top_index"].long())
+    _close(_last(out.top_log_prob.cpu()), want["top_log_prob"], f + 4 * U * t_top, "top_log_prob")
+    assert out.top_index.dtype == torch.int32 and not out.top_log_prob.requires_grad
+    if not with_grad:
+        return
+    g = torch.Generator().manual_seed(seed)
+    gl, gh = torch.randn(idx.shape, generator=g), torch.randn(idx.shape, generator=g) * 0.2
+    gl[gl.abs() < 0.05] = 0.0
+    for gh_ in (gh, torch.zeros_like(gh)):
+        use_h = bool((gh_ != 0).any())
+        outs, ups = ([out.log_prob, out.entropy], [gl.cuda(), gh_.cuda()]) if use_h else ([out.log_prob], [gl.cuda()])
+        grad, = torch.autograd.grad(outs, [xg], ups, retain_graph=True)
+        assert grad.dtype == x.dtype and grad.stride() == xg.stride()
+        w = ref.log_probs_grad(xl, idx, scale, gl, gh_)
+        _, logp, p, _ = ref.softmax(xl, scale)
+        half, tiny = _step(x.dtype)
+        lp = torch.where(p == 0, 0.0, logp).abs()
+        hit = torch.zeros_like(p).scatter_(-1, idx.clamp(0, V - 1).long()[..., None], 1.0)
+        rel = f + 4 * U * torch.where(p == 0, 0.0, t)
+        parts = gl.double().abs()[..., None] * (p + 4 * U / f * hit) + \
+            gh_.double().abs()[..., None] * p * (lp + want["entropy"][..., None] + 2)
+        _close(_last(grad.cpu()), w, half * w.abs() * (1 + 1e-6) + (rel * parts * abs(scale)).nan_to_num(0) * (1 + half) + tiny,
+               "grad")
+
+
+def _index(shape, V, seed, holes=True):
+    g = torch.Generator().manual_seed(seed + 77)
+    idx = torch.randint(0, V, shape, generator=g)
+    if holes:
+        flat = idx.view(-1)
+        flat[::5] = -1
+        flat[3::11] = V
+    return idx
+
+
+ROWS = [(1, 1), (3, 2), (2, 31), (5, 33), (1, 64), (4, 257), (3, 1000), (2, 2047), (2, 2048), (3, 2049), (2, 4096),
+        (5, 4097), (3, 8191), (2, 8193), (7, 16391), (1, 50001), (3, 131072)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V", ROWS)
+def test_log_probs_rows(n, V, dtype):
+    scale = [1.0, -1.0, 0.5][(n + V) % 3]
+    x, _ = _make("rows", (n, V), dtype, seed=V)
+    _check_log_probs(x, _index((n,), V, V), "rows", scale, min(V, [0, 1, 5, 20, 64][(V + n) % 5]))
+
+
+# enough rows that a thread takes one; the last tile is not full
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,top", [(1, 1), (7, 4), (31, 3), (32, 8), (33, 9), (63, 0), (64, 16), (65, 17), (129, 33)])
+def test_log_probs_many_short_rows(V, top, dtype):
+    x, _ = _make("rows", (8200, V), dtype, seed=V)
+    _check_log_probs(x, _index((8200,), V, V), "rows", [1.0, -0.5][V % 2], top)
+
+
+VOLUMES = [(1, 1, 1, 1), (1, 5, 1, 3), (2, 31, 3, 5), (1, 32, 8, 8), (2, 33, 5, 13), (1, 64, 9, 7), (3, 65, 1, 65),
+           (1, 96, 24, 80), (2, 193, 11, 17), (1, 256, 16, 40), (1, 1025, 3, 30)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["volume", "last"])
+@pytest.mark.parametrize("shape", VOLUMES)
+def test_log_probs_volumes(shape, layout, dtype):
+    V = shape[1]
+    scale = [-1.0, 1.0, 0.5][sum(shape) % 3]
+    x, _ = _make(layout, shape, dtype, seed=sum(shape))
+    idx = _index((shape[0],) + shape[2:], V, V)
+    _check_log_probs(x, idx, layout, scale, min(V, [0, 1, 4, 8, 10, 16, 40][sum(shape) % 7]))
+
+
+@pytest.mark.parametrize("top", [1, 4, 8, 16, 17, 64])
+@pytest.mark.parametrize("layout", ["volume", "last", "rows"])
+def test_top_with_equal_values_takes_the_lowest_index(layout, top):
+    # few distinct values, so that most of the list is decided by the index; one row constant
+    shape = (2, 200, 6, 11) if layout != "rows" else (37, 9000)
+    g = torch.Generator().manual_seed(top)
+    x = torch.randint(-3, 4, shape, generator=g).float()
+    x[0, :] = 2.0
+    x[1, ::3] = -0.0
+    x[1, 1::3] = 0.0
+    for dtype in DTYPES:
+        _check_log_probs(x.to(dtype), _index((shape[0],) + shape[2:], shape[1], 3), layout, 1.0, top, with_grad=False)
+        _check_log_probs(x.to(dtype), _index((shape[0],) + shape[2:], shape[1], 3), layout, -1.0, top, with_grad=False)
+
+
+@pytest.mark.parametrize("n", [1, 3, 700])
+def test_top_of_rows_whose_large_values_lie_in_one_threads_classes(n):
+    # values fall with the distance from classes that one thread of a block reads, so that many more classes
+    # than wanted lie above the bound the threads' maxima give
+    V = 65536
+    for dtype in DTYPES:
+        x = torch.zeros(n, V)
+        vec = 4 if dtype == torch.float32 else 8
+        pos = (torch.arange(0, V, 64 * vec)[:, None] + torch.arange(vec)).flatten() % V
+        x[:, pos] = 10 + torch.arange(len(pos)).float() % 97
+        x[0, :100] = torch.arange(100) * 0.25
+        _check_log_probs(x.to(dtype), torch.zeros(n, dtype=torch.long), "rows", 1.0, 64, with_grad=False)
+
+
+@pytest.mark.parametrize("layout", ["volume", "last", "rows", "many"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs_masks_and_special_values(layout, dtype):
+    shape = {"rows": (24, 4500), "many": (8256, 40)}.get(layout, (2, 70, 4, 12))
+    x, g = _make(layout, shape, dtype)
+    x = _last(x).flatten(0, -2) if layout in ("volume", "last") else x
+    V = x.shape[1]
+    low = torch.finfo(dtype).min
+    x[1] = -INF                                   # nothing left
+    x[2, : V - 1] = -INF                          # one class left
+    x[3] = low                                    # all at the lowest value: uniform
+    x[4, 5:] = low                                # masked by the lowest value
+    x[5, ::2] = -INF
+    x[6, 7] = float("nan")
+    x[7, 3] = INF
+    x[8] = torch.finfo(dtype).max
+    x[9, :] = 0.0
+    x[9, 4] = torch.finfo(dtype).max
+    x[10, 2:6] = float("nan")
+    x[11, 1:3] = INF
+    x[12, 9] = -INF
+    idx = _index((x.shape[0],), V, 1, holes=False)
+    idx[1], idx[2], idx[5], idx[12], idx[13] = 4, V - 1, 2, 9, -1
+    if layout in ("volume", "last"):
+        x, idx = x.view(2, 4, 12, V).movedim(-1, 1).contiguous(), idx.view(2, 4, 12)
+    lay = "rows" if layout == "many" else layout
+    _check_log_probs(x, idx, lay, 1.0, 6)
+    _check_log_probs(-x, idx, lay, -1.0, 20)
+
+
+@pytest.mark.parametrize("layout", ["volume", "last", "rows"])
+def test_rows_without_upstream_gradient_get_zeros_whatever_they_hold(layout):
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    shape = (1, 40, 5, 9) if layout != "rows" else (45, 4000)
+    x, _ = _make(layout, shape, torch.float32)
+    idx = _index(shape[:1] + shape[2:], shape[1], 2)
+    bad = idx < 0
+    x.movedim(1, -1)[bad] = float("nan")
+    xg = _gpu(x, layout).requires_grad_(True)
+    lp = log_probs(xg, idx.cuda()).log_prob
+    assert (lp[bad.cuda()] == 0).all()
+    grad, = torch.autograd.grad(lp, xg, torch.ones_like(lp))
+    assert (grad.movedim(1, -1)[bad.cuda()] == 0).all() and grad.isfinite().all()
+    # a teacher's list that is all padding, with NaN in its places
+    k = 3
+    t = torch.full(idx.shape + (k,), -1.2).movedim(-1, 1)
+    ti = torch.arange(k).expand(idx.shape + (k,)).clone().movedim(-1, 1)
+    ti.movedim(1, -1)[bad] = -1
+    t.movedim(1, -1)[bad] = float("nan")
+    loss = distill_loss(xg, t.cuda(), ti.cuda())
+    assert loss.isfinite().all() and (loss[bad.cuda()] == 0).all()
+    grad, = torch.autograd.grad(loss, xg, torch.ones_like(loss))
+    assert grad.isfinite().all() and (grad.movedim(1, -1)[bad.cuda()] == 0).all()
+    up = torch.ones_like(loss)
+    up[~bad.cuda()] = 0.0
+    grad, = torch.autograd.grad(distill_loss(xg, t.cuda(), ti.cuda()), xg, up)
+    assert (grad == 0).all()
+
+
+# ------------------------------------------------------------------------------- distillation
+
+def _teacher(rows, V, k, g, dtype=torch.float32, pad=True):
+    """List of distinct classes, class axis last."""
+    n = math.prod(rows)
+    idx = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(min(n, 64))])
+    idx = idx[torch.arange(n) % len(idx)].view(*rows, k).clone()
+    val = torch.log_softmax(torch.randn(*rows, min(V, k + 3), generator=g) * 2, -1)[..., :k].to(dtype).contiguous()
+    if pad:
+        flat = idx.view(n, k)
+        flat[1::4, k // 2:] = -1
+        flat[2::7] = V
+        val.view(n, k)[2::7] = float("nan")
+    return val, idx
+
+
+def _check_distill(x, val, idx, layout, scale, renormalise, teacher_layout="volume", with_grad=True):
+    """val, idx: class axis last, on the CPU."""
+    from depth_estimation_amd.distribution import distill_loss
+    from oracle import distribution as ref
+    V = x.shape[1]
+    xg = _gpu(x, layout).requires_grad_(with_grad)
+    tv, ti = val.movedim(-1, 1), idx.movedim(-1, 1)
+    if teacher_layout == "volume":
+        tv, ti = tv.contiguous(), ti.contiguous()
+    loss = distill_loss(xg, tv.cuda(), ti.cuda(), scale=scale, renormalise=renormalise)
+    xl = _last(x)
+    want = ref.distill(xl, val, idx, scale, renormalise)
+    z = xl.double() * scale
+    t = (z - z.amax(-1, keepdim=True)).nan_to_num(0, 0, 0).clamp_min(-1e30).abs()
+    k = val.shape[-1]
+    valid = (idx >= 0) & (idx < V)
+    t_at = torch.where(valid, t.gather(-1, idx.clamp(0, V - 1).long()), 0.0).amax(-1)
+    # the list's own sums (k terms), and the rest's distance from the maximum
+    f = _factor(V) + 2 * k * U
+    t_rest = t.masked_fill(ref._listed(idx, valid, V), INF).amin(-1)
+    t_rest = torch.where(t_rest == INF, 0.0, t_rest)
+    tol = (f + 8 * U) * want["size"] + 4 * U * (t_at + t_rest)
+    _close(loss, want["loss"], tol.nan_to_num(0, 0, 0), "loss")
+    if not with_grad:
+        return
+    up = torch.randn(idx.shape[:-1], generator=torch.Generator().manual_seed(5))
+    grad, = torch.autograd.grad(loss, xg, up.cuda())
+    assert grad.dtype == x.dtype and grad.stride() == xg.stride()
+    w = want["grad"] * up.double()[..., None]
+    half, tiny = _step(x.dtype)
+    rel = f + 8 * U + 4 * U * torch.where(t < 60, t, 0.0) + 4 * U * t_rest.clamp_max(60)[..., None]
+    tol = half * w.abs() * (1 + 1e-6) + (rel * want["grad_size"] * up.double().abs()[..., None]).nan_to_num(0, 0, 0) * (1 + half) + tiny
+    _close(_last(grad.cpu()), w, tol, "grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,k", [(1, 1, 1), (3, 2, 1), (2, 31, 31), (5, 33, 4), (1, 64, 8), (4, 257, 20), (2, 2048, 64),
+                                   (3, 2049, 33), (2, 4097, 64), (9, 8193, 5), (1, 50001, 20), (3, 131072, 64)])
+def test_distill_rows(n, V, k, dtype):
+    x, g = _make("rows", (n, V), dtype, seed=V)
+    val, idx = _teacher((n,), V, k, g, [torch.float32, torch.bfloat16, torch.float16][V % 3], pad=n > 3)
+    _check_distill(x, val, idx.int() if V % 2 else idx, "rows", [1.0, -1.0, 0.5][(n + V) % 3], bool(k % 2))
+    _check_distill(x, val, idx, "rows", 1.0, not k % 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,k", [(1, 1), (7, 7), (31, 4), (33, 8), (64, 3), (65, 20), (129, 64)])
+def test_distill_many_short_rows(V, k, dtype):
+    x, g = _make("rows", (8201, V), dtype, seed=V)
+    val, idx = _teacher((8201,), V, k, g)
+    _check_distill(x, val, idx, "rows", -0.5, bool(V % 2))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["volume", "last"])
+@pytest.mark.parametrize("shape,k", [((1, 1, 1, 1), 1), ((1, 5, 1, 3), 2), ((2, 31, 3, 5), 4), ((1, 32, 8, 8), 32),
+                                     ((2, 33, 5, 13), 8), ((3, 65, 1, 65), 5), ((1, 64, 24, 80), 4),
+                                     ((2, 193, 11, 17), 16), ((1, 256, 16, 40), 64)])
+def test_distill_volumes(shape, k, layout, dtype):
+    x, g = _make(layout, shape, dtype, seed=sum(shape))
+    rows = (shape[0],) + shape[2:]
+    val, idx = _teacher(rows, shape[1], k, g)
+    _check_distill(x, val, idx, layout, [-1.0, 1.0][k % 2], False, teacher_layout=["volume", "last"][k % 2])
+    _check_distill(x, val, idx.int(), layout, 0.5, True, teacher_layout=["last", "volume"][k % 2])
+
+
+@pytest.mark.parametrize("layout", ["volume", "last", "rows", "many"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_distill_lists_and_masks_that_go_to_the_limit(layout, dtype, renormalise):
+    n, V, k = {"rows": (96, 4500, 6), "many": (8256, 40, 6)}.get(layout, (96, 70, 6))
+    x, g = _make(layout, (n, V), dtype)
+    val, idx = _teacher((n,), V, k, g, pad=False)
+    low = torch.finfo(dtype).min
+    x[1] = -INF                                    # the student has nothing
+    x[2, 3:] = low                                 # the rest at the lowest value
+    idx[2, :3] = torch.arange(3)
+    idx[2, 3:] = -1
+    x[3, 6:] = -INF                                # nothing unlisted is left
+    idx[3] = torch.arange(6)
+    idx[4] = 5                                     # one class, six times
+    idx[5] = torch.tensor([1, 2, 1, 3, 2, 1])
+    idx[6] = -1
+    val[6] = float("nan")
+    val[7, 2] = -INF                               # listed, without probability
+    val[8] = -INF                                  # a list without probability
+    x[9, int(idx[9, 0])] = -INF                    # the teacher wants what the student cannot give
+    x[10, 20] = float("nan")
+    x[11, int(idx[11, 1])] = float("nan")
+    x[12, 21] = INF
+    x[13, int(idx[13, 2])] = INF
+    idx[14, 1:] = V
+    val[15] = -0.1                                 # more than probability 1
+    idx[16, ::2] = -(1 << 40)
+    idx[17, ::2] = 1 << 40
+    x[18, int(idx[18, 0])] = 40.0 if dtype == torch.float16 else 300.0    # the rest far below float32's range
+    x[19] = low
+    val[20, 3] = float("nan")
+    x[21, int(idx[21, 0])] = -INF
+    val[21, 0] = -INF                              # masked on both sides
+    xs, vs, ids, lay = x, val, idx, "rows"
+    if layout in ("volume", "last"):
+        xs, vs, ids, lay = x.view(2, 6, 8, V).movedim(-1, 1).contiguous(), val.view(2, 6, 8, k), idx.view(2, 6, 8, k), layout
+    _check_distill(xs, vs, ids, lay, 1.0, renormalise)
+    _check_distill(-xs, vs, ids, lay, -1.0, renormalise)
+
+
+def test_duplicated_classes_sum_before_they_are_rounded():
+    # the gradient of a class listed twice is p Q - (q1 + q2), rounded once: against the list with one entry
+    from depth_estimation_amd.distribution import distill_loss
+    x = (torch.randn(1, 50, 4, 16, generator=torch.Generator().manual_seed(0)) * 2).to(torch.bfloat16)
+    for layout in ("volume", "last"):
+        a = _gpu(x, layout).requires_grad_(True)
+        q = torch.tensor([0.25, 0.25, 0.125]).log().view(1, 3, 1, 1).expand(1, 3, 4, 16).contiguous().cuda()
+        i2 = torch.tensor([7, 7, 9]).view(1, 3, 1, 1).expand(1, 3, 4, 16).contiguous().cuda()
+        q1 = torch.tensor([0.5, 0.125]).log().view(1, 2, 1, 1).expand(1, 2, 4, 16).contiguous().cuda()
+        i1 = torch.tensor([7, 9]).view(1, 2, 1, 1).expand(1, 2, 4, 16).contiguous().cuda()
+        g2, = torch.autograd.grad(distill_loss(a, q, i2).sum(), a)
+        g1, = torch.autograd.grad(distill_loss(a, q1, i1).sum(), a)
+        # q1 + q2 and 0.5 differ by the roundings of exp alone: at most one step of bfloat16 apart, at few places
+        assert ((g1.float() - g2.float()).abs() <= 2 ** -7 * g1.float().abs()).all()
+        assert (g1 != g2).float().mean() < 0.01
+
+
+# --------------------------------------------------- gradients against differences, and a run of both
+
+@pytest.mark.parametrize("layout", ["volume", "last", "rows"])
+def test_gradients_against_differences(layout):
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    from oracle import distribution as ref
+    shape = (1, 24, 3, 5) if layout != "rows" else (15, 24)
+    x, g = _make(layout, shape, torch.float32)
+    rows = shape[:1] + shape[2:]
+    idx = _index(rows, 24, 4)
+    val, ti = _teacher(rows, 24, 5, g)
+    val = torch.where(val.isnan(), 0.0, val)
+    xg = _gpu(x, layout).requires_grad_(True)
+    out = log_probs(xg, idx.cuda(), scale=-1.0)
+    loss = distill_loss(xg, val.movedim(-1, 1).cuda(), ti.movedim(-1, 1).cuda(), scale=-1.0)
+    total = (out.log_prob * 0.7 + out.entropy * 0.2 + loss).sum()
+    grad, = torch.autograd.grad(total, xg)
+    xl = _last(x).double()
+    eps = 1e-4
+
+    def f(v):
+        o = ref.log_probs(v, idx, -1.0)
+        return o["log_prob"] * 0.7 + o["entropy"] * 0.2 + ref.distill(v, val, ti, -1.0)["loss"]
+
+    for j in range(24):
+        d = torch.zeros_like(xl)
+        d[..., j] = eps
+        num = (f(xl + d) - f(xl - d)) / (2 * eps)
+        # the differences' own error: eps^2 / 6 times a third derivative below 4
+        assert torch.allclose(_last(grad.cpu())[..., j].double(), num, atol=4e-8 + 1e-5 * 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["volume", "last"])
+def test_a_teachers_list_trains_a_student(layout, dtype):
+    """The two together, as they are used: a teacher's volume -> its top list -> the student's loss and
+    gradient, next to the likelihood of sparse ground truth and the disparity regression."""
+    from depth_estimation_amd.disparity import soft_argmin
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    from oracle import distribution as ref
+    shape, k = (2, 48, 12, 20), 8
+    tx, _ = _make(layout, shape, dtype, seed=1)
+    sx, _ = _make(layout, shape, dtype, seed=2)
+    teacher = log_probs(_gpu(tx, layout), scale=-1.0, top=k)
+    assert teacher.log_prob is None
+    student = _gpu(sx, layout).requires_grad_(True)
+    loss = distill_loss(student, teacher.top_log_prob, teacher.top_index, scale=-1.0)
+    idx = _index((2, 12, 20), 48, 9)
+    nll = -log_probs(student, idx.cuda(), scale=-1.0).log_prob
+    (loss.mean() + nll.mean()).backward()
+    t = ref.log_probs(_last(tx), None, -1.0, k)
+    want = ref.distill(_last(sx), t["top_log_prob"].float(), t["top_index"], -1.0)
+    _close(loss, want["loss"], (_factor(48) + 40 * U) * (want["size"] + 20), "loss")
+    n = 2 * 12 * 20
+    g = want["grad"] / n + ref.log_probs_grad(_last(sx), idx, -1.0, torch.full(idx.shape, -1.0 / n), torch.zeros(idx.shape))
+    half, tiny = _step(dtype)
+    # two gradients, each rounded, then added and rounded again
+    tol = 4 * half * (want["grad"].abs() / n + 2 / n) + 2 * tiny + _factor(48) * 8 / n
+    _close(_last(student.grad.cpu()), g, tol, "grad")
+    disp = soft_argmin(student.detach().float())
+    assert disp.shape == loss.shape and disp.isfinite().all()
+
+
+# ------------------------------------------------------------- strides, refusals, bytes left alone
+
+def test_strided_inputs_equal_their_copies():
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    g = torch.Generator().manual_seed(0)
+    big = torch.randn(4, 60, 10, 14, generator=g).cuda()
+    idx = torch.randint(-1, 60, (4, 5, 7), generator=g).cuda()
+    x = big[:, :, ::2, 1::2]
+    wide = torch.randint(-1, 60, (4, 5, 14), generator=g).cuda()
+    for view, i in ((x, idx), (x.transpose(2, 3), idx.transpose(1, 2)), (big[:, 3:, :5, :7], wide[..., ::2] - 3)):
+        a, b = log_probs(view, i, top=3), log_probs(view.contiguous(), i.contiguous(), top=3)
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+        v = view.detach().requires_grad_(True)
+        c = view.contiguous().requires_grad_(True)
+        t, ti = a.top_log_prob.transpose(2, 3).contiguous().transpose(2, 3), a.top_index
+        la, lb = distill_loss(v, t, ti), distill_loss(c, b.top_log_prob, b.top_index)
+        assert torch.equal(la, lb)
+        up = torch.rand(1, device="cuda").expand_as(la)
+        ga, = torch.autograd.grad(la, v, up)
+        gb, = torch.autograd.grad(lb, c, up.contiguous())
+        assert torch.equal(ga, gb)
+    # the class axis elsewhere
+    y = torch.randn(60, 6, 7, generator=g).cuda()
+    i = torch.randint(0, 60, (6, 7), generator=g).cuda()
+    a = log_probs(y, i, dim=0, top=4)
+    b = log_probs(y[None], i[None], top=4)
+    assert torch.equal(a.log_prob, b.log_prob[0]) and torch.equal(a.top_index, b.top_index[0])
+    c = log_probs(y.permute(1, 2, 0), i, dim=-1, top=4)       # the same memory, seen class axis last
+    assert torch.allclose(a.log_prob, c.log_prob, atol=1e-5) and torch.equal(a.top_index.permute(1, 2, 0), c.top_index)
+    one = log_probs(y[:, 0, 0], i[0, 0], dim=0, top=4)
+    assert one.log_prob.shape == () and one.top_index.shape == (4,)
+    assert torch.allclose(one.log_prob, a.log_prob[0, 0], atol=1e-5)
+
+
+def test_empty_batches():
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x = torch.empty(0, 9, device="cuda", requires_grad=True)
+    out = log_probs(x, torch.empty(0, dtype=torch.long, device="cuda"), top=2)
+    assert out.log_prob.shape == (0,) and out.top_index.shape == (0, 2)
+    g, = torch.autograd.grad(out.log_prob.sum(), x)
+    assert g.shape == x.shape
+    x = torch.empty(2, 9, 0, 4, device="cuda", requires_grad=True)
+    loss = distill_loss(x, torch.empty(2, 3, 0, 4, device="cuda"), torch.empty(2, 3, 0, 4, dtype=torch.int32, device="cuda"))
+    assert loss.shape == (2, 0, 4)
+    g, = torch.autograd.grad(loss.sum(), x)
+    assert g.shape == x.shape
+
+
+def test_refusals():
+    from depth_estimation_amd._lib import DepthwarpError
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x = torch.randn(3, 10, device="cuda")
+    i = torch.zeros(3, dtype=torch.long, device="cuda")
+    for bad, kw, err in [((x.double(), i), {}, TypeError), ((x, i.float()), {}, TypeError), ((x, i.short()), {}, TypeError),
+                         ((x, i[:2]), {}, ValueError), ((x, i[:, None]), {}, ValueError), ((x, i.cpu()), {}, ValueError),
+                         ((x.cpu(), i.cpu()), {}, DepthwarpError), ((x, i), dict(dim=2), ValueError),
+                         ((x, i), dict(top=11), ValueError), ((x, i), dict(top=-1), ValueError),
+                         ((x, i), dict(scale=0.0), ValueError), ((x, i), dict(scale=INF), ValueError),
+                         ((x, i), dict(scale=float("nan")), ValueError), ((x, i), dict(scale=1e-60), DepthwarpError),
+                         ((x[:, :0], i), {}, ValueError), ((torch.randn(2, 100, device="cuda"), None), dict(top=65), ValueError),
+                         ((torch.tensor(1.0, device="cuda"), None), dict(dim=0), ValueError)]:
+        with pytest.raises(err):
+            log_probs(*bad, **kw)
+    t, ti = torch.full((3, 4), -2.0, device="cuda"), torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+    for bad, kw, err in [((x, t.double(), ti), {}, TypeError), ((x, t, ti.float()), {}, TypeError),
+                         ((x, t[:2], ti), {}, ValueError), ((x, t, ti[:, :3]), {}, ValueError),
+                         ((x, t[:, :0], ti[:, :0]), {}, ValueError), ((x, t[0], ti[0]), {}, ValueError),
+                         ((x, t.cpu(), ti), {}, ValueError), ((x, t, ti.cpu()), {}, ValueError),
+                         ((x, t.clone().requires_grad_(True), ti), {}, ValueError), ((x, t, ti), dict(scale=0.0), ValueError),
+                         ((x, t.repeat(1, 17), ti.repeat(1, 17)), {}, ValueError)]:
+        with pytest.raises(err):
+            distill_loss(*bad, **kw)
+    xr = x.clone().requires_grad_(True)
+    lp = log_probs(xr, i).log_prob.sum()
+    with pytest.raises(RuntimeError):       # once differentiable
+        g, = torch.autograd.grad(lp, xr, create_graph=True)
+        torch.autograd.grad(g.sum(), xr)
+
+
+@pytest.mark.parametrize("outer,V,inner,last,dtype", [(5, 37, 1, 1, 2), (70, 100, 1, 1, 0), (8195, 19, 1, 1, 1), (2, 45, 67, 0, 1),
+                                                      (3, 5001, 1, 1, 1), (2, 300, 35, 1, 0)])
+def test_bytes_outside_the_outputs_are_left_alone(outer, V, inner, last, dtype):
+    import ctypes as C
+    from depth_estimation_amd import _lib
+    lib = _lib.lib()
+    rows, k, guard = outer * inner, 4, 97
+    td = [torch.float32, torch.bfloat16, torch.float16][dtype]
+
+    def out(n, d, fill):
+        return torch.full((n + 2 * guard,), fill, dtype=d, device="cuda")
+
+    def at(t):
+        return t.data_ptr() + guard * t.element_size()
+
+    def check(t, n, fill):
+        assert (t[:guard] == fill).all() and (t[guard + n:] == fill).all()
+        assert not (t[guard:guard + n] == fill).all()
+
+    x = out(rows * V, td, 7.0)
+    x[guard:-guard] = torch.randn(rows * V, device="cuda").to(td)
+    idx = torch.randint(0, V, (rows,), device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    d = _lib.DwDistDesc(outer, V, inner, (k * inner, 1, k) if last else (k * inner, inner, 1), 1.0, dtype, k,
+                        _lib.DW_DIST_INDEX64 | (_lib.DW_DIST_LAST if last else 0))
+    nb = max(lib.dw_log_probs_workspace_bytes(C.byref(d)), lib.dw_distill_workspace_bytes(C.byref(d)), 0)
+    ws = torch.full((nb + 512,), 171, dtype=torch.uint8, device="cuda")
+    lp, ent, stats, s4 = out(rows, torch.float32, 55.0), out(rows, torch.float32, 55.0), out(2 * rows, torch.float32, 55.0), out(4 * rows, torch.float32, 55.0)
+    tlp, tix, g = out(rows * k, torch.float32, 55.0), out(rows * k, torch.int32, -9), out(rows * V, td, 55.0)
+    assert lib.dw_log_probs_fwd(C.byref(d), at(x), idx.data_ptr(), at(lp), at(ent), at(tlp), at(tix), at(stats),
+                                ws.data_ptr(), nb, st) == 0
+    up = torch.ones(rows, device="cuda")
+    assert lib.dw_log_probs_bwd(C.byref(d), at(x), idx.data_ptr(), at(stats), at(ent), up.data_ptr(), up.data_ptr(), at(g), st) == 0
+    for t, n, f in ((lp, rows, 55.0), (ent, rows, 55.0), (stats, 2 * rows, 55.0), (tlp, rows * k, 55.0), (tix, rows * k, -9), (g, rows * V, 55.0)):
+        check(t, n, f)
+    ti = tix[guard:-guard].long().contiguous()
+    tv = tlp[guard:-guard].contiguous()
+    g2, loss = out(rows * V, td, 55.0), out(rows, torch.float32, 55.0)
+    assert lib.dw_distill_fwd(C.byref(d), at(x), tv.data_ptr(), ti.data_ptr(), at(loss), at(s4), ws.data_ptr(), nb, st) == 0
+    up = torch.full((rows,), 2.0, device="cuda")
+    assert lib.dw_distill_bwd(C.byref(d), at(x), tv.data_ptr(), ti.data_ptr(), at(s4), up.data_ptr(), at(g2), st) == 0
+    for t, n, f in ((loss, rows, 55.0), (s4, 4 * rows, 55.0), (g2, rows * V, 55.0)):
+        check(t, n, f)
+    assert (ws[nb:] == 171).all() and (x[:guard] == 7.0).all() and (x[-guard:] == 7.0).all()
+    # outputs that are not wanted may be left out; the others do not change
+    lp2 = out(rows, torch.float32, 55.0)
+    assert lib.dw_log_probs_fwd(C.byref(d), at(x), idx.data_ptr(), at(lp2), None, at(tlp), at(tix), None, ws.data_ptr(), nb, st) == 0
+    assert torch.equal(lp, lp2)
+
+
+# -------------------------------------------------------- streams, graphs, tracing, long offsets
+
+def _both(x, idx, t, ti):
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    out = log_probs(x, idx, scale=-1.0, top=5)
+    loss = distill_loss(x, t, ti, scale=-1.0)
+    grad, = torch.autograd.grad([out.log_prob, out.entropy, loss], [x], [torch.ones_like(loss)] * 3)
+    return [out.log_prob.detach(), out.entropy.detach(), out.top_log_prob, out.top_index, loss.detach(), grad]
+
+
+def _problem(shape, seed):
+    g = torch.Generator().manual_seed(seed)
+    rows = shape[:1] + shape[2:]
+    x = torch.randn(shape, generator=g).cuda().requires_grad_(True)
+    idx = torch.randint(-1, shape[1], rows, generator=g).cuda()
+    t = torch.log_softmax(torch.randn(rows + (9,), generator=g), -1)[..., :5].movedim(-1, 1).contiguous().cuda()
+    ti = torch.randint(0, shape[1], rows + (5,), generator=g).movedim(-1, 1).contiguous().cuda()
+    return x, idx, t, ti
+
+
+@pytest.mark.parametrize("shape", [(3, 40000), (1, 64, 24, 80)])
+def test_two_streams_and_repeated_calls_give_the_same_bits(shape):
+    a, b = _problem(shape, 0), _problem(shape, 1)
+    want_a, want_b = _both(*a), _both(*b)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            got_a = _both(*a)
+        with torch.cuda.stream(s2):
+            got_b = _both(*b)
+        torch.cuda.synchronize()
+        for got, want in ((got_a, want_a), (got_b, want_b)):
+            for p, q in zip(got, want):
+                assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("shape", [(3, 40000), (1, 64, 24, 80), (600, 5000)])
+def test_forward_and_backward_in_two_captured_graphs(shape):
+    a, b = _problem(shape, 0), _problem(shape, 1)
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    for p in (a, b):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _both(*p)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_both(*p))
+        graphs.append(g)
+    for seed in (5, 6, 7):
+        for p, s in ((a, seed), (b, seed + 10)):
+            for old, new in zip(p, _problem(shape, s)):
+                old.data.copy_(new.detach())
+        for o in outs:
+            for t in o:
+                t.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for p, o in ((a, outs[0]), (b, outs[1])):
+            for got, want in zip(o, _both(*p)):
+                assert torch.equal(got, want)
+
+
+def test_registered_operators():
+    import depth_estimation_amd.distribution  # noqa: F401
+    tests = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+    x, idx, t, ti = _problem((2, 20, 4, 6), 0)
+    torch.library.opcheck(torch.ops.depthwarp.log_probs.default, (x, idx, 1, -1.0, 3), test_utils=tests)
+    torch.library.opcheck(torch.ops.depthwarp.distill_loss.default, (x, t, ti, 1, 1.0, False), test_utils=tests)
+    xl = x.detach().contiguous(memory_format=torch.channels_last).requires_grad_(True)
+    torch.library.opcheck(torch.ops.depthwarp.log_probs.default, (xl, None, 1, 0.5, 2), test_utils=tests)
+    torch.library.opcheck(torch.ops.depthwarp.distill_loss.default, (xl, t, ti, 1, 1.0, True), test_utils=tests)
+
+
+def test_traced_calls_give_the_eager_results():
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x, idx, t, ti = _problem((2, 20, 4, 6), 3)
+
+    def f(x, idx, t, ti):
+        o = log_probs(x, idx, scale=-1.0, top=3)
+        return o.log_prob.sum() + (o.entropy * 0.5).sum() + distill_loss(x, t, ti).sum(), o.top_index
+
+    want, wi = f(x, idx, t, ti)
+    gw, = torch.autograd.grad(want, x)
+    got, gi = torch.compile(f, backend="aot_eager")(x, idx, t, ti)
+    gg, = torch.autograd.grad(got, x)
+    assert torch.equal(want, got) and torch.equal(wi, gi) and torch.equal(gw, gg)
+
+
+@pytest.mark.parametrize("shape", [(9, 1 << 28), (2300000, 1000), (3, 2900, 512, 512)])
+def test_offsets_beyond_32_bits(shape):
+    """More than 2^31 elements: the last rows come out as they do on their own."""
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for part in x.flatten().split(1 << 28):
+        part.copy_(torch.randn(part.numel(), generator=g, device="cuda", dtype=torch.bfloat16))
+    n = 1 if len(shape) == 4 else min(shape[0], 3)
+    rows = shape[:1] + shape[2:]
+    idx = torch.full(rows, shape[1] - 2, device="cuda")
+    top = 4 if shape[1] < 1 << 20 else 0
+    ti = torch.stack([idx, idx - 5], 1).int()
+    t = torch.full(ti.shape, -1.5, device="cuda")
+    out, loss = log_probs(x, idx, top=top), distill_loss(x, t, ti)
+    tail = log_probs(x[-n:].clone(), idx[-n:], top=top)
+    for a, b in zip(out, tail):
+        assert torch.allclose(a[-n:].float(), b.float(), rtol=1e-4, atol=1e-5)
+    assert torch.allclose(loss[-n:], distill_loss(x[-n:].clone(), t[-n:], ti[-n:]), rtol=1e-4, atol=1e-5)
+    del out, tail
+    x.requires_grad_(True)
+    for f, ups in ((lambda v, s: log_probs(v, idx[s]).log_prob, 0.5), (lambda v, s: distill_loss(v, t[s], ti[s]), 2.0)):
+        y = f(x, slice(None))
+        gr, = torch.autograd.grad(y, x, torch.full_like(y, ups))
+        del y
+        small = x.detach()[-n:].clone().requires_grad_(True)
+        ys = f(small, slice(rows[0] - n, None))
+        gs, = torch.autograd.grad(ys, small, torch.full_like(ys, ups))
+        a, b = gr[-n:], gs
+        assert ((a.float() - b.float()).abs() <= 2 ** -7 * b.float().abs() + 1e-12).all()
+        assert (gr[:1].float().abs().amax() > 0)
+        del gr, gs, a, b
