@@ -95,7 +95,7 @@ _SIGNATURES = {
                                                       _VP]),
     "dw_log_probs_workspace_bytes": (C.c_int64, [_DD]),
     "dw_log_probs_fwd": (C.c_int, [_DD] + [_VP] * 8 + [C.c_size_t, _VP]),
-    "dw_log_probs_bwd": (C.c_int, [_DD] + [_VP] * 8),
+    "dw_log_probs_bwd": (C.c_int, [_DD] + [_VP] * 7),
     "dw_distill_workspace_bytes": (C.c_int64, [_DD]),
     "dw_distill_fwd": (C.c_int, [_DD] + [_VP] * 6 + [C.c_size_t, _VP]),
     "dw_distill_bwd": (C.c_int, [_DD] + [_VP] * 7),

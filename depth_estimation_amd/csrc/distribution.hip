@@ -88,6 +88,9 @@ __device__ __forceinline__ float exp2_(float t) { return __builtin_amdgcn_exp2f(
 struct Acc {
   float m, s, w;
 };
+using Stats3 = Acc;  // what the backward pass gets of a row; m is 0 in an empty one
+// entropy = ln s - ln2 w / s: both terms are >= 0, nothing cancels
+__device__ __forceinline__ float entropy_of(float s, float w, float ln_s) { return s == 0.f ? 0.f : ln_s - kLn2 * w / s; }
 __device__ __forceinline__ Acc acc_empty() { return Acc{-kInf, 0.f, 0.f}; }
 
 template <bool ENT, int N>
@@ -381,7 +384,7 @@ __device__ __forceinline__ void settle(float (&v)[32], bool neg, int n) {
 template <class T, bool LAST, int K>
 __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
                             float* __restrict__ log_prob, float* __restrict__ entropy, float* __restrict__ top_lp,
-                            int32_t* __restrict__ top_idx, float2* __restrict__ stats) {
+                            int32_t* __restrict__ top_idx, Stats3* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
   const Place q = place<LAST>(p);
   const int nw = blockDim.x >> 6;
@@ -467,8 +470,8 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
           lp = log_p(neg ? -v : v, base, ln_s, p.scale);
         }
         if (log_prob) log_prob[q.row] = lp;
-        if (entropy) entropy[q.row] = a.s == 0.f ? 0.f : ln_s - kLn2 * a.w / a.s;
-        if (stats) stats[q.row] = make_float2(base, a.s);
+        if (entropy) entropy[q.row] = entropy_of(a.s, a.w, ln_s);
+        if (stats) stats[q.row] = Stats3{base, a.s, a.w};
       }
     }
     if constexpr (K > 0) {
@@ -495,16 +498,16 @@ struct LpCoef {
   bool dead;  // nothing comes back (or nothing is left of the row): the gradient is zero whatever the row holds
 };
 template <bool ENT>
-__device__ __forceinline__ LpCoef lp_coef(const Prob& p, int64_t row, const void* index, const float2* stats,
-                                          const float* entropy, const float* g_lp, const float* g_ent) {
+__device__ __forceinline__ LpCoef lp_coef(const Prob& p, int64_t row, const void* index, const Stats3* stats,
+                                          const float* g_lp, const float* g_ent) {
   LpCoef r;
-  const float2 st = stats[row];
+  const Stats3 st = stats[row];
   r.target = (index && g_lp) ? valid_index(load_index(index, row, p.flags), p.V) : -1;
   const float gl = r.target >= 0 ? g_lp[row] : 0.f, gh = ENT ? g_ent[row] : 0.f;
-  r.m = st.x;
-  r.dead = st.y == 0.f || (gl == 0.f && gh == 0.f);
-  const float f = p.scale / st.y;
-  r.k0 = ENT ? -f * (gl + gh * (entropy[row] - logf(st.y))) : -f * gl;
+  r.m = st.m;
+  r.dead = st.s == 0.f || (gl == 0.f && gh == 0.f);
+  const float f = p.scale / st.s;
+  r.k0 = ENT ? -f * (gl - gh * kLn2 * st.w / st.s) : -f * gl;
   r.k1 = ENT ? -f * gh * kLn2 : 0.f;
   r.hit = gl * p.scale;
   if (r.dead) r.target = -1;
@@ -518,15 +521,14 @@ __device__ __forceinline__ float lp_grad(const LpCoef& r, float v, float c, floa
 
 template <class T, bool LAST, bool ENT>
 __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
-                            const float2* __restrict__ stats, const float* __restrict__ entropy,
-                            const float* __restrict__ g_lp, const float* __restrict__ g_ent,
+                            const Stats3* __restrict__ stats, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
                             typename T::S* __restrict__ g) {
   extern __shared__ __align__(16) char smem[];
   const Place q = place<LAST>(p);
   char* stage = smem + q.wave * kStageBytes;
   const bool neg = p.scale < 0.f;
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
-  const LpCoef r = lp_coef<ENT>(p, q.row, index, stats, entropy, g_lp, g_ent);
+  const LpCoef r = lp_coef<ENT>(p, q.row, index, stats, g_lp, g_ent);
   const bool any_dead = __any(r.dead);
   for (int c0 = c_lo; c0 < c_hi; c0 += stage_classes<T, LAST>()) {
     const int n = min(stage_classes<T, LAST>(), c_hi - c0);
@@ -1007,7 +1009,7 @@ __device__ void row_top(const typename T::S* row, int begin, int end, int k, boo
 struct LpOut {
   float *log_prob, *entropy, *top_lp;
   int32_t* top_idx;
-  float2* stats;
+  Stats3* stats;
 };
 template <class T>
 __device__ __forceinline__ void lp_row_write(const Prob& p, int64_t row, const typename T::S* xr, const void* index,
@@ -1021,8 +1023,8 @@ __device__ __forceinline__ void lp_row_write(const Prob& p, int64_t row, const t
     lp = log_p(neg ? -v : v, base, ln_s, p.scale);
   }
   if (o.log_prob) o.log_prob[row] = lp;
-  if (o.entropy) o.entropy[row] = a.s == 0.f ? 0.f : ln_s - kLn2 * a.w / a.s;
-  if (o.stats) o.stats[row] = make_float2(base, a.s);
+  if (o.entropy) o.entropy[row] = entropy_of(a.s, a.w, ln_s);
+  if (o.stats) o.stats[row] = Stats3{base, a.s, a.w};
 }
 __device__ __forceinline__ void lp_row_top_write(const Prob& p, int64_t row, int rank, unsigned long long key,
                                                  const Acc& a, const LpOut& o) {
@@ -1103,8 +1105,8 @@ __global__ __launch_bounds__(256) void lp_row_join(Prob p, const typename T::S* 
 
 template <class T, int NT, bool ENT>
 __global__ __launch_bounds__(NT) void lp_row_bwd(Prob p, const typename T::S* __restrict__ x,
-                                                 const void* __restrict__ index, const float2* __restrict__ stats,
-                                                 const float* __restrict__ entropy, const float* __restrict__ g_lp,
+                                                 const void* __restrict__ index, const Stats3* __restrict__ stats,
+                                                 const float* __restrict__ g_lp,
                                                  const float* __restrict__ g_ent, typename T::S* __restrict__ g) {
   const int64_t row = blockIdx.x / (unsigned)p.chunks;
   const int chunk = blockIdx.x - (unsigned)row * p.chunks;
@@ -1113,7 +1115,7 @@ __global__ __launch_bounds__(NT) void lp_row_bwd(Prob p, const typename T::S* __
   typename T::S* gr = g + row * p.V;
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
   const bool neg = p.scale < 0.f;
-  const LpCoef r = lp_coef<ENT>(p, row, index, stats, entropy, g_lp, g_ent);
+  const LpCoef r = lp_coef<ENT>(p, row, index, stats, g_lp, g_ent);
   for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
     float v[32];
     if (r.dead) {
@@ -1431,21 +1433,21 @@ int lp_fwd(const Plan& P, const void* x, const void* index, const LpOut& o, void
   return launched();
 }
 template <class T, bool ENT>
-int lp_bwd(const Plan& P, const void* x, const void* index, const float2* stats, const float* entropy,
-           const float* g_lp, const float* g_ent, void* g, hipStream_t st) {
+int lp_bwd(const Plan& P, const void* x, const void* index, const Stats3* stats, const float* g_lp,
+           const float* g_ent, void* g, hipStream_t st) {
   using S = typename T::S;
   if (P.tile) {
     if (P.last) {
       const size_t lds = P.nw * kStageBytes;
       if (int rc = allow_lds(lp_tile_bwd<T, true, ENT>, lds)) return rc;
-      lp_tile_bwd<T, true, ENT><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, index, stats, entropy, g_lp, g_ent, (S*)g);
+      lp_tile_bwd<T, true, ENT><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
     } else {
-      lp_tile_bwd<T, false, ENT><<<P.grid, P.nw * 64, 0, st>>>(P.p, (const S*)x, index, stats, entropy, g_lp, g_ent, (S*)g);
+      lp_tile_bwd<T, false, ENT><<<P.grid, P.nw * 64, 0, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
     }
   } else if (P.nt == 64) {
-    lp_row_bwd<T, 64, ENT><<<P.grid, 64, 0, st>>>(P.p, (const S*)x, index, stats, entropy, g_lp, g_ent, (S*)g);
+    lp_row_bwd<T, 64, ENT><<<P.grid, 64, 0, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
   } else {
-    lp_row_bwd<T, 256, ENT><<<P.grid, 256, 0, st>>>(P.p, (const S*)x, index, stats, entropy, g_lp, g_ent, (S*)g);
+    lp_row_bwd<T, 256, ENT><<<P.grid, 256, 0, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
   }
   return launched();
 }
@@ -1498,7 +1500,7 @@ extern "C" int dw_log_probs_fwd(const dw_dist_desc* d, const void* logits, const
   if (P.p.rows == 0) return DW_OK;
   if (!logits || (log_prob && !index) || (P.p.k > 0 && (!top_log_prob || !top_index))) return DW_ERR_NULL;
   if (int rc = check_ws(P, workspace, workspace_bytes)) return rc;
-  const LpOut o{log_prob, entropy, top_log_prob, top_index, (float2*)stats};
+  const LpOut o{log_prob, entropy, top_log_prob, top_index, (Stats3*)stats};
   hipStream_t st = (hipStream_t)stream;
   switch (d->dtype) {
     case DW_DTYPE_F32: return lp_fwd<F32>(P, logits, index, o, workspace, st);
@@ -1508,17 +1510,17 @@ extern "C" int dw_log_probs_fwd(const dw_dist_desc* d, const void* logits, const
 }
 
 extern "C" int dw_log_probs_bwd(const dw_dist_desc* d, const void* logits, const void* index, const float* stats,
-                                const float* entropy, const float* grad_log_prob, const float* grad_entropy,
-                                void* grad_logits, void* stream) {
+                                const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
+                                void* stream) {
   Plan P;
   if (int rc = make_plan(d, false, true, &P)) return rc;
   if (P.p.rows == 0) return DW_OK;
-  if (!logits || !stats || !grad_logits || (grad_log_prob && !index) || (grad_entropy && !entropy)) return DW_ERR_NULL;
-  const float2* s2 = (const float2*)stats;
+  if (!logits || !stats || !grad_logits || (grad_log_prob && !index)) return DW_ERR_NULL;
+  const Stats3* s3 = (const Stats3*)stats;
   hipStream_t st = (hipStream_t)stream;
-#define DW_LP_BWD(T)                                                                                              \
-  return grad_entropy ? lp_bwd<T, true>(P, logits, index, s2, entropy, grad_log_prob, grad_entropy, grad_logits, st) \
-                      : lp_bwd<T, false>(P, logits, index, s2, entropy, grad_log_prob, grad_entropy, grad_logits, st)
+#define DW_LP_BWD(T)                                                                                     \
+  return grad_entropy ? lp_bwd<T, true>(P, logits, index, s3, grad_log_prob, grad_entropy, grad_logits, st) \
+                      : lp_bwd<T, false>(P, logits, index, s3, grad_log_prob, grad_entropy, grad_logits, st)
   switch (d->dtype) {
     case DW_DTYPE_F32: DW_LP_BWD(F32);
     case DW_DTYPE_BF16: DW_LP_BWD(BF16);

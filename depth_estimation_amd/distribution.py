@@ -71,15 +71,24 @@ def _rows_shape(x: Tensor, dim: int):
     return x.shape[:dim] + x.shape[dim + 1:]
 
 
+# Host time counts: a small training step is bound by it, and the interpreter runs cold in the autograd
+# engine's own thread.  So the backward passes find their descriptor made, and the device and stream are
+# read without building torch.cuda.Stream objects where torch has the calls its own compiler uses.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """One library call on the device's current stream (the library launches on the current device)."""
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if _current_device() == index:
+        rc = getattr(_lib.lib(), name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, name)
+            rc = getattr(_lib.lib(), name)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _ptr(t: Optional[Tensor]):
@@ -93,19 +102,18 @@ def _workspace(x: Tensor, nbytes: int) -> Optional[Tensor]:
 
 # ------------------------------------------------------------------------------ log-probabilities
 
-def _lp_forward(logits: Tensor, index: Optional[Tensor], dim: int, scale: float, top: int, need_stats: bool):
-    x, last = _place(logits, dim)
+def _lp_desc(x: Tensor, last: int, index: Optional[Tensor], dim: int, scale: float, top: int):
     outer, V, inner = _sizes(x, dim)
-    flags = last
-    if index is not None:
-        index = index.contiguous()
-        flags |= _INDEX_FLAGS[index.dtype]
-    ref, nbytes = _desc("dw_log_probs_workspace_bytes", outer, V, inner, (0, 0, 0), scale, _DTYPES[x.dtype], top, flags)
+    flags = last if index is None else last | _INDEX_FLAGS[index.dtype]
+    return _desc("dw_log_probs_workspace_bytes", outer, V, inner, (0, 0, 0), scale, _DTYPES[x.dtype], top, flags)
+
+
+def _lp_forward(x: Tensor, last: int, index: Optional[Tensor], dim: int, top: int, need_stats: bool, ref, nbytes: int):
     rows = _rows_shape(x, dim)
     dev = x.device
-    lp = torch.empty(rows if index is not None else (0,), dtype=torch.float32, device=dev)
     ent = torch.empty(rows, dtype=torch.float32, device=dev)
-    stats = torch.empty(rows + (2,), dtype=torch.float32, device=dev) if need_stats else None
+    lp = torch.empty_like(ent) if index is not None else torch.empty((0,), dtype=torch.float32, device=dev)
+    stats = torch.empty(rows + (3,), dtype=torch.float32, device=dev) if need_stats else None
     if last:   # the kernels write the list of a row together, too
         top_lp = torch.empty(rows + (top,), dtype=torch.float32, device=dev).movedim(-1, dim)
         top_idx = torch.empty(rows + (top,), dtype=torch.int32, device=dev).movedim(-1, dim)
@@ -120,23 +128,30 @@ def _lp_forward(logits: Tensor, index: Optional[Tensor], dim: int, scale: float,
     return lp, ent, top_lp, top_idx, stats
 
 
-def _lp_backward(logits: Tensor, index: Optional[Tensor], stats: Tensor, entropy: Tensor, g_lp: Optional[Tensor],
-                 g_ent: Optional[Tensor], dim: int, scale: float) -> Tensor:
-    x, last = _place(logits, dim)
-    outer, V, inner = _sizes(x, dim)
-    flags = last
-    if index is None:
-        g_lp = None
-    else:
-        index = index.contiguous()
-        flags |= _INDEX_FLAGS[index.dtype]
-    ref, _ = _desc("dw_log_probs_workspace_bytes", outer, V, inner, (0, 0, 0), scale, _DTYPES[x.dtype], 0, flags)
+def _lp_backward(x: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: Optional[Tensor], g_ent: Optional[Tensor],
+                 ref) -> Tensor:
     grad = torch.empty_like(x)
-    g_lp = None if g_lp is None else g_lp.contiguous()
-    g_ent = None if g_ent is None else g_ent.contiguous()
-    _call(x.device, "dw_log_probs_bwd", ref, x.data_ptr(), _ptr(index), stats.data_ptr(), entropy.data_ptr(),
-          _ptr(g_lp), _ptr(g_ent), grad.data_ptr())
+    if g_lp is not None:
+        g_lp = g_lp.contiguous() if index is not None else None
+    if g_ent is not None:
+        g_ent = g_ent.contiguous()
+    _call(x.device, "dw_log_probs_bwd", ref, x.data_ptr(), _ptr(index), stats.data_ptr(), _ptr(g_lp), _ptr(g_ent),
+          grad.data_ptr())
     return grad
+
+
+def _once(backward):
+    """`once_differentiable`, whose bookkeeping only a pass that builds a graph has to pay for."""
+    guarded = once_differentiable(backward)
+    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+
+def _lp_node_backward(ctx, g_lp, g_ent, _g_top, _g_index):
+    logits, index = ctx.saved_tensors
+    if g_lp is None and g_ent is None:
+        return None, None, None, None, None
+    x = logits if ctx.in_place else logits.contiguous()
+    return _lp_backward(x, index, ctx.stats, g_lp, g_ent, ctx.ref), None, None, None, None
 
 
 class _LogProbsFunction(torch.autograd.Function):
@@ -144,27 +159,25 @@ class _LogProbsFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, index, dim, scale, top):
-        lp, ent, top_lp, top_idx, stats = _lp_forward(logits, index, dim, scale, top, True)
+        x, last = _place(logits, dim)
+        ctx.ref, nbytes = _lp_desc(x, last, index, dim, scale, top)
+        lp, ent, top_lp, top_idx, ctx.stats = _lp_forward(x, last, index, dim, top, True, ctx.ref, nbytes)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_lp, top_idx)
-        ctx.save_for_backward(logits, index, stats, ent)
-        ctx.dim, ctx.scale = dim, scale
+        ctx.save_for_backward(logits, index)
+        ctx.in_place = x is logits
         return lp, ent, top_lp, top_idx
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, _g_top, _g_index):
-        logits, index, stats, ent = ctx.saved_tensors
-        if g_lp is None and g_ent is None:
-            return None, None, None, None, None
-        return _lp_backward(logits, index, stats, ent, g_lp, g_ent, ctx.dim, ctx.scale), None, None, None, None
+    backward = staticmethod(_once(_lp_node_backward))
 
 
 @torch.library.custom_op("depthwarp::log_probs", mutates_args=())
 def _log_probs_op(logits: Tensor, index: Optional[Tensor], dim: int, scale: float,
                   top: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """The same as a torch operator (what torch.compile traces); the last result is the backward's."""
-    return _lp_forward(logits, index, dim, scale, top, True)
+    x, last = _place(logits, dim)
+    index = None if index is None else index.contiguous()
+    return _lp_forward(x, last, index, dim, top, True, *_lp_desc(x, last, index, dim, scale, top))
 
 
 @_log_probs_op.register_fake
@@ -179,30 +192,32 @@ def _(logits, index, dim, scale, top):
     else:
         shape = x.shape[:dim] + (top,) + x.shape[dim + 1:]
         top_lp, top_idx = x.new_empty(shape, dtype=torch.float32), x.new_empty(shape, dtype=torch.int32)
-    return lp, ent, top_lp, top_idx, x.new_empty(rows + (2,), dtype=torch.float32)
+    return lp, ent, top_lp, top_idx, x.new_empty(rows + (3,), dtype=torch.float32)
 
 
 @torch.library.custom_op("depthwarp::log_probs_bwd", mutates_args=())
-def _log_probs_bwd_op(logits: Tensor, index: Optional[Tensor], stats: Tensor, entropy: Tensor, g_lp: Optional[Tensor],
+def _log_probs_bwd_op(logits: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: Optional[Tensor],
                       g_ent: Optional[Tensor], dim: int, scale: float) -> Tensor:
-    return _lp_backward(logits, index, stats, entropy, g_lp, g_ent, dim, scale)
+    x, last = _place(logits, dim)
+    index = None if index is None else index.contiguous()
+    return _lp_backward(x, index, stats, g_lp, g_ent, _lp_desc(x, last, index, dim, scale, 0)[0])
 
 
 @_log_probs_bwd_op.register_fake
-def _(logits, index, stats, entropy, g_lp, g_ent, dim, scale):
+def _(logits, index, stats, g_lp, g_ent, dim, scale):
     return torch.empty_like(_place(logits, dim)[0])
 
 
 def _lp_setup(ctx, inputs, output):
     logits, index, dim, scale, _top = inputs
     ctx.mark_non_differentiable(*output[2:])
-    ctx.save_for_backward(logits, index, output[4], output[1])
+    ctx.save_for_backward(logits, index, output[4])
     ctx.dim, ctx.scale = dim, scale
 
 
 def _lp_op_backward(ctx, g_lp, g_ent, _g_top, _g_index, _g_stats):
-    logits, index, stats, ent = ctx.saved_tensors
-    return _log_probs_bwd_op(logits, index, stats, ent, g_lp, g_ent, ctx.dim, ctx.scale), None, None, None, None
+    logits, index, stats = ctx.saved_tensors
+    return _log_probs_bwd_op(logits, index, stats, g_lp, g_ent, ctx.dim, ctx.scale), None, None, None, None
 
 
 _log_probs_op.register_autograd(_lp_op_backward, setup_context=_lp_setup)
@@ -255,12 +270,15 @@ def log_probs(logits: Tensor, index: Optional[Tensor] = None, *, dim: int = 1, s
         raise ValueError(f"top: expected 0 to {min(_lib.DW_DIST_MAX_ENTRIES, logits.shape[dim])}, got {top}")
     if index is not None:
         _check_index("index", index, _rows_shape(logits, dim), logits.device)
+        index = index.contiguous()
     if torch.compiler.is_compiling():
         lp, ent, top_lp, top_idx, _ = _log_probs_op(logits, index, dim, scale, top)
     elif logits.requires_grad and torch.is_grad_enabled():
         lp, ent, top_lp, top_idx = _LogProbsFunction.apply(logits, index, dim, scale, top)
     else:
-        lp, ent, top_lp, top_idx, _ = _lp_forward(logits, index, dim, scale, top, False)
+        x, last = _place(logits, dim)
+        lp, ent, top_lp, top_idx, _ = _lp_forward(x, last, index, dim, top, False,
+                                                  *_lp_desc(x, last, index, dim, scale, top))
     return LogProbs(lp if index is not None else None, ent, top_lp, top_idx)
 
 
@@ -284,14 +302,11 @@ def _ds_desc(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale: fl
     flags = last | _INDEX_FLAGS[index.dtype] | _TEACHER_FLAGS[teacher.dtype]
     if renormalise:
         flags |= _lib.DW_DIST_RENORMALISE
-    ref, nbytes = _desc("dw_distill_workspace_bytes", outer, V, inner, stride, scale, _DTYPES[x.dtype],
-                        teacher.shape[dim], flags)
-    return x, teacher, index, ref, nbytes
+    return x, teacher, index, _desc("dw_distill_workspace_bytes", outer, V, inner, stride, scale, _DTYPES[x.dtype],
+                                    teacher.shape[dim], flags)
 
 
-def _ds_forward(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale: float, renormalise: bool,
-                need_stats: bool):
-    x, teacher, index, ref, nbytes = _ds_desc(logits, teacher, index, dim, scale, renormalise)
+def _ds_forward(x: Tensor, teacher: Tensor, index: Tensor, dim: int, need_stats: bool, ref, nbytes: int):
     rows = _rows_shape(x, dim)
     loss = torch.empty(rows, dtype=torch.float32, device=x.device)
     stats = torch.empty(rows + (4,), dtype=torch.float32, device=x.device) if need_stats else None
@@ -301,9 +316,7 @@ def _ds_forward(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale:
     return loss, stats
 
 
-def _ds_backward(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, g_loss: Tensor, dim: int,
-                 scale: float, renormalise: bool) -> Tensor:
-    x, teacher, index, ref, _ = _ds_desc(logits, teacher, index, dim, scale, renormalise)
+def _ds_backward(x: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, g_loss: Tensor, ref) -> Tensor:
     grad = torch.empty_like(x)
     g_loss = g_loss.contiguous()
     _call(x.device, "dw_distill_bwd", ref, x.data_ptr(), teacher.data_ptr(), index.data_ptr(), stats.data_ptr(),
@@ -311,24 +324,29 @@ def _ds_backward(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, 
     return grad
 
 
+def _ds_node_backward(ctx, g_loss):
+    logits, teacher, index = ctx.saved_tensors
+    x = logits if ctx.in_place else logits.contiguous()
+    return _ds_backward(x, teacher, index, ctx.stats, g_loss, ctx.ref), None, None, None, None, None
+
+
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, index, dim, scale, renormalise):
-        loss, stats = _ds_forward(logits, teacher, index, dim, scale, renormalise, True)
-        ctx.save_for_backward(logits, teacher, index, stats)
-        ctx.args = (dim, scale, renormalise)
+        x, teacher, index, (ctx.ref, nbytes) = _ds_desc(logits, teacher, index, dim, scale, renormalise)
+        loss, ctx.stats = _ds_forward(x, teacher, index, dim, True, ctx.ref, nbytes)
+        ctx.save_for_backward(logits, teacher, index)
+        ctx.in_place = x is logits
         return loss
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_loss):
-        return _ds_backward(*ctx.saved_tensors, g_loss, *ctx.args), None, None, None, None, None
+    backward = staticmethod(_once(_ds_node_backward))
 
 
 @torch.library.custom_op("depthwarp::distill_loss", mutates_args=())
 def _distill_op(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale: float,
                 renormalise: bool) -> Tuple[Tensor, Tensor]:
-    return _ds_forward(logits, teacher, index, dim, scale, renormalise, True)
+    x, teacher, index, plan = _ds_desc(logits, teacher, index, dim, scale, renormalise)
+    return _ds_forward(x, teacher, index, dim, True, *plan)
 
 
 @_distill_op.register_fake
@@ -340,7 +358,8 @@ def _(logits, teacher, index, dim, scale, renormalise):
 @torch.library.custom_op("depthwarp::distill_loss_bwd", mutates_args=())
 def _distill_bwd_op(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, g_loss: Tensor, dim: int,
                     scale: float, renormalise: bool) -> Tensor:
-    return _ds_backward(logits, teacher, index, stats, g_loss, dim, scale, renormalise)
+    x, teacher, index, (ref, _) = _ds_desc(logits, teacher, index, dim, scale, renormalise)
+    return _ds_backward(x, teacher, index, stats, g_loss, ref)
 
 
 @_distill_bwd_op.register_fake
@@ -397,4 +416,5 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
         return _distill_op(logits, teacher, teacher_index, dim, scale, renormalise)[0]
     if grad and logits.requires_grad:
         return _DistillFunction.apply(logits, teacher, teacher_index, dim, scale, renormalise)
-    return _ds_forward(logits, teacher, teacher_index, dim, scale, renormalise, False)[0]
+    x, teacher, teacher_index, plan = _ds_desc(logits, teacher, teacher_index, dim, scale, renormalise)
+    return _ds_forward(x, teacher, teacher_index, dim, False, *plan)[0]

@@ -410,18 +410,18 @@ typedef struct dw_dist_desc {
  *   log_prob       (rows) out, or NULL          entropy  (rows) out, or NULL
  *   top_log_prob, top_index   (outer, entries, inner) out, with DW_DIST_LAST (rows, entries);
  *                  descending, ties by lowest index; NULL with entries = 0
- *   stats          (rows, 2) out for the backward pass, or NULL
+ *   stats          (rows, 3) out for the backward pass, or NULL
  * dw_log_probs_workspace_bytes: bytes (0: no workspace needed), or a negative DW_ERR_* code.
  * Backward: grad_logits from grad_log_prob and / or grad_entropy ((rows), either may be
  * NULL); a row whose gradients are all 0 (or whose class is not given) gets zeros
- * whatever its logits are.  `entropy` is needed with grad_entropy. */
+ * whatever its logits are. */
 DW_API int64_t dw_log_probs_workspace_bytes(const dw_dist_desc* d);
 DW_API int dw_log_probs_fwd(const dw_dist_desc* d, const void* logits, const void* index, float* log_prob,
                             float* entropy, float* top_log_prob, int32_t* top_index, float* stats,
                             void* workspace, size_t workspace_bytes, void* stream);
 DW_API int dw_log_probs_bwd(const dw_dist_desc* d, const void* logits, const void* index, const float* stats,
-                            const float* entropy, const float* grad_log_prob, const float* grad_entropy,
-                            void* grad_logits, void* stream);
+                            const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
+                            void* stream);
 
 /* Kullback-Leibler divergence of the logits from a teacher known by its top entries: classes i_e with
  * log-probabilities l_e.  An entry with an index outside [0, classes) is padding, whatever its value.

@@ -98,7 +98,7 @@ def test_abi_refuses_bad_problems_before_touching_a_pointer(kw, code):
     d = _desc(**kw)
     assert lib.dw_log_probs_workspace_bytes(d) == code
     assert lib.dw_log_probs_fwd(d, None, None, None, None, None, None, None, None, 0, None) == code
-    assert lib.dw_log_probs_bwd(d, None, None, None, None, None, None, None, None) == code
+    assert lib.dw_log_probs_bwd(d, None, None, None, None, None, None, None) == code
     assert lib.dw_distill_workspace_bytes(d) == code
     assert lib.dw_distill_fwd(d, None, None, None, None, None, None, 0, None) == code
     assert lib.dw_distill_bwd(d, None, None, None, None, None, None, None) == code
@@ -112,9 +112,9 @@ def test_abi_refuses_null_pointers_small_workspaces_and_misfit_lists():
     assert lib.dw_log_probs_fwd(d, None, x, x, x, x, x, x, None, 0, None) == -1
     assert lib.dw_log_probs_fwd(d, x, None, x, x, x, x, x, None, 0, None) == -1      # log_prob without an index
     assert lib.dw_log_probs_fwd(d, x, x, x, x, None, x, x, None, 0, None) == -1      # entries without their outputs
-    assert lib.dw_log_probs_bwd(d, x, x, None, x, x, x, x, None) == -1
-    assert lib.dw_log_probs_bwd(d, x, x, x, None, x, x, x, None) == -1               # entropy's gradient needs the entropy
-    assert lib.dw_log_probs_bwd(d, x, None, x, x, x, None, x, None) == -1
+    assert lib.dw_log_probs_bwd(d, x, x, None, x, x, x, None) == -1
+    assert lib.dw_log_probs_bwd(d, x, None, x, x, None, x, None) == -1               # its gradient without an index
+    assert lib.dw_log_probs_bwd(d, x, x, x, x, x, None, None) == -1
     assert lib.dw_distill_fwd(d, x, x, None, x, x, None, 0, None) == -1
     assert lib.dw_distill_bwd(d, x, x, x, None, x, x, None) == -1
     assert lib.dw_log_probs_workspace_bytes(_desc(classes=1, entries=2)) == -2       # more top classes than classes

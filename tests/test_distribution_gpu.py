@@ -541,13 +541,13 @@ def test_bytes_outside_the_outputs_are_left_alone(outer, V, inner, last, dtype):
                         _lib.DW_DIST_INDEX64 | (_lib.DW_DIST_LAST if last else 0))
     nb = max(lib.dw_log_probs_workspace_bytes(C.byref(d)), lib.dw_distill_workspace_bytes(C.byref(d)), 0)
     ws = torch.full((nb + 512,), 171, dtype=torch.uint8, device="cuda")
-    lp, ent, stats, s4 = out(rows, torch.float32, 55.0), out(rows, torch.float32, 55.0), out(2 * rows, torch.float32, 55.0), out(4 * rows, torch.float32, 55.0)
+    lp, ent, stats, s4 = out(rows, torch.float32, 55.0), out(rows, torch.float32, 55.0), out(3 * rows, torch.float32, 55.0), out(4 * rows, torch.float32, 55.0)
     tlp, tix, g = out(rows * k, torch.float32, 55.0), out(rows * k, torch.int32, -9), out(rows * V, td, 55.0)
     assert lib.dw_log_probs_fwd(C.byref(d), at(x), idx.data_ptr(), at(lp), at(ent), at(tlp), at(tix), at(stats),
                                 ws.data_ptr(), nb, st) == 0
     up = torch.ones(rows, device="cuda")
-    assert lib.dw_log_probs_bwd(C.byref(d), at(x), idx.data_ptr(), at(stats), at(ent), up.data_ptr(), up.data_ptr(), at(g), st) == 0
-    for t, n, f in ((lp, rows, 55.0), (ent, rows, 55.0), (stats, 2 * rows, 55.0), (tlp, rows * k, 55.0), (tix, rows * k, -9), (g, rows * V, 55.0)):
+    assert lib.dw_log_probs_bwd(C.byref(d), at(x), idx.data_ptr(), at(stats), up.data_ptr(), up.data_ptr(), at(g), st) == 0
+    for t, n, f in ((lp, rows, 55.0), (ent, rows, 55.0), (stats, 3 * rows, 55.0), (tlp, rows * k, 55.0), (tix, rows * k, -9), (g, rows * V, 55.0)):
         check(t, n, f)
     ti = tix[guard:-guard].long().contiguous()
     tv = tlp[guard:-guard].contiguous()
