@@ -2,12 +2,14 @@
 // entropy and the top alternatives, and distillation from a teacher's listed classes; forward and
 // backward, for float32, bfloat16 and float16 logits.
 //
-// Per row, with z_j = scale * x_j and everything in base 2 (c = |scale| * log2 e, v_j = sign(scale) * x_j):
-//   m = max v_j,  t_j = (v_j - m) c,  e_j = 2^t_j,  s = sum e_j,  w = sum e_j t_j
+// Per row, with z_j = scale * x_j and everything in base 2 (c = scale * log2 e):
+//   m = the x_j of the largest z_j,  t_j = (x_j - m) c,  e_j = 2^t_j,  s = sum e_j,  w = sum e_j t_j
 //   log p_j = ln2 t_j - ln s,   entropy = ln s - ln2 w / s
-// one pass over the data with a running (m, s, w): when the maximum moves by d = (m_old - m_new) c,
-// s <- s 2^d and w <- 2^d (w + s d).  The difference v_j - m is taken before the product, so rows
-// at the end of the float32 range (all classes at the type's lowest value) keep their meaning.
+// one pass over the data with a running (m, s, w): when the extremum moves by d = (m_old - m_new) c,
+// s <- s 2^d and w <- 2^d (w + s d).  The difference x_j - m is taken before the product, so rows
+// at the end of the float32 range (all classes at the type's lowest value) keep their meaning.  A
+// negative scale (costs) needs no sign change of the data: m is the smallest x_j then, c is negative,
+// and `far`, the x of an impossible class, is +inf.
 //
 // Two families of kernels:
 //   tile  one thread a row, 64 rows a wave; the waves of a block share the classes of their 64 rows.
@@ -28,61 +30,165 @@ constexpr float kLog2e = 0x1.715476p+0f;   // fl(log2 e)
 constexpr float kFloor = -1e30f;           // stands in for an exponent of -inf where 0 * -inf would be NaN
 constexpr int kMaxEntries = 64;
 
-// mark(e): a NaN that names entry e of a teacher's list; marked(): that entry, 64 for any other value.
-// (A NaN of the caller's may look the same: whoever reads a mark compares the entries' classes.)
 // ---- element types -------------------------------------------------------------------------
 struct F32 {
   using S = float;
   static constexpr int VEC = 4;
   static __device__ __forceinline__ float up(float v) { return v; }
   static __device__ __forceinline__ float down(float v) { return v; }
-  static __device__ __forceinline__ float mark(int e) { return __builtin_bit_cast(float, 0xffc00000u | (unsigned)e); }
-  static __device__ __forceinline__ int marked(float v) {
-    const unsigned b = __builtin_bit_cast(unsigned, v);
-    return (b & ~63u) == 0xffc00000u ? (int)(b & 63u) : 64;
-  }
 };
 struct BF16 {
   using S = uint16_t;
   static constexpr int VEC = 8;
   static __device__ __forceinline__ float up(uint16_t v) { return __builtin_bit_cast(float, (unsigned)v << 16); }
   static __device__ __forceinline__ uint16_t down(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
-  static __device__ __forceinline__ uint16_t mark(int e) { return (uint16_t)(0xffc0 | e); }
-  static __device__ __forceinline__ int marked(uint16_t v) { return (v & ~63) == 0xffc0 ? (v & 63) : 64; }
+  static __device__ __forceinline__ float lower(unsigned d) { return __builtin_bit_cast(float, d << 16); }
+  static __device__ __forceinline__ float upper(unsigned d) { return __builtin_bit_cast(float, d & 0xffff0000u); }
 };
 struct F16 {
   using S = uint16_t;
   static constexpr int VEC = 8;
   static __device__ __forceinline__ float up(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
   static __device__ __forceinline__ uint16_t down(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
-  static __device__ __forceinline__ uint16_t mark(int e) { return (uint16_t)(0xff40 | e); }
-  static __device__ __forceinline__ int marked(uint16_t v) { return (v & ~63) == 0xff40 ? (v & 63) : 64; }
+  static __device__ __forceinline__ float lower(unsigned d) { return up((uint16_t)d); }
+  static __device__ __forceinline__ float upper(unsigned d) { return up((uint16_t)(d >> 16)); }
 };
 
-// 16 bytes of elements at any element-aligned address (gfx950 loads and stores them unaligned)
+// 16 bytes of elements, kept as the four words they are loaded as: taken apart at the load, they would have
+// to be waited for there
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 template <class T>
 struct Vec {
-  typename T::S e[T::VEC];
+  u32x4 d;
+  __device__ __forceinline__ float get(int e) const {
+    const unsigned w = d[T::VEC == 4 ? e : e / 2];  // (a bit_cast of d[e] itself always takes the first element)
+    if constexpr (T::VEC == 4) return __builtin_bit_cast(float, w);
+    else return e & 1 ? T::upper(w) : T::lower(w);
+  }
+  __device__ __forceinline__ void put(const float* v) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if constexpr (T::VEC == 4) d[w] = __builtin_bit_cast(unsigned, v[w]);
+      else d[w] = (unsigned)T::down(v[2 * w]) | (unsigned)T::down(v[2 * w + 1]) << 16;
+    }
+  }
 };
+// at any element-aligned address (gfx950 loads and stores 16 bytes unaligned); `at` counts bytes, so that the
+// address is a scalar base and one 32-bit lane offset
 template <class T>
-__device__ __forceinline__ Vec<T> load_vec(const typename T::S* p) {
+__device__ __forceinline__ Vec<T> load_vec(const typename T::S* base, unsigned at) {
   Vec<T> r;
-  __builtin_memcpy(&r, p, 16);
+  __builtin_memcpy(&r.d, (const char*)base + at, 16);
   return r;
 }
 template <class T>
-__device__ __forceinline__ void store_vec(typename T::S* p, const Vec<T>& v) {
-  __builtin_memcpy(p, &v, 16);
+__device__ __forceinline__ void store_vec(typename T::S* base, unsigned at, const Vec<T>& v) {
+  __builtin_memcpy((char*)base + at, &v.d, 16);
+}
+template <class S>
+__device__ __forceinline__ S& at_byte(S* base, unsigned at) { return *(S*)((char*)base + at); }
+template <class S>
+__device__ __forceinline__ const S& at_byte(const S* base, unsigned at) { return *(const S*)((const char*)base + at); }
+// the first `n` of a vector's elements (n < VEC; the others repeat the last one, nothing behind it is read)
+template <class T>
+__device__ __forceinline__ Vec<T> load_some(const typename T::S* base, unsigned at, int n) {
+  using S = typename T::S;
+  Vec<T> r;
+  S e[T::VEC];
+#pragma unroll
+  for (int i = 0; i < T::VEC; ++i) e[i] = n > 0 ? at_byte(base, at + (unsigned)(min(i, n - 1) * (int)sizeof(S))) : S(0);
+  __builtin_memcpy(&r.d, e, 16);
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void store_some(typename T::S* base, unsigned at, int n, const Vec<T>& v) {
+  using S = typename T::S;
+  S e[T::VEC];
+  __builtin_memcpy(e, &v.d, 16);
+#pragma unroll
+  for (int i = 0; i < T::VEC; ++i)
+    if (i < n) at_byte(base, at + (unsigned)(i * (int)sizeof(S))) = e[i];
 }
 
-// v_max_f32 without the canonicalisation the compiler puts before fmaxf of loaded values; a quiet
+// v_max_f32 / v_min_f32 without the canonicalisation the compiler puts before fmaxf of loaded values; a quiet
 // NaN operand gives the other one (the sum carries the NaN)
 __device__ __forceinline__ float vmax(float a, float b) {
   float r;
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
   return r;
 }
+__device__ __forceinline__ float vmin(float a, float b) {
+  float r;
+  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float vmax3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float vmin3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// Which way the logits count (the same in every lane)
+struct Side {
+  bool neg;
+  float c;     // scale * log2 e
+  float sign;  // of the scale
+  __device__ __forceinline__ float far() const { return neg ? kInf : -kInf; }
+  __device__ __forceinline__ float best(float a, float b) const { return neg ? vmin(a, b) : vmax(a, b); }
+  template <int N>
+  __device__ __forceinline__ float best_of(const float (&v)[N]) const {
+    float m;
+    if (neg) {
+      m = vmin(v[0], v[1]);
+#pragma unroll
+      for (int i = 2; i < N; i += 2) m = vmin3(m, v[i], v[i + 1]);
+    } else {
+      m = vmax(v[0], v[1]);
+#pragma unroll
+      for (int i = 2; i < N; i += 2) m = vmax3(m, v[i], v[i + 1]);
+    }
+    return m;
+  }
+};
 __device__ __forceinline__ float exp2_(float t) { return __builtin_amdgcn_exp2f(t); }
+
+// Hides where a value comes from, so that addresses are formed from it where they are used, not kept in a
+// register pair each across the loop
+__device__ __forceinline__ unsigned fresh(unsigned v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+__device__ __forceinline__ int64_t fresh_uniform(int64_t v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+// a plane's start, to be used with a 32-bit lane offset (without this the compiler adds the lane's offset to
+// the tensor's start once and then 64 bits to that for every plane, in vector registers)
+template <class S>
+using Global = __attribute__((address_space(1))) S*;
+template <class P>
+__device__ __forceinline__ P scalar_base(P p) {
+  asm volatile("" : "+s"(p));
+  return p;
+}
+template <class S>
+using GlobalBytes = std::conditional_t<std::is_const_v<S>, const __attribute__((address_space(1))) char*,
+                                       __attribute__((address_space(1))) char*>;
+template <class S>
+__device__ __forceinline__ Global<S> at_byte(Global<S> base, unsigned at) {
+  return (Global<S>)((GlobalBytes<S>)base + at);
+}
+// keeps a branch that is hardly ever taken a branch
+__device__ __forceinline__ void rare() { asm volatile(""); }
+// Keeps the compiler from computing all 32 intermediate values at once (it would spill): nothing moves over
+// every eighth value
+__device__ __forceinline__ void fence_schedule(int i) {
+  if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+}
 
 // ---- running soft-max ------------------------------------------------------------------------
 struct Acc {
@@ -91,44 +197,50 @@ struct Acc {
 using Stats3 = Acc;  // what the backward pass gets of a row; m is 0 in an empty one
 // entropy = ln s - ln2 w / s: both terms are >= 0, nothing cancels
 __device__ __forceinline__ float entropy_of(float s, float w, float ln_s) { return s == 0.f ? 0.f : ln_s - kLn2 * w / s; }
-__device__ __forceinline__ Acc acc_empty() { return Acc{-kInf, 0.f, 0.f}; }
+__device__ __forceinline__ Acc acc_empty(const Side& z) { return Acc{z.far(), 0.f, 0.f}; }
 
 template <bool ENT, int N>
-__device__ __forceinline__ void absorb(Acc& a, const float (&v)[N], float c) {
-  float m = a.m;
-#pragma unroll
-  for (int i = 0; i < N; ++i) m = vmax(m, v[i]);
-  const float b = m == -kInf ? 0.f : m;
-  const float d = fmaxf((a.m - b) * c, kFloor), al = exp2_(d);
+__device__ __forceinline__ void absorb(Acc& a, const float (&v)[N], float top, const Side& z) {  // top: best_of(v)
+  const float m = z.best(a.m, top);
+  const float b = m == z.far() ? 0.f : m;
+  const float d = fmaxf((a.m - b) * z.c, kFloor), al = exp2_(d);
   if (ENT) a.w = al * fmaf(a.s, d, a.w);
   a.s *= al;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float t = (v[i] - b) * c, e = exp2_(t);
-    a.s += e;
-    if (ENT) a.w = fmaf(e, vmax(t, kFloor), a.w);
+  for (int i = 0; i < N; i += 8) {
+    float t[8], e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = (v[i + k] - b) * z.c;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = exp2_(t[k]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      a.s += e[k];
+      if (ENT) a.w = fmaf(e[k], vmax(t[k], kFloor), a.w);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
   a.m = m;
 }
-__device__ __forceinline__ Acc acc_join(const Acc& a, const Acc& b, float c) {
-  const float m = vmax(a.m, b.m), o = m == -kInf ? 0.f : m;
-  const float da = fmaxf((a.m - o) * c, kFloor), db = fmaxf((b.m - o) * c, kFloor);
+__device__ __forceinline__ Acc acc_join(const Acc& a, const Acc& b, const Side& z) {
+  const float m = z.best(a.m, b.m), o = m == z.far() ? 0.f : m;
+  const float da = fmaxf((a.m - o) * z.c, kFloor), db = fmaxf((b.m - o) * z.c, kFloor);
   const float ea = exp2_(da), eb = exp2_(db);
   return Acc{m, a.s * ea + b.s * eb, ea * fmaf(a.s, da, a.w) + eb * fmaf(b.s, db, b.w)};
 }
 __device__ __forceinline__ float shfl_xor(float v, int mask) { return __shfl_xor(v, mask, 64); }
-__device__ __forceinline__ Acc acc_wave(Acc a, float c) {
+__device__ __forceinline__ Acc acc_wave(Acc a, const Side& z) {
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) {
     Acc b{shfl_xor(a.m, k), shfl_xor(a.s, k), shfl_xor(a.w, k)};
     // both lanes of a pair evaluate the same expression (lower lane's sums first): one result everywhere
-    a = (threadIdx.x & k) ? acc_join(b, a, c) : acc_join(a, b, c);
+    a = (threadIdx.x & k) ? acc_join(b, a, z) : acc_join(a, b, z);
   }
   return a;
 }
-__device__ __forceinline__ float wave_max_all(float v) {
+__device__ __forceinline__ float wave_best_all(float v, const Side& z) {
 #pragma unroll
-  for (int k = 1; k < 64; k <<= 1) v = vmax(v, shfl_xor(v, k));
+  for (int k = 1; k < 64; k <<= 1) v = z.best(v, shfl_xor(v, k));
   return v;
 }
 __device__ __forceinline__ float wave_sum_all(float v) {
@@ -137,11 +249,11 @@ __device__ __forceinline__ float wave_sum_all(float v) {
   return v;
 }
 
-// log p of a class of value v in a row of (m, ln s): -inf for a masked class, also where the whole row
-// is masked (ln s = -inf); NaN where the row holds NaN or +inf
+// log p of a class of value x in a row of (m, ln s): -inf for an impossible class, also where the whole row
+// is impossible (ln s = -inf); NaN where the row holds NaN or z = +inf
 // (in base e: in base 2 the log-probability of a class at float32's lowest value would overflow)
-__device__ __forceinline__ float log_p(float v, float m, float ln_s, float scale) {
-  return (v == -kInf && ln_s == ln_s) ? -kInf : fmaf(v - m, fabsf(scale), -ln_s);
+__device__ __forceinline__ float log_p(float x, float m, float ln_s, float scale) {
+  return (x * scale == -kInf && fabsf(x) == kInf && ln_s == ln_s) ? -kInf : fmaf(x - m, scale, -ln_s);
 }
 
 // ---- order keys --------------------------------------------------------------------------------
@@ -158,30 +270,25 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)(0xffffffffu - (unsigned)k); }
 
-// The same order as a float64, so that a comparator is one v_max_f64 and one v_min_f64 (full rate on
-// this chip): the value in the upper bits, the index in the 29 mantissa bits a converted float32
-// leaves empty, complemented for positive values.  Infinities and NaN become finite values beyond
-// every float32.
-constexpr double kKeyInf = 0x1p+200, kKeyNan = 0x1p+300, kKeyNone = -0x1p+400;
-__device__ __forceinline__ double key_f64(float v, int idx) {
-  double d = (double)(v + 0.f);
-  if (!(fabsf(v) < kInf)) d = v != v ? kKeyNan : (v > 0.f ? kKeyInf : -kKeyInf);
-  unsigned long long b = __builtin_bit_cast(unsigned long long, d);
-  const unsigned low = (b >> 63) ? (unsigned)idx : (0x1fffffffu - (unsigned)idx);
-  return __builtin_bit_cast(double, b | low);
+// The same order as a float64, so that a comparator is one v_max_f64 and one v_min_f64: the upper word is
+// the value as it is (the bits of a float32 read as the upper half of a float64 keep their order, and
+// infinities stay finite numbers there), the lower word the index, complemented for positive values.
+// v must not be NaN; key_of_nan() puts one above +inf, as a number.
+constexpr double kKeyNone = __builtin_bit_cast(double, 0xff90000000000000ull);  // below -inf of any index
+__device__ __forceinline__ double key_f64(float v, float sign, int idx) {  // of sign * v
+  const unsigned hi = __builtin_bit_cast(unsigned, fmaf(v, sign, 0.f));  // -0 counts as 0
+  const unsigned lo = (unsigned)((int)hi >> 31) ^ ~(unsigned)idx;
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double key_of_nan(int idx) {
+  return __builtin_bit_cast(double, 0x7fc00000ull << 32 | ~(unsigned)idx);
 }
 __device__ __forceinline__ float key_f64_value(double k) {
-  const unsigned long long b = __builtin_bit_cast(unsigned long long, k) & ~0x1fffffffull;
-  const double d = __builtin_bit_cast(double, b);
-  if (d >= kKeyNan) return __builtin_nanf("");
-  if (d >= kKeyInf) return kInf;
-  if (d <= -kKeyInf) return -kInf;
-  return (float)d;
+  return __builtin_bit_cast(float, (unsigned)(__builtin_bit_cast(unsigned long long, k) >> 32));
 }
 __device__ __forceinline__ int key_f64_index(double k) {
   const unsigned long long b = __builtin_bit_cast(unsigned long long, k);
-  const int low = (int)(b & 0x1fffffffull);
-  return (b >> 63) ? low : 0x1fffffff - low;
+  return (int)((unsigned)((long long)b >> 63) ^ ~(unsigned)b);
 }
 __device__ __forceinline__ double max64(double a, double b) {
   double r;
@@ -233,6 +340,10 @@ struct Prob {
   float scale, c;
   int flags;
 };
+__device__ __forceinline__ Side side(const Prob& p) {
+  const bool neg = __builtin_bit_cast(int, p.scale) < 0;
+  return Side{neg, p.c, neg ? -1.f : 1.f};
+}
 constexpr int kIdx64 = DW_DIST_INDEX64, kRenorm = DW_DIST_RENORMALISE;
 
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t at, int flags) {
@@ -247,11 +358,12 @@ __device__ __forceinline__ float load_teacher(const void* p, int64_t at, int fla
 
 // ---- tile kernels: where the 64 rows of a block are, and how their classes come in -----------------
 struct Place {
-  int64_t row;    // this lane's row, clamped to the last one
+  int64_t row;    // this lane's row (planes: the last pixel again behind the end)
   int64_t o, i;   // its outer and inner index
   int64_t first;  // first row (LAST) or first pixel (planes) of the block
   int lane, wave;
-  bool live;      // the row exists
+  int skip;       // LAST: so many of the block's first rows belong to the block before
+  bool live;      // this lane's row is the block's to write
 };
 template <bool LAST>
 __device__ __forceinline__ Place place(const Prob& p) {
@@ -259,10 +371,13 @@ __device__ __forceinline__ Place place(const Prob& p) {
   q.lane = threadIdx.x & 63;
   q.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (LAST) {
-    q.first = (int64_t)blockIdx.x * 64;
+    // the last block starts 64 rows before the end (there are at least 64) and leaves the ones before its
+    // own to their block
+    const int64_t own = (int64_t)blockIdx.x * 64;
+    q.first = own + 64 <= p.rows ? own : p.rows - 64;
+    q.skip = (int)(own - q.first);
     q.row = q.first + q.lane;
-    q.live = q.row < p.rows;
-    if (!q.live) q.row = p.rows - 1;
+    q.live = q.lane >= q.skip;
     q.o = p.inner == 1 ? q.row : q.row / p.inner;
     q.i = p.inner == 1 ? 0 : q.row - q.o * p.inner;
   } else {
@@ -295,46 +410,85 @@ constexpr int kStageBytes = 64 * kRowBytes;
 template <class T, bool LAST>
 constexpr int stage_classes() { return LAST ? kSegBytes / (int)sizeof(typename T::S) : 32; }
 
-// 64 row segments of classes [c0, c0 + n) into LDS (n <= stage_classes); 8 lanes a row
+// The next stage on its way: loads are issued a stage ahead, while the one before is worked on.
+template <class T, bool LAST>
+struct Feed;
 template <class T>
-__device__ __forceinline__ void stage_in(const typename T::S* x, const Prob& p, const Place& q, int c0, int n,
-                                         char* lds) {
-  constexpr int PER = kSegBytes / 16;
-  const int seg = q.lane % PER, j = seg * T::VEC;
+struct Feed<T, true> {  // 64 row segments of classes [c0, c0 + n), 8 lanes a row
+  static constexpr int PER = kSegBytes / 16;
   Vec<T> v[PER];
+  __device__ __forceinline__ void issue(const typename T::S* x, const Prob& p, const Place& q, int c0, int n) {
+    using S = typename T::S;
+    const int j = q.lane % PER * T::VEC;
+    const unsigned at = fresh((unsigned)(q.lane / PER * p.V + j) * (unsigned)sizeof(S));
+    int64_t off = q.first * p.V + c0;
+    if (n == kSegBytes / (int)sizeof(S)) {
 #pragma unroll
-  for (int it = 0; it < PER; ++it) {
-    const int64_t row = min(q.first + it * (64 / PER) + q.lane / PER, p.rows - 1);
-    const typename T::S* src = x + row * p.V + c0 + j;
-    if (j + T::VEC <= n) {
-      v[it] = load_vec<T>(src);
+      for (int it = 0; it < PER; ++it) {
+        v[it] = load_vec<T>(x + off, at);
+        off = fresh_uniform(off + (64 / PER) * p.V);
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < T::VEC; ++e) v[it].e[e] = j + e < n ? src[e] : typename T::S(0);
+      for (int it = 0; it < PER; ++it) {
+        if (j + T::VEC <= n) v[it] = load_vec<T>(x + off, at);
+        else v[it] = load_some<T>(x + off, at, n - j);
+        off = fresh_uniform(off + (64 / PER) * p.V);
+      }
     }
   }
+  __device__ __forceinline__ void to_lds(const Place& q, char* lds) const {
 #pragma unroll
-  for (int it = 0; it < PER; ++it)
-    *(Vec<T>*)(lds + (it * (64 / PER) + q.lane / PER) * kRowBytes + seg * 16) = v[it];
-}
+    for (int it = 0; it < PER; ++it)
+      *(Vec<T>*)(lds + (it * (64 / PER) + q.lane / PER) * kRowBytes + q.lane % PER * 16) = v[it];
+  }
+};
+template <class T>
+struct Feed<T, false> {  // 32 planes from class c0 on; the planes behind the n-th repeat it
+  typename T::S v[32];
+  __device__ __forceinline__ void issue(const typename T::S* x, const Prob& p, const Place& q, int c0, int n) {
+    using S = typename T::S;
+    Global<const S> plane = (Global<const S>)(x + (q.o * p.V + c0) * p.inner + q.first);
+    const unsigned at = fresh((unsigned)(q.i - q.first) * (unsigned)sizeof(S));
+    if (n == 32) {
+#pragma unroll
+      for (int u = 0; u < 32; ++u) {
+        plane = scalar_base(plane);
+        v[u] = *at_byte<const S>(plane, at);
+        plane += p.inner;
+      }
+    } else {
+      const int last = (int)fresh_uniform(n) - 1;
+#pragma unroll
+      for (int u = 0; u < 32; ++u) {
+        plane = scalar_base(plane);
+        v[u] = *at_byte<const S>(plane, at);
+        plane += u < last ? p.inner : 0;
+      }
+    }
+  }
+  __device__ __forceinline__ void take(float (&f)[32]) const {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) f[u] = T::up(v[u]);
+  }
+};
 template <class T>
 __device__ __forceinline__ void stage_out(typename T::S* g, const Prob& p, const Place& q, int c0, int n,
                                           const char* lds) {
+  using S = typename T::S;
   constexpr int PER = kSegBytes / 16;
-  const int seg = q.lane % PER, j = seg * T::VEC;
+  const int j = q.lane % PER * T::VEC;
+  const unsigned at = fresh((unsigned)(q.lane / PER * p.V + j) * (unsigned)sizeof(S));
+  int64_t off = q.first * p.V + c0;
 #pragma unroll
   for (int it = 0; it < PER; ++it) {
     const int r = it * (64 / PER) + q.lane / PER;
-    if (q.first + r >= p.rows) continue;
-    const Vec<T> v = *(const Vec<T>*)(lds + r * kRowBytes + seg * 16);
-    typename T::S* dst = g + (q.first + r) * p.V + c0 + j;
-    if (j + T::VEC <= n) {
-      store_vec<T>(dst, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < T::VEC; ++e)
-        if (j + e < n) dst[e] = v.e[e];
+    if (r >= q.skip) {
+      const Vec<T> v = *(const Vec<T>*)(lds + r * kRowBytes + q.lane % PER * 16);
+      if (j + T::VEC <= n) store_vec<T>(g + off, at, v);
+      else store_some<T>(g + off, at, n - j, v);
     }
+    off = fresh_uniform(off + (64 / PER) * p.V);
   }
 }
 // 32 classes of this lane's row from the stage, from class h of the segment on
@@ -344,7 +498,7 @@ __device__ __forceinline__ void stage_read(const char* lds, int lane, int h, flo
   for (int u = 0; u < 32 / T::VEC; ++u) {
     const Vec<T> w = *(const Vec<T>*)(lds + lane * kRowBytes + h * (int)sizeof(typename T::S) + u * 16);
 #pragma unroll
-    for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = T::up(w.e[e]);
+    for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = w.get(e);
   }
 }
 template <class T>
@@ -352,29 +506,40 @@ __device__ __forceinline__ void stage_write(char* lds, int lane, int h, const fl
 #pragma unroll
   for (int u = 0; u < 32 / T::VEC; ++u) {
     Vec<T> w;
-#pragma unroll
-    for (int e = 0; e < T::VEC; ++e) w.e[e] = T::down(v[u * T::VEC + e]);
+    w.put(v + u * T::VEC);
     *(Vec<T>*)(lds + lane * kRowBytes + h * (int)sizeof(typename T::S) + u * 16) = w;
   }
 }
-// 32 planes from class c0 on; the planes behind the n-th repeat it
 template <class T>
-__device__ __forceinline__ void planes_in(const typename T::S* x, const Prob& p, const Place& q, int c0, int n,
-                                          float (&v)[32]) {
-  const typename T::S* base = x + (q.o * p.V + c0) * p.inner + q.first;
-  const unsigned at = (unsigned)(q.i - q.first);
+__device__ __forceinline__ void planes_out(typename T::S* g, const Prob& p, const Place& q, int c0, int n,
+                                           const float (&v)[32]) {
+  using S = typename T::S;
+  Global<S> plane = (Global<S>)(g + (q.o * p.V + c0) * p.inner + q.first);
+  const unsigned at = fresh((unsigned)(q.i - q.first) * (unsigned)sizeof(S));
+  if (!q.live) return;
+  if (n == 32) {
 #pragma unroll
-  for (int u = 0; u < 32; ++u) v[u] = T::up((base + (int64_t)min(u, n - 1) * p.inner)[at]);
-}
-// z's sign, and -inf behind the n-th class
-__device__ __forceinline__ void settle(float (&v)[32], bool neg, int n) {
-  if (neg) {
+    for (int u = 0; u < 32; ++u) {
+      plane = scalar_base(plane);
+      *at_byte<S>(plane, at) = T::down(v[u]);
+      plane += p.inner;
+    }
+  } else {
+    const int m = (int)fresh_uniform(n);
 #pragma unroll
-    for (int u = 0; u < 32; ++u) v[u] = -v[u];
+    for (int u = 0; u < 32; ++u) {
+      plane = scalar_base(plane);
+      if (u < m) *at_byte<S>(plane, at) = T::down(v[u]);
+      plane += p.inner;
+    }
   }
+}
+// nothing possible behind the n-th class
+__device__ __forceinline__ void settle(float (&v)[32], float far, int n) {
   if (n < 32) {
+    n = (int)fresh_uniform(n);
 #pragma unroll
-    for (int u = 0; u < 32; ++u) v[u] = u < n ? v[u] : -kInf;
+    for (int u = 0; u < 32; ++u) v[u] = u < n ? v[u] : far;
   }
 }
 
@@ -392,42 +557,53 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   char* joint = smem + (LAST ? nw * kStageBytes : 0);
   float* red = (float*)joint;                                      // [3][nw][64]
   double* keys = (double*)(joint + 3 * nw * 64 * sizeof(float));   // [nw][K][64]
-  const bool neg = p.scale < 0.f;
+  constexpr int CH = stage_classes<T, LAST>();
+  const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
 
-  Acc a = acc_empty();
+  Acc a = acc_empty(z);
   double limit = 0.0;
   float ln_s = 0.f, base = 0.f;
   for (int done = 0; done == 0 || done < p.k; done += (K ? K : 1)) {
     double top[K ? K : 1];
 #pragma unroll
     for (int i = 0; i < K; ++i) top[i] = kKeyNone;
-    for (int c0 = c_lo; c0 < c_hi; c0 += stage_classes<T, LAST>()) {
-      const int n = min(stage_classes<T, LAST>(), c_hi - c0);
-      if (LAST) {
+    Feed<T, LAST> feed;
+    if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
+    for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
+      const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
+      float v[32];
+      if constexpr (LAST) {
         wave_sync();
-        stage_in<T>(x, p, q, c0, n, stage);
+        feed.to_lds(q, stage);
         wave_sync();
+      } else {
+        feed.take(v);
       }
+      if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
       for (int h = 0; h < n; h += 32) {
-        float v[32];
-        if (LAST)
-          stage_read<T>(stage, q.lane, h, v);
-        else
-          planes_in<T>(x, p, q, c0, n, v);
-        settle(v, neg, n - h);
-        if (done == 0) absorb<true>(a, v, p.c);
+        if (LAST) stage_read<T>(stage, q.lane, h, v);
+        settle(v, z.far(), n - h);
+        if (done == 0) absorb<true>(a, v, z.best_of(v), z);
         if constexpr (K > 0) {
+          const bool nan = __any(a.s != a.s);  // NaN or +inf in some row
 #pragma unroll
           for (int g = 0; g < 32; g += K) {
             double nk[K];
 #pragma unroll
-            for (int i = 0; i < K; ++i) {
-              nk[i] = key_f64(v[g + i], c0 + h + g + i);
-              if (done > 0 && !(nk[i] < limit)) nk[i] = kKeyNone;
+            for (int i = 0; i < K; ++i) nk[i] = key_f64(v[g + i], z.sign, c0 + h + g + i);
+            if (nan) {
+              rare();
+#pragma unroll
+              for (int i = 0; i < K; ++i) nk[i] = v[g + i] != v[g + i] ? key_of_nan(c0 + h + g + i) : nk[i];
+            }
+            if (done > 0) {
+#pragma unroll
+              for (int i = 0; i < K; ++i) nk[i] = nk[i] < limit ? nk[i] : kKeyNone;
             }
             sort_desc<K>(nk);
             merge_desc<K>(top, nk);
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
@@ -445,7 +621,7 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
       if (done == 0) {
         a = Acc{red[q.lane], red[nw * 64 + q.lane], red[2 * nw * 64 + q.lane]};
         for (int w = 1; w < nw; ++w)
-          a = acc_join(a, Acc{red[w * 64 + q.lane], red[(nw + w) * 64 + q.lane], red[(2 * nw + w) * 64 + q.lane]}, p.c);
+          a = acc_join(a, Acc{red[w * 64 + q.lane], red[(nw + w) * 64 + q.lane], red[(2 * nw + w) * 64 + q.lane]}, z);
       }
       if constexpr (K > 0) {
 #pragma unroll
@@ -460,14 +636,14 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
       __syncthreads();
     }
     if (done == 0) {
-      base = a.m == -kInf ? 0.f : a.m;
+      base = a.m == z.far() ? 0.f : a.m;
       ln_s = logf(a.s);
       if (q.wave == 0 && q.live) {
         const int t = index ? valid_index(load_index(index, q.row, p.flags), p.V) : -1;
         float lp = 0.f;
         if (t >= 0) {
           const float v = T::up(x[element<LAST>(p, q, t)]);
-          lp = log_p(neg ? -v : v, base, ln_s, p.scale);
+          lp = log_p(v, base, ln_s, p.scale);
         }
         if (log_prob) log_prob[q.row] = lp;
         if (entropy) entropy[q.row] = entropy_of(a.s, a.w, ln_s);
@@ -480,7 +656,7 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
 #pragma unroll
         for (int i = 0; i < K; ++i) {
           if (done + i < p.k) {
-            const float v = key_f64_value(top[i]);
+            const float v = key_f64_value(top[i]) * z.sign;
             const int64_t at = LAST ? q.row * p.k + done + i : (q.o * p.k + done + i) * p.inner + q.i;
             top_lp[at] = log_p(v, base, ln_s, p.scale);
             top_idx[at] = key_f64_index(top[i]);
@@ -526,27 +702,33 @@ __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
   extern __shared__ __align__(16) char smem[];
   const Place q = place<LAST>(p);
   char* stage = smem + q.wave * kStageBytes;
-  const bool neg = p.scale < 0.f;
+  const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
   const LpCoef r = lp_coef<ENT>(p, q.row, index, stats, g_lp, g_ent);
   const bool any_dead = __any(r.dead);
-  for (int c0 = c_lo; c0 < c_hi; c0 += stage_classes<T, LAST>()) {
-    const int n = min(stage_classes<T, LAST>(), c_hi - c0);
-    if (LAST) {
+  constexpr int CH = stage_classes<T, LAST>();
+  Feed<T, LAST> feed;
+  if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
+  for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
+    const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
+    float v[32];
+    if constexpr (LAST) {
       wave_sync();
-      stage_in<T>(x, p, q, c0, n, stage);
+      feed.to_lds(q, stage);
       wave_sync();
+    } else {
+      feed.take(v);
     }
+    if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
     for (int h = 0; h < n; h += 32) {
-      float v[32];
-      if (LAST)
-        stage_read<T>(stage, q.lane, h, v);
-      else
-        planes_in<T>(x, p, q, c0, n, v);
-      settle(v, neg, n - h);
+      if (LAST) stage_read<T>(stage, q.lane, h, v);
+      settle(v, z.far(), n - h);
       const int rel = r.target - c0 - h;
 #pragma unroll
-      for (int u = 0; u < 32; ++u) v[u] = lp_grad<ENT>(r, v[u], p.c, rel == u ? r.hit : 0.f);
+      for (int u = 0; u < 32; ++u) {
+        v[u] = lp_grad<ENT>(r, v[u], p.c, rel == u ? r.hit : 0.f);
+        fence_schedule(u);
+      }
       if (any_dead) {
 #pragma unroll
         for (int u = 0; u < 32; ++u) v[u] = r.dead ? 0.f : v[u];
@@ -554,13 +736,7 @@ __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
       if (LAST) {
         stage_write<T>(stage, q.lane, h, v);
       } else {
-        typename T::S* dst = g + (q.o * p.V + c0) * p.inner + q.first;
-        const unsigned at = (unsigned)(q.i - q.first);
-        if (q.live) {
-#pragma unroll
-          for (int u = 0; u < 32; ++u)
-            if (u < n) (dst + (int64_t)u * p.inner)[at] = T::down(v[u]);
-        }
+        planes_out<T>(g, p, q, c0, n, v);
       }
     }
     if (LAST) {
@@ -579,7 +755,7 @@ struct RowSums {
 };
 __device__ __forceinline__ float rest_term(const RowSums& r, float scale, float rr) {
   // log of the unlisted classes' probability
-  const float lp = fmaf(r.m_r - r.b, fabsf(scale), logf(r.s_r) - r.ln_s);
+  const float lp = fmaf(r.m_r - r.b, scale, logf(r.s_r) - r.ln_s);
   return rr > 0.f ? rr * (logf(rr) - lp) : 0.f;
 }
 __device__ __forceinline__ float4 distill_stats(const RowSums& r, float c, float mass, float rr, bool alive) {
@@ -593,84 +769,103 @@ __device__ __forceinline__ float4 distill_stats(const RowSums& r, float c, float
   return st;
 }
 
-// Column of this lane's row inside the stage: planes [class][64] float32, or the row's own bytes
+// Column of this lane's row inside the stage: planes [class][64] float32, or the row's own bytes.  What a
+// lane does for a listed class that is not in the stage goes to a place of its own behind the column.
 template <class T, bool LAST>
 struct Column {
   using S = std::conditional_t<LAST, typename T::S, float>;
   using M = std::conditional_t<LAST, T, F32>;
+  static constexpr int kNowhere = LAST ? kSegBytes / (int)sizeof(S) : 32;
   char* lds;
   int lane;
   __device__ __forceinline__ S* at(int u) const {
     return LAST ? (S*)(lds + lane * kRowBytes) + u : (S*)lds + u * 64 + lane;
   }
 };
-constexpr int kPlaneStage = 32 * 64 * 4;
 template <bool LAST>
-constexpr int distill_stage_bytes() { return LAST ? kStageBytes : kPlaneStage; }
+constexpr int distill_stage_bytes() { return LAST ? kStageBytes : 33 * 64 * 4; }
+constexpr int kGroup = 8;  // entries handled at once: their LDS accesses overlap
+__host__ __device__ constexpr int padded(int k) { return (k + kGroup - 1) / kGroup * kGroup; }
+// LDS of a block besides the stages: columns of 64 lanes, of list entries and of the waves' sums
+__host__ __device__ constexpr size_t distill_lds(int nw, int k, bool backward) {
+  return (size_t)256 * (padded(k) * (backward ? 3 : 2) + 1 + (backward ? 0 : 2 * nw));
+}
+
+// The first entry before e of the same class, or e.  Asked only where a listed class was found impossible:
+// masked, or taken out for an earlier entry.
+__device__ __forceinline__ int listed_before(const int* idx, int e) {
+  const int mine = idx[e * 64];
+  for (int k = 0; k < e; ++k)
+    if (idx[k * 64] == mine) return k;
+  return e;
+}
+
+// Reads the listed classes of the stage [c0, c0 + n) out of the lane's column and leaves `far` in their
+// places (so a class listed twice reads `far` the second time); f(e, hit, value) gets what was read.
+template <class C, class F>
+__device__ __forceinline__ void take_listed(const C& col, const int* idx, int K, int c0, int n, float far, F f) {
+  for (int e0 = 0; e0 < K; e0 += kGroup) {
+    float old[kGroup];
+    bool hit[kGroup];
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const int rel = idx[(e0 + i) * 64] - c0;
+      hit[i] = (unsigned)rel < (unsigned)n;
+      typename C::S* at = col.at(hit[i] ? rel : C::kNowhere);
+      old[i] = C::M::up(*at);
+      *at = C::M::down(far);
+    }
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) f(e0 + i, hit[i], old[i]);
+  }
+}
 
 // ---- distillation, forward, tile ------------------------------------------------------------------------
 // Each listed class is taken out of its column before the running soft-max sees the column, so the
 // unlisted classes are summed on their own (1 - sum of the listed would cancel where the list holds
-// nearly everything).  A class listed twice is taken out once: a mark left in the column shows it.
+// nearly everything).
 template <class T, bool LAST>
 __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ teacher,
                             const void* __restrict__ index, float* __restrict__ loss, float4* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
   const Place q = place<LAST>(p);
-  const int nw = blockDim.x >> 6, K = p.k;
+  const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
   char* stage = smem + q.wave * distill_stage_bytes<LAST>();
   char* rest = smem + nw * distill_stage_bytes<LAST>();
-  int* idx = (int*)rest + q.lane;                  // [K][64]
-  float* xk = (float*)rest + K * 64 + q.lane;      // value of the entry's class
-  float* xs = (float*)rest + 2 * K * 64 + q.lane;  // the same, -inf where the class was listed before
-  float* red = (float*)rest + 3 * K * 64 + q.lane; // [2][nw][64]
+  int* idx = (int*)rest + q.lane;                            // [KP][64]
+  float* xs = (float*)rest + KP * 64 + q.lane;               // [KP + 1][64]: the listed classes' values
+  float* red = (float*)rest + (2 * KP + 1) * 64 + q.lane;    // [2][nw][64]
   const Column<T, LAST> col{stage, q.lane};
-  using C = Column<T, LAST>;
-  const bool neg = p.scale < 0.f;
+  constexpr int CH = stage_classes<T, LAST>();
+  const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
   const int64_t t0 = q.o * p.es[0] + q.i * p.es[2];
 
-  for (int e = q.wave; e < K; e += nw) {
-    idx[e * 64] = valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V);
-    xk[e * 64] = -kInf;
-    xs[e * 64] = -kInf;
+  for (int e = q.wave; e < KP; e += nw) {
+    idx[e * 64] = e < K ? valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V) : -1;
+    xs[e * 64] = z.far();
   }
   __syncthreads();
   bool alive = false;
   for (int e = 0; e < K; ++e) alive |= idx[e * 64] >= 0;
-  Acc a = acc_empty();
+  Acc a = acc_empty(z);
   if (__any(alive)) {  // the same in every wave of the block
-    for (int c0 = c_lo; c0 < c_hi; c0 += stage_classes<T, LAST>()) {
-      const int n = min(stage_classes<T, LAST>(), c_hi - c0);
+    Feed<T, LAST> feed;
+    if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
+    for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
+      const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
       float v[32];
       wave_sync();
-      if (LAST) {
-        stage_in<T>(x, p, q, c0, n, stage);
+      if constexpr (LAST) {
+        feed.to_lds(q, stage);
       } else {
-        planes_in<T>(x, p, q, c0, n, v);
+        feed.take(v);
 #pragma unroll
         for (int u = 0; u < 32; ++u) *(float*)col.at(u) = v[u];
       }
+      if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
       wave_sync();
-      for (int e = 0; e < K; ++e) {
-        const int rel = idx[e * 64] - c0;
-        if ((unsigned)rel < (unsigned)n) {
-          const typename C::S raw = *col.at(rel);
-          const int before = C::M::marked(raw);
-          if (before < e && idx[before * 64] == idx[e * 64]) {
-            xk[e * 64] = xk[before * 64];
-          } else {
-            const float f = neg ? -C::M::up(raw) : C::M::up(raw);
-            xk[e * 64] = f;
-            xs[e * 64] = f;
-            *col.at(rel) = C::M::mark(e);
-          }
-        }
-      }
-      for (int e = 0; e < K; ++e) {
-        const int rel = idx[e * 64] - c0;
-        if ((unsigned)rel < (unsigned)n) *col.at(rel) = C::M::down(neg ? kInf : -kInf);
-      }
+      take_listed(col, idx, K, c0, n, z.far(), [&](int e, bool hit, float old) { xs[(hit ? e : KP) * 64] = old; });
       wave_sync();
       for (int h = 0; h < n; h += 32) {
         if (LAST) {
@@ -679,8 +874,8 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
 #pragma unroll
           for (int u = 0; u < 32; ++u) v[u] = *(const float*)col.at(u);
         }
-        settle(v, neg, n - h);
-        absorb<false>(a, v, p.c);
+        settle(v, z.far(), n - h);
+        absorb<false>(a, v, z.best_of(v), z);
       }
     }
   }
@@ -689,17 +884,17 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   __syncthreads();
   if (q.wave != 0 || !q.live) return;
   a = Acc{red[0], red[nw * 64], 0.f};
-  for (int w = 1; w < nw; ++w) a = acc_join(a, Acc{red[w * 64], red[(nw + w) * 64], 0.f}, p.c);
+  for (int w = 1; w < nw; ++w) a = acc_join(a, Acc{red[w * 64], red[(nw + w) * 64], 0.f}, z);
 
   RowSums r;
   r.m_r = a.m;
   r.s_r = a.s;
   float m = a.m, tm = -kInf;
   for (int e = 0; e < K; ++e) {
-    m = vmax(m, xs[e * 64]);
+    m = z.best(m, xs[e * 64]);
     if ((p.flags & kRenorm) && idx[e * 64] >= 0) tm = fmaxf(tm, load_teacher(teacher, t0 + e * p.es[1], p.flags));
   }
-  r.b = m == -kInf ? 0.f : m;
+  r.b = m == z.far() ? 0.f : m;
   r.s = a.s * exp2_((a.m - r.b) * p.c);
   float ts = 0.f;
   for (int e = 0; e < K; ++e) {
@@ -714,7 +909,9 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
     if (idx[e * 64] < 0) continue;
     const float lq = load_teacher(teacher, t0 + e * p.es[1], p.flags) - shift, qe = expf(lq);
     mass += qe;
-    if (qe != 0.f) l = fmaf(qe, lq - log_p(xk[e * 64], r.b, r.ln_s, p.scale), l);
+    float v = xs[e * 64];
+    if (v == z.far()) v = xs[listed_before(idx, e) * 64];
+    if (qe != 0.f) l = fmaf(qe, lq - log_p(v, r.b, r.ln_s, p.scale), l);
   }
   const float rr = (alive && !(p.flags & kRenorm) && r.s_r != 0.f) ? fmaxf(1.f - mass, 0.f) : 0.f;
   if (rr > 0.f) l += rest_term(r, p.scale, rr);
@@ -729,22 +926,25 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
                             const float* __restrict__ g_loss, typename T::S* __restrict__ g) {
   extern __shared__ __align__(16) char smem[];
   const Place q = place<LAST>(p);
-  const int nw = blockDim.x >> 6, K = p.k;
+  const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
   char* stage = smem + q.wave * distill_stage_bytes<LAST>();
   char* rest = smem + nw * distill_stage_bytes<LAST>();
-  int* idx = (int*)rest + q.lane;
-  float* gq = (float*)rest + K * 64 + q.lane;      // upstream gradient * scale * teacher's probability
-  float* xk = (float*)rest + 2 * K * 64 + q.lane;  // gradient of a listed class before gq
-  unsigned long long again = 0;                    // entries whose class this wave has met in an earlier entry
+  int* idx = (int*)rest + q.lane;                    // [KP][64]
+  float* gq = (float*)rest + KP * 64 + q.lane;       // [KP][64]: upstream gradient * scale * teacher's probability
+  float* gv = (float*)rest + 2 * KP * 64 + q.lane;   // [KP + 1][64]: the listed classes' gradients
   const Column<T, LAST> col{stage, q.lane};
   using C = Column<T, LAST>;
-  const bool neg = p.scale < 0.f, renorm = p.flags & kRenorm;
+  constexpr int CH = stage_classes<T, LAST>();
+  const Side z = side(p);
+  const bool renorm = p.flags & kRenorm;
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
   const int64_t t0 = q.o * p.es[0] + q.i * p.es[2];
   const float4 st = stats[q.row];
   const float up = g_loss[q.row];
   const bool dead = up == 0.f || st.w == 0.f;
   const float gs = up * p.scale, rest_f = gs * st.y, member_f = gs * st.w;
+  Feed<T, LAST> feed;
+  if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
 
   float shift = 0.f;
   if (renorm && !dead) {
@@ -757,47 +957,44 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
         ts += expf(load_teacher(teacher, t0 + e * p.es[1], p.flags) - (tm == -kInf ? 0.f : tm));
     shift = ts == 0.f ? 0.f : tm + logf(ts);
   }
-  for (int e = q.wave; e < K; e += nw) {
-    const int i = dead ? -1 : valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V);
+  for (int e = q.wave; e < KP; e += nw) {
+    const int i = dead || e >= K ? -1 : valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V);
     idx[e * 64] = i;
     gq[e * 64] = i >= 0 ? gs * expf(load_teacher(teacher, t0 + e * p.es[1], p.flags) - shift) : 0.f;
   }
   __syncthreads();
   const bool any_dead = __any(dead);
-  for (int c0 = c_lo; c0 < c_hi; c0 += stage_classes<T, LAST>()) {
-    const int n = min(stage_classes<T, LAST>(), c_hi - c0);
+  for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
+    const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
     float v[32];
     wave_sync();
-    if (LAST) {
-      stage_in<T>(x, p, q, c0, n, stage);
+    if constexpr (LAST) {
+      feed.to_lds(q, stage);
     } else {
-      planes_in<T>(x, p, q, c0, n, v);
+      feed.take(v);
 #pragma unroll
       for (int u = 0; u < 32; ++u) *(float*)col.at(u) = v[u];
     }
+    if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
     wave_sync();
-    // listed classes: their soft-max gradient, the rest of it later; a class listed again adds its share to the first entry
-    for (int e = 0; e < K; ++e) {
-      const int rel = idx[e * 64] - c0;
-      if ((unsigned)rel < (unsigned)n) {
-        const typename C::S raw = *col.at(rel);
-        const int before = C::M::marked(raw);
-        if (before < e && idx[before * 64] == idx[e * 64]) {
-          gq[before * 64] += gq[e * 64];
-          again |= 1ull << e;
-        } else {
-          const float f = neg ? -C::M::up(raw) : C::M::up(raw);
-          xk[e * 64] = exp2_((f - st.z) * p.c) * member_f;
-          *col.at(rel) = C::M::mark(e);
-        }
+    // p Q - q of the listed classes; one that is listed again goes on from its earlier entry's value
+    take_listed(col, idx, K, c0, n, z.far(), [&](int e, bool hit, float old) {
+      float f = fmaf(exp2_((old - st.z) * p.c), member_f, -gq[e * 64]);
+      if (hit && old == z.far()) {
+        for (int k = 0; k < e; ++k)
+          if (idx[k * 64] == idx[e * 64]) f = gv[k * 64] - gq[e * 64];
       }
-    }
+      gv[(hit ? e : KP) * 64] = f;
+    });
     wave_sync();
     for (int h = 0; h < n; h += 32) {
       if (LAST) stage_read<T>(stage, q.lane, h, v);
-      settle(v, neg, n - h);
+      settle(v, z.far(), n - h);
 #pragma unroll
-      for (int u = 0; u < 32; ++u) v[u] = exp2_((v[u] - st.x) * p.c) * rest_f;
+      for (int u = 0; u < 32; ++u) {
+        v[u] = exp2_((v[u] - st.x) * p.c) * rest_f;
+        fence_schedule(u);
+      }
       if (any_dead) {
 #pragma unroll
         for (int u = 0; u < 32; ++u) v[u] = dead ? 0.f : v[u];
@@ -810,20 +1007,20 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
       }
     }
     wave_sync();
-    for (int e = 0; e < K; ++e) {
-      const int rel = idx[e * 64] - c0;
-      if ((unsigned)rel < (unsigned)n && !(again >> e & 1))
-        *col.at(rel) = C::M::down(xk[e * 64] - gq[e * 64]);
+    for (int e0 = 0; e0 < K; e0 += kGroup) {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const int rel = idx[(e0 + i) * 64] - c0;
+        *col.at((unsigned)rel < (unsigned)n ? rel : C::kNowhere) = C::M::down(gv[(e0 + i) * 64]);
+      }
     }
     wave_sync();
     if (LAST) {
       stage_out<T>(g, p, q, c0, n, stage);
-    } else if (q.live) {
-      typename T::S* dst = g + (q.o * p.V + c0) * p.inner + q.first;
-      const unsigned at = (unsigned)(q.i - q.first);
+    } else {
 #pragma unroll
-      for (int u = 0; u < 32; ++u)
-        if (u < n) (dst + (int64_t)u * p.inner)[at] = T::down(*(const float*)col.at(u));
+      for (int u = 0; u < 32; ++u) v[u] = *(const float*)col.at(u);
+      planes_out<T>(g, p, q, c0, n, v);
     }
   }
 }
@@ -836,69 +1033,107 @@ __device__ __forceinline__ int tile_class(int lane, int u) {  // class of a lane
   return (u / T::VEC) * 64 * T::VEC + lane * T::VEC + u % T::VEC;
 }
 template <class T>
-__device__ __forceinline__ void row_in(const typename T::S* row, int base, int end, int lane, bool neg, float (&v)[32]) {
-  if (base + kWaveTile <= end) {
-    Vec<T> w[32 / T::VEC];
+__device__ __forceinline__ void row_in(const typename T::S* row, int base, int end, int lane, float far, float (&v)[32]) {
+  const unsigned first = fresh((unsigned)(base + lane * T::VEC));
 #pragma unroll
-    for (int u = 0; u < 32 / T::VEC; ++u) w[u] = load_vec<T>(row + base + tile_class<T>(lane, u * T::VEC));
+  for (int u = 0; u < 32 / T::VEC; ++u) {
+    const unsigned j = first + u * 64 * T::VEC;
+    const int n = end - (int)j;
+    const Vec<T> w = n >= T::VEC ? load_vec<T>(row, j * (unsigned)sizeof(typename T::S))
+                                 : load_some<T>(row, j * (unsigned)sizeof(typename T::S), n);
 #pragma unroll
-    for (int u = 0; u < 32; ++u) v[u] = T::up(w[u / T::VEC].e[u % T::VEC]);
-  } else {
-#pragma unroll
-    for (int u = 0; u < 32 / T::VEC; ++u) {
-      const int j = base + tile_class<T>(lane, u * T::VEC);
-      if (j + T::VEC <= end) {
-        const Vec<T> w = load_vec<T>(row + j);
-#pragma unroll
-        for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = T::up(w.e[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < T::VEC; ++e)
-          v[u * T::VEC + e] = j + e < end ? T::up(row[j + e]) : (neg ? kInf : -kInf);
-      }
-    }
-  }
-  if (neg) {
-#pragma unroll
-    for (int u = 0; u < 32; ++u) v[u] = -v[u];
+    for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = e < n ? w.get(e) : far;
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 template <class T>
 __device__ __forceinline__ void row_out(typename T::S* row, int base, int end, int lane, const float (&v)[32]) {
+  const unsigned first = fresh((unsigned)(base + lane * T::VEC));
 #pragma unroll
   for (int u = 0; u < 32 / T::VEC; ++u) {
-    const int j = base + tile_class<T>(lane, u * T::VEC);
+    const unsigned j = first + u * 64 * T::VEC;
+    const int n = end - (int)j;
     Vec<T> w;
+    w.put(v + u * T::VEC);
+    if (n >= T::VEC) store_vec<T>(row, j * (unsigned)sizeof(typename T::S), w);
+    else store_some<T>(row, j * (unsigned)sizeof(typename T::S), n, w);
+  }
+}
+template <class T, int NT>
+__device__ __forceinline__ void row_zero(typename T::S* row, int begin, int end, int lane, int wave) {
+  float v[32];
 #pragma unroll
-    for (int e = 0; e < T::VEC; ++e) w.e[e] = T::down(v[u * T::VEC + e]);
-    if (j + T::VEC <= end) {
-      store_vec<T>(row + j, w);
-    } else {
+  for (int u = 0; u < 32; ++u) v[u] = 0.f;
+  for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) row_out<T>(row, base, end, lane, v);
+}
+template <class T>
+__device__ __forceinline__ void row_out_full(typename T::S* row, int base, int lane, const float (&v)[32]) {
+  const unsigned first = fresh((unsigned)(base + lane * T::VEC) * (unsigned)sizeof(typename T::S));
 #pragma unroll
-      for (int e = 0; e < T::VEC; ++e)
-        if (j + e < end) row[j + e] = w.e[e];
+  for (int u = 0; u < 32 / T::VEC; ++u) {
+    Vec<T> w;
+    w.put(v + u * T::VEC);
+    store_vec<T>(row, first + u * 1024, w);
+  }
+}
+// the next full tile of a wave, loaded while the one before is worked on
+template <class T>
+struct RowFeed {
+  Vec<T> w[32 / T::VEC];
+  __device__ __forceinline__ void issue(const typename T::S* row, int base, int lane) {
+    const unsigned first = fresh((unsigned)(base + lane * T::VEC) * (unsigned)sizeof(typename T::S));
+#pragma unroll
+    for (int u = 0; u < 32 / T::VEC; ++u) w[u] = load_vec<T>(row, first + u * 1024);
+  }
+  __device__ __forceinline__ void take(float (&v)[32]) const {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) v[u] = w[u / T::VEC].get(u % T::VEC);
+  }
+};
+// f(v, base, it, full) for every block-wide step `it` of [begin, end): first the steps that are full for every
+// wave, then at most one that is not (v is all `far` for a wave that has nothing left)
+template <class T, int NT, class F>
+__device__ __forceinline__ void walk_row(const typename T::S* row, int begin, int end, int lane, int wave, float far, F f) {
+  const int full = (end - begin) / (NT * 32);
+  int base = begin + wave * kWaveTile;
+  if (full > 0) {
+    RowFeed<T> feed;
+    feed.issue(row, base, lane);
+    for (int it = 0; it < full; ++it, base += NT * 32) {
+      float v[32];
+      feed.take(v);
+      if (it + 1 < full) feed.issue(row, base + NT * 32, lane);
+      f(v, base, it, std::true_type{});
     }
+  }
+  if (begin + full * NT * 32 < end) {
+    float v[32];
+    row_in<T>(row, base, end, lane, far, v);
+    f(v, base, full, std::false_type{});
   }
 }
 template <int NT>
-__device__ __forceinline__ Acc acc_block(Acc a, float c, Acc* red) {
-  a = acc_wave(a, c);
+__device__ __forceinline__ Acc acc_block(Acc a, const Side& z, Acc* red) {
+  a = acc_wave(a, z);
   if (NT == 64) return a;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
   __syncthreads();
   a = red[0];
 #pragma unroll
-  for (int w = 1; w < NT / 64; ++w) a = acc_join(a, red[w], c);
+  for (int w = 1; w < NT / 64; ++w) a = acc_join(a, red[w], z);
   return a;
 }
 
 // ---- top classes of a stretch of a row ---------------------------------------------------------------------
-// The k-th largest of the threads' own maxima is a bound that at least k classes reach; few others do, and
-// only the threads whose maximum reaches it look at their classes again.  What reaches the bound is
-// collected in LDS and ranked by counting.  Where more classes tie at the bound than LDS holds, the ones
-// above it are collected and the ties are filled in from the first on.  Rows with NaN, and rows with
-// more classes above the bound than fit, take k rounds of "largest below the last".
+// The k-th largest of the threads' own maxima so far is a bound that at least k classes reach, and few others
+// do.  It is raised after steps 1, 2, 4, 8, ... of the walk, and what reaches it is put down in LDS from the
+// registers: about k classes for each doubling, no second look at the row.  At the end the last bound
+// thins the candidates out and the rest is ranked by counting.
+// More candidates than LDS holds (rows that are constant, or masked but for a few classes), and rows
+// with NaN, take row_top_again(), which goes back to the row: the classes above the bound, then the ones
+// at it from the first on; and k rounds of "largest below the last" where that does not fit either.
 constexpr int kCand = 1024;
+constexpr int kBoundBits = 20;  // of a maximum's 32 order bits: a bound a little too low only lets a few more in
 struct TopShared {
   unsigned long long cand[kCand];
   float maxima[256];
@@ -906,86 +1141,114 @@ struct TopShared {
   int count, total[4];
   float bound;
 };
+__device__ __forceinline__ unsigned order_bits(float v) {
+  const unsigned b = __builtin_bit_cast(unsigned, v + 0.f);
+  return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+}
+// (just below) the k-th largest of the block's maxima, the same in every thread; two barriers
+template <int NT>
+__device__ __forceinline__ float raise_bound(float my_max, int k, TopShared& sh) {
+  unsigned o[NT / 64];
+  if (NT == 64) {
+    o[0] = order_bits(my_max);
+  } else {
+    __syncthreads();
+    sh.maxima[threadIdx.x] = my_max;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) o[w] = order_bits(sh.maxima[w * 64 + (threadIdx.x & 63)]);
+  }
+  unsigned t = 0;
+#pragma unroll
+  for (int bit = 31; bit > 31 - kBoundBits; --bit) {
+    const unsigned c = t | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) n += __popcll(__ballot(o[w] >= c));
+    t = n >= k ? c : t;
+  }
+  if (t <= 0x007fffffu) return -kInf;  // at or below the order bits of -inf
+  return __builtin_bit_cast(float, (t >> 31) ? (t ^ 0x80000000u) : ~t);
+}
+template <class T>
+__device__ __forceinline__ void put_down(const float (&v)[32], float sign, int base, int end, int lane, float bound,
+                                         TopShared& sh) {
+#pragma unroll
+  for (int u = 0; u < 32; ++u) {
+    const int j = base + tile_class<T>(lane, u);
+    if (v[u] * sign >= bound && j < end) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) sh.cand[at] = key_u64(v[u] * sign, j);
+    }
+  }
+}
+// ranks the candidates; out: the `want` largest, descending
+template <int NT>
+__device__ __forceinline__ void rank_candidates(int n, int want, unsigned long long* out, const TopShared& sh) {
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const unsigned long long mine = sh.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.cand[j] > mine ? 1 : 0;
+    if (rank < want) out[rank] = mine;
+  }
+}
 template <class T, int NT>
-__device__ void row_top(const typename T::S* row, int begin, int end, int k, bool neg, float my_max, bool bad,
-                        unsigned long long* out, TopShared& sh) {
+__device__ __noinline__ void row_top_again(const typename T::S* row, int begin, int end, int k, float sign, float my_max,
+                                           bool bad, unsigned long long* out, TopShared& sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int want = min(k, end - begin);
+  __syncthreads();
   if (tid == 0) sh.count = 0;
-  sh.maxima[tid] = my_max;
+  const float bound = raise_bound<NT>(my_max, k, sh);
   __syncthreads();
-  {
-    int rank = 0;
-    for (int j = 0; j < NT; ++j) {
-      const float o = sh.maxima[j];
-      rank += (o > my_max || (o == my_max && j < tid)) ? 1 : 0;
-    }
-    if (rank == min(k, NT) - 1) sh.bound = my_max;
-  }
-  __syncthreads();
-  const float bound = sh.bound;
   bool slow = bad;
   int n = 0;
   if (!slow) {
-    for (int pass = 0; pass < 2; ++pass) {  // 0: all that reach the bound; 1: the ones above it
-      if (my_max >= bound) {
-        for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
-          if (pass == 0 && *(volatile int*)&sh.count > kCand) break;
-          float v[32];
-          row_in<T>(row, base, end, lane, neg, v);
+    // the classes above the bound
+    if (my_max > bound) {
+      for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
+        float v[32];
+        row_in<T>(row, base, end, lane, -kInf, v);
 #pragma unroll
-          for (int u = 0; u < 32; ++u) {
-            const int j = base + tile_class<T>(lane, u);
-            if ((pass == 0 ? v[u] >= bound : v[u] > bound) && j < end) {
-              const int at = atomicAdd(&sh.count, 1);
-              if (at < kCand) sh.cand[at] = key_u64(v[u], j);
-            }
+        for (int u = 0; u < 32; ++u) {
+          const int j = base + tile_class<T>(lane, u);
+          if (v[u] * sign > bound && j < end) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kCand) sh.cand[at] = key_u64(v[u] * sign, j);
           }
         }
       }
-      __syncthreads();
-      n = sh.count;
-      if (n <= kCand) {
-        if (pass == 1 && n < want) {  // ties, lowest index first
-          __syncthreads();
-          for (int base = begin; base < end && n < want; base += NT) {
-            const int j = base + tid;
-            const float v = j < end ? T::up(row[j]) : 0.f;
-            const bool tie = j < end && (neg ? -v : v) == bound;
-            const unsigned long long b = __ballot(tie);
-            if (lane == 0) sh.total[wave] = __popcll(b);
-            __syncthreads();
-            int at = n + __popcll(b & ((1ull << lane) - 1));
-            for (int w = 0; w < wave; ++w) at += sh.total[w];
-            if (tie && at < want) sh.cand[at] = key_u64(neg ? -v : v, j);
-            for (int w = 0; w < NT / 64; ++w) n += sh.total[w];
-            __syncthreads();
-          }
-          n = min(n, want);
-        }
-        break;
+    }
+    __syncthreads();
+    n = sh.count;
+    slow = n > kCand;
+    if (!slow && n < want) {  // the ones at it, lowest index first
+      for (int base = begin; base < end && n < want; base += NT) {
+        const int j = base + tid;
+        const float v = j < end ? T::up(row[j]) * sign : 0.f;
+        const bool tie = j < end && v == bound;
+        const unsigned long long b = __ballot(tie);
+        if (lane == 0) sh.total[wave] = __popcll(b);
+        __syncthreads();
+        int at = n + __popcll(b & ((1ull << lane) - 1));
+        for (int w = 0; w < wave; ++w) at += sh.total[w];
+        if (tie && at < want) sh.cand[at] = key_u64(v, j);
+        for (int w = 0; w < NT / 64; ++w) n += sh.total[w];
+        __syncthreads();
       }
-      if (pass == 1) slow = true;
-      __syncthreads();
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
+      n = min(n, want);
+      slow = n < want;  // the bound lies between two values: too few above it, and none at it
     }
   }
   if (!slow) {
     __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-      const unsigned long long mine = sh.cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += sh.cand[j] > mine ? 1 : 0;
-      if (rank < want) out[rank] = mine;
-    }
+    rank_candidates<NT>(n, want, out, sh);
   } else {
     unsigned long long last = ~0ull;
     for (int r = 0; r < want; ++r) {
       unsigned long long best = 0;
       for (int j = begin + tid; j < end; j += NT) {
-        const float v = T::up(row[j]);
-        const unsigned long long key = key_u64(neg ? -v : v, j);
+        const unsigned long long key = key_u64(T::up(row[j]) * sign, j);
         if (key < last && key > best) best = key;
       }
 #pragma unroll
@@ -1002,8 +1265,6 @@ __device__ void row_top(const typename T::S* row, int begin, int end, int k, boo
       last = best;
     }
   }
-  for (int i = want + tid; i < k; i += NT) out[i] = 0;  // shorter than k: nothing
-  __syncthreads();
 }
 
 struct LpOut {
@@ -1014,13 +1275,13 @@ struct LpOut {
 template <class T>
 __device__ __forceinline__ void lp_row_write(const Prob& p, int64_t row, const typename T::S* xr, const void* index,
                                              const Acc& a, const LpOut& o) {
-  const bool neg = p.scale < 0.f;
-  const float base = a.m == -kInf ? 0.f : a.m, ln_s = logf(a.s);
+  const Side z = side(p);
+  const float base = a.m == z.far() ? 0.f : a.m, ln_s = logf(a.s);
   const int t = index ? valid_index(load_index(index, row, p.flags), p.V) : -1;
   float lp = 0.f;
   if (t >= 0) {
     const float v = T::up(xr[t]);
-    lp = log_p(neg ? -v : v, base, ln_s, p.scale);
+    lp = log_p(v, base, ln_s, p.scale);
   }
   if (o.log_prob) o.log_prob[row] = lp;
   if (o.entropy) o.entropy[row] = entropy_of(a.s, a.w, ln_s);
@@ -1028,8 +1289,9 @@ __device__ __forceinline__ void lp_row_write(const Prob& p, int64_t row, const t
 }
 __device__ __forceinline__ void lp_row_top_write(const Prob& p, int64_t row, int rank, unsigned long long key,
                                                  const Acc& a, const LpOut& o) {
-  const float base = a.m == -kInf ? 0.f : a.m;
-  o.top_lp[row * p.k + rank] = log_p(key_value(key), base, logf(a.s), p.scale);
+  const Side z = side(p);
+  const float base = a.m == z.far() ? 0.f : a.m;
+  o.top_lp[row * p.k + rank] = log_p(key_value(key) * z.sign, base, logf(a.s), p.scale);
   o.top_idx[row * p.k + rank] = key_index(key);
 }
 
@@ -1042,7 +1304,7 @@ __host__ __device__ inline size_t parts_bytes(int64_t rows, int chunks) {
 }
 
 template <class T, int NT, bool TOP>
-__global__ __launch_bounds__(NT) void lp_row_fwd(Prob p, const typename T::S* __restrict__ x,
+__global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S* __restrict__ x,
                                                  const void* __restrict__ index, LpOut o, Part* __restrict__ parts,
                                                  unsigned long long* __restrict__ part_keys) {
   __shared__ Acc red[NT / 64];
@@ -1051,29 +1313,62 @@ __global__ __launch_bounds__(NT) void lp_row_fwd(Prob p, const typename T::S* __
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const typename T::S* xr = x + row * p.V;
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
-  const bool neg = p.scale < 0.f;
-  Acc a = acc_empty();
-  for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
-    float v[32];
-    row_in<T>(xr, base, end, lane, neg, v);
-    absorb<true>(a, v, p.c);
+  const Side z = side(p);
+  __shared__ std::conditional_t<TOP, TopShared, char> shared_top;
+  if constexpr (TOP) {
+    if (threadIdx.x == 0) shared_top.count = 0;
+    __syncthreads();
   }
-  const float my_max = a.m;
-  a = acc_block<NT>(a, p.c, red);
+  Acc a = acc_empty(z);
+  float bound = -kInf;
+  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](const float (&v)[32], int base, int it, auto) {
+    const float top = z.best_of(v);
+    absorb<true>(a, v, top, z);
+    if constexpr (TOP) {
+      if (((it + 1) & it) == 0) bound = raise_bound<NT>(a.m * z.sign, p.k, shared_top);
+      if (top * z.sign >= bound) put_down<T>(v, z.sign, base, end, lane, bound, shared_top);
+    }
+  });
+  const float my_max = a.m * z.sign;
+  a = acc_block<NT>(a, z, red);
   if (p.chunks == 1) {
     if (threadIdx.x == 0) lp_row_write<T>(p, row, xr, index, a, o);
   } else if (threadIdx.x == 0) {
     parts[row * p.chunks + chunk] = Part{a.m, a.s, a.w, 0.f};
   }
   if constexpr (TOP) {
-    __shared__ TopShared sh;
+    TopShared& sh = shared_top;
     __shared__ unsigned long long best[kMaxEntries];
-    row_top<T, NT>(xr, begin, end, p.k, neg, my_max, a.s != a.s, best, sh);
+    const int want = min(p.k, end - begin);
+    bound = raise_bound<NT>(my_max, p.k, sh);
+    __syncthreads();
+    int n = sh.count;
+    if (n > kCand || a.s != a.s) {
+      row_top_again<T, NT>(xr, begin, end, p.k, z.sign, my_max, a.s != a.s, best, sh);
+    } else {
+      unsigned long long mine[kCand / NT];
+#pragma unroll
+      for (int i = 0; i < kCand / NT; ++i) {
+        const int at = threadIdx.x + i * NT;
+        mine[i] = at < n ? sh.cand[at] : 0;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) sh.count = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kCand / NT; ++i) {
+        if (mine[i] != 0 && key_value(mine[i]) >= bound) sh.cand[atomicAdd(&sh.count, 1)] = mine[i];
+      }
+      __syncthreads();
+      rank_candidates<NT>(sh.count, want, best, sh);
+    }
+    __syncthreads();
     if ((int)threadIdx.x < p.k) {
+      const unsigned long long key = (int)threadIdx.x < want ? best[threadIdx.x] : 0;
       if (p.chunks == 1)
-        lp_row_top_write(p, row, threadIdx.x, best[threadIdx.x], a, o);
+        lp_row_top_write(p, row, threadIdx.x, key, a, o);
       else
-        part_keys[(row * p.chunks + chunk) * p.k + threadIdx.x] = best[threadIdx.x];
+        part_keys[(row * p.chunks + chunk) * p.k + threadIdx.x] = key;
     }
   }
 }
@@ -1086,10 +1381,11 @@ __global__ __launch_bounds__(256) void lp_row_join(Prob p, const typename T::S* 
                                                    const unsigned long long* __restrict__ part_keys) {
   __shared__ unsigned long long keys[kCand];
   const int64_t row = blockIdx.x;
-  Acc a = acc_empty();
+  const Side z = side(p);
+  Acc a = acc_empty(z);
   for (int i = 0; i < p.chunks; ++i) {
     const Part q = parts[row * p.chunks + i];
-    a = acc_join(a, Acc{q.m, q.s, q.w}, p.c);
+    a = acc_join(a, Acc{q.m, q.s, q.w}, z);
   }
   if (threadIdx.x == 0) lp_row_write<T>(p, row, x + row * p.V, index, a, o);
   const int n = p.chunks * p.k;  // at most kCand
@@ -1104,7 +1400,7 @@ __global__ __launch_bounds__(256) void lp_row_join(Prob p, const typename T::S* 
 }
 
 template <class T, int NT, bool ENT>
-__global__ __launch_bounds__(NT) void lp_row_bwd(Prob p, const typename T::S* __restrict__ x,
+__global__ __launch_bounds__(NT, 4) void lp_row_bwd(Prob p, const typename T::S* __restrict__ x,
                                                  const void* __restrict__ index, const Stats3* __restrict__ stats,
                                                  const float* __restrict__ g_lp,
                                                  const float* __restrict__ g_ent, typename T::S* __restrict__ g) {
@@ -1114,25 +1410,26 @@ __global__ __launch_bounds__(NT) void lp_row_bwd(Prob p, const typename T::S* __
   const typename T::S* xr = x + row * p.V;
   typename T::S* gr = g + row * p.V;
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
-  const bool neg = p.scale < 0.f;
+  const Side z = side(p);
   const LpCoef r = lp_coef<ENT>(p, row, index, stats, g_lp, g_ent);
-  for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
-    float v[32];
-    if (r.dead) {
-#pragma unroll
-      for (int u = 0; u < 32; ++u) v[u] = 0.f;
-    } else {
-      row_in<T>(xr, base, end, lane, neg, v);
-#pragma unroll
-      for (int u = 0; u < 32; ++u) v[u] = lp_grad<ENT>(r, v[u], p.c, 0.f);
-      const int rel = r.target - base;
-      if ((unsigned)rel < (unsigned)kWaveTile) {
-#pragma unroll
-        for (int u = 0; u < 32; ++u) v[u] += tile_class<T>(lane, u) == rel ? r.hit : 0.f;
-      }
-    }
-    row_out<T>(gr, base, end, lane, v);
+  if (r.dead) {
+    row_zero<T, NT>(gr, begin, end, lane, wave);
+    return;
   }
+  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, auto full) {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) {
+      v[u] = lp_grad<ENT>(r, v[u], p.c, 0.f);
+      fence_schedule(u);
+    }
+    const int rel = r.target - base;
+    if ((unsigned)rel < (unsigned)kWaveTile) {
+#pragma unroll
+      for (int u = 0; u < 32; ++u) v[u] += tile_class<T>(lane, u) == rel ? r.hit : 0.f;
+    }
+    if (decltype(full)::value) row_out_full<T>(gr, base, lane, v);
+    else row_out<T>(gr, base, end, lane, v);
+  });
 }
 
 // ---- distillation over long rows: every wave holds the whole list, one entry a lane --------------------
@@ -1186,15 +1483,14 @@ __device__ __forceinline__ void patch_tile(float (&v)[32], int base, int lane, i
 template <class T>
 __device__ __forceinline__ void ds_row_write(const Prob& p, int64_t row, const typename T::S* xr, const Entry& e,
                                              const Acc& a, float* loss, float4* stats) {
-  const bool neg = p.scale < 0.f;
-  float v = -kInf;
-  if (e.idx >= 0) v = neg ? -T::up(xr[e.idx]) : T::up(xr[e.idx]);
-  const float first = e.again ? -kInf : v;
+  const Side z = side(p);
+  const float v = e.idx >= 0 ? T::up(xr[e.idx]) : z.far();
+  const float first = e.again ? z.far() : v;
   RowSums r;
   r.m_r = a.m;
   r.s_r = a.s;
-  const float m = vmax(a.m, wave_max_all(first));
-  r.b = m == -kInf ? 0.f : m;
+  const float m = z.best(a.m, wave_best_all(first, z));
+  r.b = m == z.far() ? 0.f : m;
   r.s = fmaf(a.s, exp2_((a.m - r.b) * p.c), wave_sum_all(exp2_((first - r.b) * p.c)));
   r.ln_s = logf(r.s);
   const bool alive = __any(e.idx >= 0);
@@ -1210,7 +1506,7 @@ __device__ __forceinline__ void ds_row_write(const Prob& p, int64_t row, const t
 }
 
 template <class T, int NT>
-__global__ __launch_bounds__(NT) void ds_row_fwd(Prob p, const typename T::S* __restrict__ x,
+__global__ __launch_bounds__(NT, 4) void ds_row_fwd(Prob p, const typename T::S* __restrict__ x,
                                                  const void* __restrict__ teacher, const void* __restrict__ index,
                                                  float* __restrict__ loss, float4* __restrict__ stats,
                                                  Part* __restrict__ parts) {
@@ -1220,18 +1516,17 @@ __global__ __launch_bounds__(NT) void ds_row_fwd(Prob p, const typename T::S* __
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const typename T::S* xr = x + row * p.V;
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
-  const bool neg = p.scale < 0.f;
+  const Side z = side(p);
   const Entry e = load_entry(p, row, p.chunks == 1 ? teacher : nullptr, index, lane);
-  Acc a = acc_empty();
+  Acc a = acc_empty(z);
   if (__any(e.idx >= 0)) {  // the same in every wave
-    for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
-      float v[32];
-      row_in<T>(xr, base, end, lane, neg, v);
-      patch_tile<T>(v, base, lane, e.idx, -kInf);
-      absorb<false>(a, v, p.c);
-    }
+    walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, auto full) {
+      (void)full;
+      patch_tile<T>(v, base, lane, e.idx, z.far());
+      absorb<false>(a, v, z.best_of(v), z);
+    });
   }
-  a = acc_block<NT>(a, p.c, red);
+  a = acc_block<NT>(a, z, red);
   if (p.chunks > 1) {
     if (threadIdx.x == 0) parts[row * p.chunks + chunk] = Part{a.m, a.s, 0.f, 0.f};
   } else if (wave == 0) {
@@ -1244,18 +1539,19 @@ __global__ __launch_bounds__(64) void ds_row_join(Prob p, const typename T::S* _
                                                   float* __restrict__ loss, float4* __restrict__ stats,
                                                   const Part* __restrict__ parts) {
   const int64_t row = blockIdx.x;
+  const Side z = side(p);
   const Entry e = load_entry(p, row, teacher, index, threadIdx.x);
-  Acc a = acc_empty();
+  Acc a = acc_empty(z);
   for (int i = threadIdx.x; i < p.chunks; i += 64) {
     const Part q = parts[row * p.chunks + i];
-    a = acc_join(a, Acc{q.m, q.s, 0.f}, p.c);
+    a = acc_join(a, Acc{q.m, q.s, 0.f}, z);
   }
-  a = acc_wave(a, p.c);
+  a = acc_wave(a, z);
   ds_row_write<T>(p, row, x + row * p.V, e, a, loss, stats);
 }
 
 template <class T, int NT>
-__global__ __launch_bounds__(NT) void ds_row_bwd(Prob p, const typename T::S* __restrict__ x,
+__global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S* __restrict__ x,
                                                  const void* __restrict__ teacher, const void* __restrict__ index,
                                                  const float4* __restrict__ stats, const float* __restrict__ g_loss,
                                                  typename T::S* __restrict__ g) {
@@ -1265,15 +1561,18 @@ __global__ __launch_bounds__(NT) void ds_row_bwd(Prob p, const typename T::S* __
   const typename T::S* xr = x + row * p.V;
   typename T::S* gr = g + row * p.V;
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
-  const bool neg = p.scale < 0.f;
+  const Side z = side(p);
   const float4 st = stats[row];
   const float up = g_loss[row];
   const bool dead = up == 0.f || st.w == 0.f;
   const float gs = up * p.scale, rest_f = gs * st.y, member_f = gs * st.w;
-  Entry e{-1, 0.f, false};
+  if (dead) {
+    row_zero<T, NT>(gr, begin, end, lane, wave);
+    return;
+  }
+  Entry e = load_entry(p, row, teacher, index, lane);
   float with = 0.f;
-  if (!dead) {
-    e = load_entry(p, row, teacher, index, lane);
+  {
     float qe = e.idx >= 0 ? expf(e.value) : 0.f;
     float sum = qe;  // of all entries of this class
     for (int k = 0; k < p.k; ++k) {
@@ -1282,24 +1581,21 @@ __global__ __launch_bounds__(NT) void ds_row_bwd(Prob p, const typename T::S* __
       if (k != lane && other == e.idx && other >= 0) sum += oq;
     }
     if (e.idx >= 0) {
-      const float v = neg ? -T::up(xr[e.idx]) : T::up(xr[e.idx]);
+      const float v = T::up(xr[e.idx]);
       with = exp2_((v - st.z) * p.c) * member_f - gs * sum;
     }
     if (e.again) e.idx = -1;
   }
-  for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
-    float v[32];
-    if (dead) {
+  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, auto full) {
 #pragma unroll
-      for (int u = 0; u < 32; ++u) v[u] = 0.f;
-    } else {
-      row_in<T>(xr, base, end, lane, neg, v);
-#pragma unroll
-      for (int u = 0; u < 32; ++u) v[u] = exp2_((v[u] - st.x) * p.c) * rest_f;
-      patch_tile<T>(v, base, lane, e.idx, with);
+    for (int u = 0; u < 32; ++u) {
+      v[u] = exp2_((v[u] - st.x) * p.c) * rest_f;
+      fence_schedule(u);
     }
-    row_out<T>(gr, base, end, lane, v);
-  }
+    patch_tile<T>(v, base, lane, e.idx, with);
+    if (decltype(full)::value) row_out_full<T>(gr, base, lane, v);
+    else row_out<T>(gr, base, end, lane, v);
+  });
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------
@@ -1341,7 +1637,7 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
   p.V = (int)d->classes;
   p.k = d->entries;
   p.scale = d->scale;
-  p.c = (d->scale < 0.f ? -d->scale : d->scale) * kLog2e;
+  p.c = d->scale * kLog2e;
   p.flags = d->flags;
   p.chunks = 1;
   p.chunk = p.V;
@@ -1355,7 +1651,8 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
     const int stages = (p.V + stage - 1) / stage;
     P.nw = 1;
     while (P.nw < 16 && tiles * P.nw < kWantWaves && P.nw * 2 <= stages) P.nw *= 2;
-    const size_t per_wave = kStageBytes + (distill ? 512 : 64 * (12 + 8 * 16)), shared = distill ? p.k * 768 : 0;
+    const size_t per_wave = kStageBytes + (distill ? 512 : 64 * (12 + 8 * 16));
+    const size_t shared = distill ? distill_lds(0, p.k, true) : 0;
     while (P.nw > 1 && P.nw * per_wave + shared > kLdsBudget) P.nw /= 2;
     p.cpw = (stages + P.nw - 1) / P.nw * stage;
     if (tiles > 0x7fffffff) return DW_ERR_SHAPE;
@@ -1455,7 +1752,7 @@ template <class T, bool LAST>
 int ds_tile_launch(const Plan& P, bool backward, const void* x, const void* teacher, const void* index, float* loss,
                    float4* stats, const float* g_loss, void* g, hipStream_t st) {
   using S = typename T::S;
-  const size_t lds = P.nw * (size_t)distill_stage_bytes<LAST>() + (size_t)P.p.k * 768 + P.nw * 512;
+  const size_t lds = P.nw * (size_t)distill_stage_bytes<LAST>() + distill_lds(P.nw, P.p.k, backward);
   if (backward) {
     if (int rc = allow_lds(ds_tile_bwd<T, LAST>, lds)) return rc;
     ds_tile_bwd<T, LAST><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, stats, g_loss, (S*)g);
