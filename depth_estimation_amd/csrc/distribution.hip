@@ -356,6 +356,44 @@ __device__ __forceinline__ float load_teacher(const void* p, int64_t at, int fla
   return ((const float*)p)[at];
 }
 
+// N entries of a list from the e0-th on; -1 for what is padding or behind the k-th.  All loads are issued
+// before the first is looked at.
+template <int N>
+__device__ __forceinline__ void load_indices(const Prob& p, const void* index, int64_t t0, int e0, int (&idx)[N]) {
+  int64_t at[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) at[i] = t0 + min(e0 + i, p.k - 1) * p.es[1];
+  if (p.flags & kIdx64) {
+    int64_t v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = ((const int64_t*)index)[at[i]];
+#pragma unroll
+    for (int i = 0; i < N; ++i) idx[i] = e0 + i < p.k ? valid_index(v[i], p.V) : -1;
+  } else {
+    int v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = ((const int32_t*)index)[at[i]];
+#pragma unroll
+    for (int i = 0; i < N; ++i) idx[i] = e0 + i < p.k ? valid_index(v[i], p.V) : -1;
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_teachers(const Prob& p, const void* teacher, int64_t t0, int e0, float (&l)[N]) {
+  int64_t at[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) at[i] = t0 + min(e0 + i, p.k - 1) * p.es[1];
+  if (p.flags & (DW_DIST_TEACHER_BF16 | DW_DIST_TEACHER_F16)) {
+    uint16_t v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = ((const uint16_t*)teacher)[at[i]];
+#pragma unroll
+    for (int i = 0; i < N; ++i) l[i] = (p.flags & DW_DIST_TEACHER_BF16) ? BF16::up(v[i]) : F16::up(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) l[i] = ((const float*)teacher)[at[i]];
+  }
+}
+
 // ---- tile kernels: where the 64 rows of a block are, and how their classes come in -----------------
 struct Place {
   int64_t row;    // this lane's row (planes: the last pixel again behind the end)
@@ -365,15 +403,18 @@ struct Place {
   int skip;       // LAST: so many of the block's first rows belong to the block before
   bool live;      // this lane's row is the block's to write
 };
+// Backward passes take the blocks from the last to the first: what the forward pass read last is what the
+// last-level cache still holds.
+__device__ __forceinline__ unsigned block_from_end() { return gridDim.x - 1 - blockIdx.x; }
 template <bool LAST>
-__device__ __forceinline__ Place place(const Prob& p) {
+__device__ __forceinline__ Place place(const Prob& p, unsigned block) {
   Place q;
   q.lane = threadIdx.x & 63;
   q.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (LAST) {
     // the last block starts 64 rows before the end (there are at least 64) and leaves the ones before its
     // own to their block
-    const int64_t own = (int64_t)blockIdx.x * 64;
+    const int64_t own = (int64_t)block * 64;
     q.first = own + 64 <= p.rows ? own : p.rows - 64;
     q.skip = (int)(own - q.first);
     q.row = q.first + q.lane;
@@ -382,8 +423,8 @@ __device__ __forceinline__ Place place(const Prob& p) {
     q.i = p.inner == 1 ? 0 : q.row - q.o * p.inner;
   } else {
     const unsigned tiles = (unsigned)((p.inner + 63) / 64);
-    q.o = blockIdx.x / tiles;
-    q.first = (int64_t)(blockIdx.x - (unsigned)q.o * tiles) * 64;
+    q.o = block / tiles;
+    q.first = (int64_t)(block - (unsigned)q.o * tiles) * 64;
     q.i = q.first + q.lane;
     q.live = q.i < p.inner;
     if (!q.live) q.i = p.inner - 1;
@@ -551,7 +592,7 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
                             float* __restrict__ log_prob, float* __restrict__ entropy, float* __restrict__ top_lp,
                             int32_t* __restrict__ top_idx, Stats3* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
-  const Place q = place<LAST>(p);
+  const Place q = place<LAST>(p, blockIdx.x);
   const int nw = blockDim.x >> 6;
   char* stage = smem + q.wave * kStageBytes;                       // LAST only
   char* joint = smem + (LAST ? nw * kStageBytes : 0);
@@ -560,6 +601,10 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   constexpr int CH = stage_classes<T, LAST>();
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
+
+  // the given class, on its way while the classes are read
+  const int given = index ? valid_index(load_index(index, q.row, p.flags), p.V) : -1;
+  const float x_given = given >= 0 ? T::up(x[element<LAST>(p, q, given)]) : 0.f;
 
   Acc a = acc_empty(z);
   double limit = 0.0;
@@ -639,12 +684,7 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
       base = a.m == z.far() ? 0.f : a.m;
       ln_s = logf(a.s);
       if (q.wave == 0 && q.live) {
-        const int t = index ? valid_index(load_index(index, q.row, p.flags), p.V) : -1;
-        float lp = 0.f;
-        if (t >= 0) {
-          const float v = T::up(x[element<LAST>(p, q, t)]);
-          lp = log_p(v, base, ln_s, p.scale);
-        }
+        const float lp = given >= 0 ? log_p(x_given, base, ln_s, p.scale) : 0.f;
         if (log_prob) log_prob[q.row] = lp;
         if (entropy) entropy[q.row] = entropy_of(a.s, a.w, ln_s);
         if (stats) stats[q.row] = Stats3{base, a.s, a.w};
@@ -700,7 +740,7 @@ __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
                             const Stats3* __restrict__ stats, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
                             typename T::S* __restrict__ g) {
   extern __shared__ __align__(16) char smem[];
-  const Place q = place<LAST>(p);
+  const Place q = place<LAST>(p, block_from_end());
   char* stage = smem + q.wave * kStageBytes;
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
@@ -788,7 +828,32 @@ constexpr int kGroup = 8;  // entries handled at once: their LDS accesses overla
 __host__ __device__ constexpr int padded(int k) { return (k + kGroup - 1) / kGroup * kGroup; }
 // LDS of a block besides the stages: columns of 64 lanes, of list entries and of the waves' sums
 __host__ __device__ constexpr size_t distill_lds(int nw, int k, bool backward) {
-  return (size_t)256 * (padded(k) * (backward ? 3 : 2) + 1 + (backward ? 0 : 2 * nw));
+  return (size_t)256 * (padded(k) * 3 + 1 + (backward ? 0 : 2 * nw));
+}
+
+template <class S>
+__device__ __forceinline__ void read_group(const S* column, int e0, S (&v)[kGroup]) {
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) v[i] = column[(e0 + i) * 64];
+}
+// Natural log of what the listed values' exponentials sum to (0 where that is nothing): the shift that
+// makes log-probabilities of them.  Padding holds -inf.
+__device__ __forceinline__ float list_shift(const float* tl, int KP) {
+  float tm = -kInf, ts = 0.f;  // fmaxf drops a NaN; the sum brings it back
+  for (int e0 = 0; e0 < KP; e0 += kGroup) {
+    float l[kGroup];
+    read_group(tl, e0, l);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) tm = fmaxf(tm, l[i]);
+  }
+  if (tm == -kInf) tm = 0.f;
+  for (int e0 = 0; e0 < KP; e0 += kGroup) {
+    float l[kGroup];
+    read_group(tl, e0, l);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) ts += expf(l[i] - tm);
+  }
+  return ts == 0.f ? 0.f : tm + logf(ts);
 }
 
 // The first entry before e of the same class, or e.  Asked only where a listed class was found impossible:
@@ -828,30 +893,44 @@ template <class T, bool LAST>
 __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ teacher,
                             const void* __restrict__ index, float* __restrict__ loss, float4* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
-  const Place q = place<LAST>(p);
+  const Place q = place<LAST>(p, blockIdx.x);
   const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
   char* stage = smem + q.wave * distill_stage_bytes<LAST>();
   char* rest = smem + nw * distill_stage_bytes<LAST>();
   int* idx = (int*)rest + q.lane;                            // [KP][64]
-  float* xs = (float*)rest + KP * 64 + q.lane;               // [KP + 1][64]: the listed classes' values
-  float* red = (float*)rest + (2 * KP + 1) * 64 + q.lane;    // [2][nw][64]
+  float* tl = (float*)rest + KP * 64 + q.lane;               // [KP][64]: the teacher's values, -inf for padding
+  float* xs = (float*)rest + 2 * KP * 64 + q.lane;           // [KP + 1][64]: the listed classes' values
+  float* red = (float*)rest + (3 * KP + 1) * 64 + q.lane;    // [2][nw][64]
   const Column<T, LAST> col{stage, q.lane};
   constexpr int CH = stage_classes<T, LAST>();
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
   const int64_t t0 = q.o * p.es[0] + q.i * p.es[2];
+  Feed<T, LAST> feed;
+  if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
 
-  for (int e = q.wave; e < KP; e += nw) {
-    idx[e * 64] = e < K ? valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V) : -1;
-    xs[e * 64] = z.far();
+  for (int e0 = q.wave * kGroup; e0 < KP; e0 += nw * kGroup) {
+    int i8[kGroup];
+    float l8[kGroup];
+    load_indices(p, index, t0, e0, i8);
+    load_teachers(p, teacher, t0, e0, l8);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      idx[(e0 + i) * 64] = i8[i];
+      tl[(e0 + i) * 64] = i8[i] >= 0 ? l8[i] : -kInf;
+      xs[(e0 + i) * 64] = z.far();
+    }
   }
   __syncthreads();
   bool alive = false;
-  for (int e = 0; e < K; ++e) alive |= idx[e * 64] >= 0;
+  for (int e0 = 0; e0 < KP; e0 += kGroup) {
+    int i8[kGroup];
+    read_group(idx, e0, i8);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) alive |= i8[i] >= 0;
+  }
   Acc a = acc_empty(z);
   if (__any(alive)) {  // the same in every wave of the block
-    Feed<T, LAST> feed;
-    if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
     for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
       const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
       float v[32];
@@ -889,29 +968,35 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   RowSums r;
   r.m_r = a.m;
   r.s_r = a.s;
-  float m = a.m, tm = -kInf;
-  for (int e = 0; e < K; ++e) {
-    m = z.best(m, xs[e * 64]);
-    if ((p.flags & kRenorm) && idx[e * 64] >= 0) tm = fmaxf(tm, load_teacher(teacher, t0 + e * p.es[1], p.flags));
+  float m = a.m;
+  for (int e0 = 0; e0 < KP; e0 += kGroup) {
+    float v[kGroup];
+    read_group(xs, e0, v);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) m = z.best(m, v[i]);
   }
   r.b = m == z.far() ? 0.f : m;
   r.s = a.s * exp2_((a.m - r.b) * p.c);
-  float ts = 0.f;
-  for (int e = 0; e < K; ++e) {
-    r.s += exp2_((xs[e * 64] - r.b) * p.c);
-    if ((p.flags & kRenorm) && idx[e * 64] >= 0)
-      ts += expf(load_teacher(teacher, t0 + e * p.es[1], p.flags) - (tm == -kInf ? 0.f : tm));
+  for (int e0 = 0; e0 < KP; e0 += kGroup) {
+    float v[kGroup];
+    read_group(xs, e0, v);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) r.s += exp2_((v[i] - r.b) * p.c);
   }
   r.ln_s = logf(r.s);
-  const float shift = (p.flags & kRenorm) ? (ts == 0.f ? 0.f : tm + logf(ts)) : 0.f;
+  const float shift = (p.flags & kRenorm) ? list_shift(tl, KP) : 0.f;
   float mass = 0.f, l = 0.f;
-  for (int e = 0; e < K; ++e) {
-    if (idx[e * 64] < 0) continue;
-    const float lq = load_teacher(teacher, t0 + e * p.es[1], p.flags) - shift, qe = expf(lq);
-    mass += qe;
-    float v = xs[e * 64];
-    if (v == z.far()) v = xs[listed_before(idx, e) * 64];
-    if (qe != 0.f) l = fmaf(qe, lq - log_p(v, r.b, r.ln_s, p.scale), l);
+  for (int e0 = 0; e0 < KP; e0 += kGroup) {
+    float v[kGroup], t[kGroup];
+    read_group(xs, e0, v);
+    read_group(tl, e0, t);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const float lq = t[i] - shift, qe = expf(lq);  // 0 for padding
+      mass += qe;
+      if (v[i] == z.far() && idx[(e0 + i) * 64] >= 0) v[i] = xs[listed_before(idx, e0 + i) * 64];
+      if (qe != 0.f) l = fmaf(qe, lq - log_p(v[i], r.b, r.ln_s, p.scale), l);
+    }
   }
   const float rr = (alive && !(p.flags & kRenorm) && r.s_r != 0.f) ? fmaxf(1.f - mass, 0.f) : 0.f;
   if (rr > 0.f) l += rest_term(r, p.scale, rr);
@@ -925,7 +1010,7 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
                             const void* __restrict__ index, const float4* __restrict__ stats,
                             const float* __restrict__ g_loss, typename T::S* __restrict__ g) {
   extern __shared__ __align__(16) char smem[];
-  const Place q = place<LAST>(p);
+  const Place q = place<LAST>(p, block_from_end());
   const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
   char* stage = smem + q.wave * distill_stage_bytes<LAST>();
   char* rest = smem + nw * distill_stage_bytes<LAST>();
@@ -946,21 +1031,26 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
   Feed<T, LAST> feed;
   if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
 
-  float shift = 0.f;
-  if (renorm && !dead) {
-    float tm = -kInf, ts = 0.f;
-    for (int e = 0; e < K; ++e)
-      if (valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V) >= 0)
-        tm = fmaxf(tm, load_teacher(teacher, t0 + e * p.es[1], p.flags));
-    for (int e = 0; e < K; ++e)
-      if (valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V) >= 0)
-        ts += expf(load_teacher(teacher, t0 + e * p.es[1], p.flags) - (tm == -kInf ? 0.f : tm));
-    shift = ts == 0.f ? 0.f : tm + logf(ts);
+  for (int e0 = q.wave * kGroup; e0 < KP; e0 += nw * kGroup) {
+    int i8[kGroup];
+    float l8[kGroup];
+    load_indices(p, index, t0, e0, i8);
+    load_teachers(p, teacher, t0, e0, l8);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      if (dead) i8[i] = -1;
+      idx[(e0 + i) * 64] = i8[i];
+      gq[(e0 + i) * 64] = i8[i] < 0 ? (renorm ? -kInf : 0.f) : renorm ? l8[i] : gs * expf(l8[i]);
+    }
   }
-  for (int e = q.wave; e < KP; e += nw) {
-    const int i = dead || e >= K ? -1 : valid_index(load_index(index, t0 + e * p.es[1], p.flags), p.V);
-    idx[e * 64] = i;
-    gq[e * 64] = i >= 0 ? gs * expf(load_teacher(teacher, t0 + e * p.es[1], p.flags) - shift) : 0.f;
+  if (renorm) {  // values first, probabilities when their sum is known
+    __syncthreads();
+    const float shift = list_shift(gq, KP);
+    __syncthreads();
+    for (int e0 = q.wave * kGroup; e0 < KP; e0 += nw * kGroup) {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) gq[(e0 + i) * 64] = gs * expf(gq[(e0 + i) * 64] - shift);
+    }
   }
   __syncthreads();
   const bool any_dead = __any(dead);
@@ -1404,8 +1494,9 @@ __global__ __launch_bounds__(NT, 4) void lp_row_bwd(Prob p, const typename T::S*
                                                  const void* __restrict__ index, const Stats3* __restrict__ stats,
                                                  const float* __restrict__ g_lp,
                                                  const float* __restrict__ g_ent, typename T::S* __restrict__ g) {
-  const int64_t row = blockIdx.x / (unsigned)p.chunks;
-  const int chunk = blockIdx.x - (unsigned)row * p.chunks;
+  const unsigned block = block_from_end();
+  const int64_t row = block / (unsigned)p.chunks;
+  const int chunk = block - (unsigned)row * p.chunks;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const typename T::S* xr = x + row * p.V;
   typename T::S* gr = g + row * p.V;
@@ -1555,8 +1646,9 @@ __global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S*
                                                  const void* __restrict__ teacher, const void* __restrict__ index,
                                                  const float4* __restrict__ stats, const float* __restrict__ g_loss,
                                                  typename T::S* __restrict__ g) {
-  const int64_t row = blockIdx.x / (unsigned)p.chunks;
-  const int chunk = blockIdx.x - (unsigned)row * p.chunks;
+  const unsigned block = block_from_end();
+  const int64_t row = block / (unsigned)p.chunks;
+  const int chunk = block - (unsigned)row * p.chunks;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const typename T::S* xr = x + row * p.V;
   typename T::S* gr = g + row * p.V;

@@ -37,62 +37,32 @@ _INDEX_FLAGS = {torch.int32: 0, torch.int64: _lib.DW_DIST_INDEX64}
 
 
 class LogProbs(NamedTuple):
-    log_prob: Optional[Tensor]   # of the given class; 0 where none is given; None without an index
-    entropy: Tensor              # of the row's distribution, in nats
-    top_log_prob: Tensor         # the `top` most likely classes along the class axis, descending
-    top_index: Tensor            # their indices, int32; ties: the lowest first
-
-
-@functools.lru_cache(maxsize=1024)
-def _desc(workspace_of, outer, classes, inner, stride, scale, dtype, entries, flags):
-    """(descriptor for ctypes, workspace bytes) of one problem; raises on what the library refuses."""
-    d = _lib.DwDistDesc(outer, classes, inner, stride, scale, dtype, entries, flags)
-    ref = C.byref(d)
-    nbytes = getattr(_lib.lib(), workspace_of)(ref)
-    if nbytes < 0:
-        _lib.check(int(nbytes), f"{workspace_of}(classes={classes}, entries={entries}, scale={scale})")
-    return ref, nbytes
-
-
-def _place(x: Tensor, dim: int) -> Tuple[Tensor, int]:
-    """The tensor as the kernels read it, and DW_DIST_LAST if its classes lie together."""
-    if x.is_contiguous():
-        return x, 0
-    if x.movedim(dim, -1).is_contiguous():
-        return x, _lib.DW_DIST_LAST
-    return x.contiguous(), 0
-
-
-def _sizes(x: Tensor, dim: int) -> Tuple[int, int, int]:
-    return math.prod(x.shape[:dim]), x.shape[dim], math.prod(x.shape[dim + 1:])
-
-
-def _rows_shape(x: Tensor, dim: int):
-    return x.shape[:dim] + x.shape[dim + 1:]
+    log_prob: Optional[Tensor]       # of the given class; 0 where none is given; None without an index
+    entropy: Tensor                  # of the row's distribution, in nats
+    top_log_prob: Optional[Tensor]   # the `top` most likely classes along the class axis, descending; None for top = 0
+    top_index: Optional[Tensor]      # their indices, int32; ties: the lowest first
 
 
 # Host time counts: a small training step is bound by it, and the interpreter runs cold in the autograd
-# engine's own thread.  So the backward passes find their descriptor made, and the device and stream are
-# read without building torch.cuda.Stream objects where torch has the calls its own compiler uses.
+# engine's own thread.  What a call's shapes and types decide -- every check, the descriptor, the workspace's
+# size -- is worked out once and kept by them (`_lp_plan`, `_ds_plan`); the backward passes get it from the
+# forward's; and the device and stream are read without building torch.cuda.Stream objects where torch
+# has the calls its own compiler uses.
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(device: torch.device, name: str, *args) -> None:
+def _call(device: torch.device, fn, *args) -> None:
     """One library call on the device's current stream (the library launches on the current device)."""
     index = device.index
     if _current_device() == index:
-        rc = getattr(_lib.lib(), name)(*args, _raw_stream(index))
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = getattr(_lib.lib(), name)(*args, _raw_stream(index))
+            rc = fn(*args, _raw_stream(index))
     if rc:
-        _lib.check(rc, name)
-
-
-def _ptr(t: Optional[Tensor]):
-    return None if t is None else t.data_ptr()
+        _lib.check(rc, fn.__name__)
 
 
 def _workspace(x: Tensor, nbytes: int) -> Optional[Tensor]:
@@ -100,44 +70,82 @@ def _workspace(x: Tensor, nbytes: int) -> Optional[Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
 
 
-# ------------------------------------------------------------------------------ log-probabilities
-
-def _lp_desc(x: Tensor, last: int, index: Optional[Tensor], dim: int, scale: float, top: int):
-    outer, V, inner = _sizes(x, dim)
-    flags = last if index is None else last | _INDEX_FLAGS[index.dtype]
-    return _desc("dw_log_probs_workspace_bytes", outer, V, inner, (0, 0, 0), scale, _DTYPES[x.dtype], top, flags)
-
-
-def _lp_forward(x: Tensor, last: int, index: Optional[Tensor], dim: int, top: int, need_stats: bool, ref, nbytes: int):
-    rows = _rows_shape(x, dim)
-    dev = x.device
-    ent = torch.empty(rows, dtype=torch.float32, device=dev)
-    lp = torch.empty_like(ent) if index is not None else torch.empty((0,), dtype=torch.float32, device=dev)
-    stats = torch.empty(rows + (3,), dtype=torch.float32, device=dev) if need_stats else None
-    if last:   # the kernels write the list of a row together, too
-        top_lp = torch.empty(rows + (top,), dtype=torch.float32, device=dev).movedim(-1, dim)
-        top_idx = torch.empty(rows + (top,), dtype=torch.int32, device=dev).movedim(-1, dim)
-    else:
-        shape = x.shape[:dim] + (top,) + x.shape[dim + 1:]
-        top_lp = torch.empty(shape, dtype=torch.float32, device=dev)
-        top_idx = torch.empty(shape, dtype=torch.int32, device=dev)
-    ws = _workspace(x, nbytes)
-    _call(dev, "dw_log_probs_fwd", ref, x.data_ptr(), _ptr(index), lp.data_ptr() if index is not None else None,
-          ent.data_ptr(), top_lp.data_ptr() if top else None, top_idx.data_ptr() if top else None, _ptr(stats),
-          _ptr(ws), nbytes)
-    return lp, ent, top_lp, top_idx, stats
+class _Plan(NamedTuple):
+    """What shapes and types decide."""
+    layout: int        # _IN_PLACE, _LAST, or _COPY: how the kernels read the logits
+    dim: int
+    rows: tuple        # shape without the class axis
+    ref: object        # descriptor, for ctypes
+    nbytes: int        # workspace
+    top: int = 0
+    copy_list: bool = False   # distillation: the teacher's tensors have no common order
 
 
-def _lp_backward(x: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: Optional[Tensor], g_ent: Optional[Tensor],
-                 ref) -> Tensor:
-    grad = torch.empty_like(x)
-    if g_lp is not None:
-        g_lp = g_lp.contiguous() if index is not None else None
-    if g_ent is not None:
-        g_ent = g_ent.contiguous()
-    _call(x.device, "dw_log_probs_bwd", ref, x.data_ptr(), _ptr(index), stats.data_ptr(), _ptr(g_lp), _ptr(g_ent),
-          grad.data_ptr())
-    return grad
+_IN_PLACE, _LAST, _COPY = 0, 1, 2
+
+
+def _contiguous(shape, stride) -> bool:
+    n = 1
+    for size, step in zip(reversed(shape), reversed(stride)):
+        if size != 1:
+            if step != n:
+                return 0 in shape
+            n *= size
+    return True
+
+
+def _moved(t, dim):
+    """Sizes or strides with the class axis moved to the end."""
+    return tuple(t[:dim]) + tuple(t[dim + 1:]) + (t[dim],)
+
+
+def _layout(shape, stride, dim: int) -> int:
+    if _contiguous(shape, stride):
+        return _IN_PLACE
+    return _LAST if _contiguous(_moved(shape, dim), _moved(stride, dim)) else _COPY
+
+
+def _descriptor(workspace_of: str, shape, dim: int, last: bool, dtype, scale: float, entries: int, flags: int,
+                stride=(0, 0, 0)):
+    if last:
+        flags |= _lib.DW_DIST_LAST
+    d = _lib.DwDistDesc(math.prod(shape[:dim]), shape[dim], math.prod(shape[dim + 1:]), stride, scale, _DTYPES[dtype],
+                        entries, flags)
+    ref = C.byref(d)
+    nbytes = getattr(_lib.lib(), workspace_of)(ref)
+    if nbytes < 0:
+        _lib.check(int(nbytes), f"{workspace_of}(shape={tuple(shape)}, entries={entries}, scale={scale})")
+    return ref, nbytes
+
+
+def _check_problem(shape, dtype, dim: int, scale: float) -> int:
+    if dtype not in _DTYPES:
+        raise TypeError(f"logits: expected float32, bfloat16 or float16, got {dtype}")
+    n = len(shape)
+    if not -n <= dim < n:
+        raise ValueError(f"dim: no axis {dim} in logits of shape {tuple(shape)}")
+    dim %= n
+    if shape[dim] == 0:
+        raise ValueError(f"logits: no classes along axis {dim} of {tuple(shape)}")
+    if not math.isfinite(scale) or scale == 0.0:
+        raise ValueError(f"scale: expected a finite number other than 0, got {scale}")
+    return dim
+
+
+def _check_index(name: str, dtype, shape, want) -> None:
+    if dtype not in _INDEX_FLAGS:
+        raise TypeError(f"{name}: expected int32 or int64, got {dtype}")
+    if tuple(shape) != tuple(want):
+        raise ValueError(f"{name}: expected shape {tuple(want)}, got {tuple(shape)}")
+
+
+def _check_device(logits: Tensor, **others: Optional[Tensor]) -> None:
+    if not logits.is_cuda:
+        raise _lib.DepthwarpError(f"logits: expected a ROCm device tensor, got {logits.device} "
+                                  "(the HIP kernels have no CPU path)")
+    for name, t in others.items():
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"{name}: expected a tensor on {logits.device}, got {t.device}")
 
 
 def _once(backward):
@@ -146,66 +154,153 @@ def _once(backward):
     return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
-def _lp_node_backward(ctx, g_lp, g_ent, _g_top, _g_index):
-    logits, index = ctx.saved_tensors
+# ------------------------------------------------------------------------------ log-probabilities
+
+def _lp_check(shape, dtype, index_dtype, index_shape, dim: int, scale: float, top: int) -> int:
+    dim = _check_problem(shape, dtype, dim, scale)
+    most = min(_lib.DW_DIST_MAX_ENTRIES, shape[dim])
+    if not 0 <= top <= most:
+        raise ValueError(f"top: expected 0 to {most}, got {top}")
+    if index_dtype is not None:
+        _check_index("index", index_dtype, index_shape, tuple(shape[:dim]) + tuple(shape[dim + 1:]))
+    return dim
+
+
+def _make_lp_plan(shape, stride, dtype, index_dtype, index_shape, dim: int, scale: float, top: int) -> _Plan:
+    dim = _lp_check(shape, dtype, index_dtype, index_shape, dim, scale, top)
+    layout = _layout(shape, stride, dim)
+    flags = 0 if index_dtype is None else _INDEX_FLAGS[index_dtype]
+    ref, nbytes = _descriptor("dw_log_probs_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, top, flags)
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, nbytes, top)
+
+
+_lp_plan = functools.lru_cache(maxsize=512)(_make_lp_plan)
+
+
+def _plan_of(logits: Tensor, index: Optional[Tensor], dim: int, scale: float, top: int) -> _Plan:
+    if index is None:
+        return _lp_plan(logits.shape, logits.stride(), logits.dtype, None, None, dim, scale, top)
+    return _lp_plan(logits.shape, logits.stride(), logits.dtype, index.dtype, index.shape, dim, scale, top)
+
+
+def _lp_forward(logits: Tensor, index: Optional[Tensor], plan: _Plan, need_stats: bool):
+    x = logits.contiguous() if plan.layout == _COPY else logits
+    dev, rows, top = x.device, plan.rows, plan.top
+    ent = torch.empty(rows, dtype=torch.float32, device=dev)
+    lp = lp_ptr = index_ptr = stats = stats_ptr = top_lp = top_lp_ptr = top_idx = top_idx_ptr = ws = None
+    if index is not None:
+        index = index.contiguous()
+        index_ptr = index.data_ptr()
+        lp = torch.empty(rows, dtype=torch.float32, device=dev)
+        lp_ptr = lp.data_ptr()
+    if need_stats:
+        stats = torch.empty(rows + (3,), dtype=torch.float32, device=dev)
+        stats_ptr = stats.data_ptr()
+    if top:
+        if plan.layout == _LAST:   # the kernels write the list of a row together, too
+            top_lp = torch.empty(rows + (top,), dtype=torch.float32, device=dev).movedim(-1, plan.dim)
+            top_idx = torch.empty(rows + (top,), dtype=torch.int32, device=dev).movedim(-1, plan.dim)
+        else:
+            shape = rows[:plan.dim] + (top,) + rows[plan.dim:]
+            top_lp = torch.empty(shape, dtype=torch.float32, device=dev)
+            top_idx = torch.empty(shape, dtype=torch.int32, device=dev)
+        top_lp_ptr, top_idx_ptr = top_lp.data_ptr(), top_idx.data_ptr()
+        ws = _workspace(x, plan.nbytes)
+    elif plan.nbytes:
+        ws = _workspace(x, plan.nbytes)
+    _call(dev, _lib.lib().dw_log_probs_fwd, plan.ref, x.data_ptr(), index_ptr, lp_ptr, ent.data_ptr(), top_lp_ptr,
+          top_idx_ptr, stats_ptr, None if ws is None else ws.data_ptr(), plan.nbytes)
+    return lp, ent, top_lp, top_idx, stats
+
+
+def _lp_backward(logits: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: Optional[Tensor],
+                 g_ent: Optional[Tensor], plan: _Plan) -> Tensor:
+    x = logits.contiguous() if plan.layout == _COPY else logits
+    grad = torch.empty_like(x)
+    index_ptr = g_lp_ptr = g_ent_ptr = None
+    if index is not None:
+        index = index.contiguous()
+        index_ptr = index.data_ptr()
+        if g_lp is not None:
+            g_lp = g_lp.contiguous()
+            g_lp_ptr = g_lp.data_ptr()
+    if g_ent is not None:
+        g_ent = g_ent.contiguous()
+        g_ent_ptr = g_ent.data_ptr()
+    _call(x.device, _lib.lib().dw_log_probs_bwd, plan.ref, x.data_ptr(), index_ptr, stats.data_ptr(), g_lp_ptr,
+          g_ent_ptr, grad.data_ptr())
+    return grad
+
+
+def _lp_node_backward(ctx, g_lp, g_ent, *_g_top):
     if g_lp is None and g_ent is None:
-        return None, None, None, None, None
-    x = logits if ctx.in_place else logits.contiguous()
-    return _lp_backward(x, index, ctx.stats, g_lp, g_ent, ctx.ref), None, None, None, None
+        return None, None, None
+    logits, index = ctx.saved_tensors
+    return _lp_backward(logits, index, ctx.stats, g_lp, g_ent, ctx.plan), None, None
 
 
 class _LogProbsFunction(torch.autograd.Function):
     """Eager calls with a gradient skip the operator dispatcher."""
 
     @staticmethod
-    def forward(ctx, logits, index, dim, scale, top):
-        x, last = _place(logits, dim)
-        ctx.ref, nbytes = _lp_desc(x, last, index, dim, scale, top)
-        lp, ent, top_lp, top_idx, ctx.stats = _lp_forward(x, last, index, dim, top, True, ctx.ref, nbytes)
+    def forward(ctx, logits, index, plan):
+        lp, ent, top_lp, top_idx, ctx.stats = _lp_forward(logits, index, plan, True)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(top_lp, top_idx)
         ctx.save_for_backward(logits, index)
-        ctx.in_place = x is logits
+        ctx.plan = plan
+        if not plan.top:
+            return lp, ent
+        ctx.mark_non_differentiable(top_lp, top_idx)
         return lp, ent, top_lp, top_idx
 
     backward = staticmethod(_once(_lp_node_backward))
 
 
+# The same as torch operators, which is what torch.compile traces.  An operator always returns tensors:
+# without an index, log_prob is empty; the last result is for the backward pass.
+
 @torch.library.custom_op("depthwarp::log_probs", mutates_args=())
 def _log_probs_op(logits: Tensor, index: Optional[Tensor], dim: int, scale: float,
                   top: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """The same as a torch operator (what torch.compile traces); the last result is the backward's."""
-    x, last = _place(logits, dim)
-    index = None if index is None else index.contiguous()
-    return _lp_forward(x, last, index, dim, top, True, *_lp_desc(x, last, index, dim, scale, top))
+    lp, ent, top_lp, top_idx, stats = _lp_forward(logits, index, _plan_of(logits, index, dim, scale, top), True)
+    if lp is None:
+        lp = ent.new_empty((0,))
+    if not top:
+        top_lp, top_idx = ent.new_empty((0,)), ent.new_empty((0,), dtype=torch.int32)
+    return lp, ent, top_lp, top_idx, stats
 
 
 @_log_probs_op.register_fake
 def _(logits, index, dim, scale, top):
-    x, last = _place(logits, dim)
-    rows = _rows_shape(x, dim)
-    ent = x.new_empty(rows, dtype=torch.float32)
-    lp = torch.empty_like(ent) if index is not None else x.new_empty((0,), dtype=torch.float32)
-    if last:
-        top_lp = x.new_empty(rows + (top,), dtype=torch.float32).movedim(-1, dim)
-        top_idx = x.new_empty(rows + (top,), dtype=torch.int32).movedim(-1, dim)
+    dim %= logits.dim()
+    rows = logits.shape[:dim] + logits.shape[dim + 1:]
+    ent = logits.new_empty(rows, dtype=torch.float32)
+    lp = torch.empty_like(ent) if index is not None else ent.new_empty((0,))
+    if not top:
+        top_lp, top_idx = ent.new_empty((0,)), ent.new_empty((0,), dtype=torch.int32)
+    elif not logits.is_contiguous() and logits.movedim(dim, -1).is_contiguous():
+        top_lp = ent.new_empty(rows + (top,)).movedim(-1, dim)
+        top_idx = ent.new_empty(rows + (top,), dtype=torch.int32).movedim(-1, dim)
     else:
-        shape = x.shape[:dim] + (top,) + x.shape[dim + 1:]
-        top_lp, top_idx = x.new_empty(shape, dtype=torch.float32), x.new_empty(shape, dtype=torch.int32)
-    return lp, ent, top_lp, top_idx, x.new_empty(rows + (3,), dtype=torch.float32)
+        shape = logits.shape[:dim] + (top,) + logits.shape[dim + 1:]
+        top_lp, top_idx = ent.new_empty(shape), ent.new_empty(shape, dtype=torch.int32)
+    return lp, ent, top_lp, top_idx, ent.new_empty(rows + (3,))
+
+
+def _fake_grad(logits: Tensor, dim: int) -> Tensor:
+    in_place = logits.is_contiguous() or logits.movedim(dim, -1).is_contiguous()
+    return torch.empty_like(logits) if in_place else torch.empty_like(logits, memory_format=torch.contiguous_format)
 
 
 @torch.library.custom_op("depthwarp::log_probs_bwd", mutates_args=())
 def _log_probs_bwd_op(logits: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: Optional[Tensor],
                       g_ent: Optional[Tensor], dim: int, scale: float) -> Tensor:
-    x, last = _place(logits, dim)
-    index = None if index is None else index.contiguous()
-    return _lp_backward(x, index, stats, g_lp, g_ent, _lp_desc(x, last, index, dim, scale, 0)[0])
+    return _lp_backward(logits, index, stats, g_lp, g_ent, _plan_of(logits, index, dim, scale, 0))
 
 
 @_log_probs_bwd_op.register_fake
 def _(logits, index, stats, g_lp, g_ent, dim, scale):
-    return torch.empty_like(_place(logits, dim)[0])
+    return _fake_grad(logits, dim)
 
 
 def _lp_setup(ctx, inputs, output):
@@ -223,40 +318,13 @@ def _lp_op_backward(ctx, g_lp, g_ent, _g_top, _g_index, _g_stats):
 _log_probs_op.register_autograd(_lp_op_backward, setup_context=_lp_setup)
 
 
-def _check_logits(logits: Tensor, dim: int, scale: float) -> Tuple[int, float]:
-    if not logits.is_cuda:
-        raise _lib.DepthwarpError(f"logits: expected a ROCm device tensor, got {logits.device} "
-                                  "(the HIP kernels have no CPU path)")
-    if logits.dtype not in _DTYPES:
-        raise TypeError(f"logits: expected float32, bfloat16 or float16, got {logits.dtype}")
-    n = logits.dim()
-    if not -n <= dim < n:
-        raise ValueError(f"dim: no axis {dim} in logits of shape {tuple(logits.shape)}")
-    dim %= n
-    if logits.shape[dim] == 0:
-        raise ValueError(f"logits: no classes along axis {dim} of {tuple(logits.shape)}")
-    scale = float(scale)
-    if not math.isfinite(scale) or scale == 0.0:
-        raise ValueError(f"scale: expected a finite number other than 0, got {scale}")
-    return dim, scale
-
-
-def _check_index(name: str, index: Tensor, shape, device) -> None:
-    if index.dtype not in _INDEX_FLAGS:
-        raise TypeError(f"{name}: expected int32 or int64, got {index.dtype}")
-    if index.shape != shape:
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(index.shape)}")
-    if index.device != device:
-        raise ValueError(f"{name}: expected a tensor on {device}, got {index.device}")
-
-
 def log_probs(logits: Tensor, index: Optional[Tensor] = None, *, dim: int = 1, scale: float = 1.0,
               top: int = 0) -> LogProbs:
     """Scores rows of `logits` against the classes `index` and describes their distribution.
 
     `index` (int32 or int64) has the shape of `logits` without `dim`; a value outside [0, classes) means
     that no class is given there (a pixel without ground truth, or beyond the range): log-probability 0 and
-    no gradient.  `top` (0 to 64) most likely classes come back as log-probabilities and int32 indices, in
+    no gradient.  The `top` (0 to 64) most likely classes come back as log-probabilities and int32 indices, in
     descending order, equal values by lowest index.
 
     `log_prob` and `entropy` are differentiable with respect to `logits`, once; the top lists are not.
@@ -264,79 +332,92 @@ def log_probs(logits: Tensor, index: Optional[Tensor] = None, *, dim: int = 1, s
     gradient 0.  A row with NaN (or +inf) has NaN results.  A row that gets no upstream gradient gets
     zeros whatever it holds.
     """
-    dim, scale = _check_logits(logits, dim, scale)
-    top = int(top)
-    if not 0 <= top <= min(_lib.DW_DIST_MAX_ENTRIES, logits.shape[dim]):
-        raise ValueError(f"top: expected 0 to {min(_lib.DW_DIST_MAX_ENTRIES, logits.shape[dim])}, got {top}")
-    if index is not None:
-        _check_index("index", index, _rows_shape(logits, dim), logits.device)
-        index = index.contiguous()
+    _check_device(logits, index=index)
+    scale, top = float(scale), int(top)
     if torch.compiler.is_compiling():
+        dim = _lp_check(logits.shape, logits.dtype, None if index is None else index.dtype,
+                        None if index is None else index.shape, dim, scale, top)
         lp, ent, top_lp, top_idx, _ = _log_probs_op(logits, index, dim, scale, top)
-    elif logits.requires_grad and torch.is_grad_enabled():
-        lp, ent, top_lp, top_idx = _LogProbsFunction.apply(logits, index, dim, scale, top)
-    else:
-        x, last = _place(logits, dim)
-        lp, ent, top_lp, top_idx, _ = _lp_forward(x, last, index, dim, top, False,
-                                                  *_lp_desc(x, last, index, dim, scale, top))
-    return LogProbs(lp if index is not None else None, ent, top_lp, top_idx)
+        return LogProbs(None if index is None else lp, ent, top_lp if top else None, top_idx if top else None)
+    plan = _plan_of(logits, index, dim, scale, top)
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _LogProbsFunction.apply(logits, index, plan)
+        return LogProbs(*out) if top else LogProbs(*out, None, None)
+    return LogProbs(*_lp_forward(logits, index, plan, False)[:4])
 
 
 # --------------------------------------------------------------------------------- distillation
 
-def _entries(teacher: Tensor, index: Tensor, dim: int):
-    """The list's two tensors in one memory order, and its element strides along outer, entry, inner."""
-    if not (teacher.is_contiguous() and index.is_contiguous()):
-        if teacher.movedim(dim, -1).is_contiguous() and index.movedim(dim, -1).is_contiguous():
-            _, k, inner = _sizes(teacher, dim)
-            return teacher, index, (k * inner, 1, k)
+def _ds_check(shape, dtype, t_shape, t_dtype, i_shape, i_dtype, dim: int, scale: float) -> int:
+    dim = _check_problem(shape, dtype, dim, scale)
+    if t_dtype not in _TEACHER_FLAGS:
+        raise TypeError(f"teacher: expected float32, bfloat16 or float16, got {t_dtype}")
+    k = t_shape[dim] if len(t_shape) == len(shape) else 0
+    want = tuple(shape[:dim]) + (k,) + tuple(shape[dim + 1:])
+    if not 1 <= k <= _lib.DW_DIST_MAX_ENTRIES or tuple(t_shape) != want:
+        raise ValueError(f"teacher: expected the shape of the logits {tuple(shape)} with 1 to "
+                         f"{_lib.DW_DIST_MAX_ENTRIES} entries along axis {dim}, got {tuple(t_shape)}")
+    _check_index("teacher_index", i_dtype, i_shape, want)
+    return dim
+
+
+def _make_ds_plan(shape, stride, dtype, t_shape, t_stride, t_dtype, i_shape, i_stride, i_dtype, dim: int,
+                  scale: float, renormalise: bool) -> _Plan:
+    dim = _ds_check(shape, dtype, t_shape, t_dtype, i_shape, i_dtype, dim, scale)
+    k, inner = t_shape[dim], math.prod(t_shape[dim + 1:])
+    # the list's element strides along outer, entry, inner: its tensors as they are if they share an order
+    t_layout, i_layout = _layout(t_shape, t_stride, dim), _layout(i_shape, i_stride, dim)
+    copy = t_layout != i_layout or t_layout == _COPY
+    strides = (k * inner, 1, k) if not copy and t_layout == _LAST else (k * inner, inner, 1)
+    layout = _layout(shape, stride, dim)
+    flags = _INDEX_FLAGS[i_dtype] | _TEACHER_FLAGS[t_dtype] | (_lib.DW_DIST_RENORMALISE if renormalise else 0)
+    ref, nbytes = _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k, flags, strides)
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, nbytes, copy_list=copy)
+
+
+_ds_plan = functools.lru_cache(maxsize=512)(_make_ds_plan)
+
+
+def _ds_plan_of(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale: float, renormalise: bool) -> _Plan:
+    return _ds_plan(logits.shape, logits.stride(), logits.dtype, teacher.shape, teacher.stride(), teacher.dtype,
+                    index.shape, index.stride(), index.dtype, dim, scale, renormalise)
+
+
+def _ds_forward(logits: Tensor, teacher: Tensor, index: Tensor, plan: _Plan, need_stats: bool):
+    x = logits.contiguous() if plan.layout == _COPY else logits
+    if plan.copy_list:
         teacher, index = teacher.contiguous(), index.contiguous()
-    _, k, inner = _sizes(teacher, dim)
-    return teacher, index, (k * inner, inner, 1)
-
-
-def _ds_desc(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale: float, renormalise: bool):
-    x, last = _place(logits, dim)
-    teacher, index, stride = _entries(teacher, index, dim)
-    outer, V, inner = _sizes(x, dim)
-    flags = last | _INDEX_FLAGS[index.dtype] | _TEACHER_FLAGS[teacher.dtype]
-    if renormalise:
-        flags |= _lib.DW_DIST_RENORMALISE
-    return x, teacher, index, _desc("dw_distill_workspace_bytes", outer, V, inner, stride, scale, _DTYPES[x.dtype],
-                                    teacher.shape[dim], flags)
-
-
-def _ds_forward(x: Tensor, teacher: Tensor, index: Tensor, dim: int, need_stats: bool, ref, nbytes: int):
-    rows = _rows_shape(x, dim)
-    loss = torch.empty(rows, dtype=torch.float32, device=x.device)
-    stats = torch.empty(rows + (4,), dtype=torch.float32, device=x.device) if need_stats else None
-    ws = _workspace(x, nbytes)
-    _call(x.device, "dw_distill_fwd", ref, x.data_ptr(), teacher.data_ptr(), index.data_ptr(), loss.data_ptr(),
-          _ptr(stats), _ptr(ws), nbytes)
+    loss = torch.empty(plan.rows, dtype=torch.float32, device=x.device)
+    stats = torch.empty(plan.rows + (4,), dtype=torch.float32, device=x.device) if need_stats else None
+    ws = _workspace(x, plan.nbytes)
+    _call(x.device, _lib.lib().dw_distill_fwd, plan.ref, x.data_ptr(), teacher.data_ptr(), index.data_ptr(),
+          loss.data_ptr(), None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(),
+          plan.nbytes)
     return loss, stats
 
 
-def _ds_backward(x: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, g_loss: Tensor, ref) -> Tensor:
+def _ds_backward(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, g_loss: Tensor, plan: _Plan) -> Tensor:
+    x = logits.contiguous() if plan.layout == _COPY else logits
+    if plan.copy_list:
+        teacher, index = teacher.contiguous(), index.contiguous()
     grad = torch.empty_like(x)
     g_loss = g_loss.contiguous()
-    _call(x.device, "dw_distill_bwd", ref, x.data_ptr(), teacher.data_ptr(), index.data_ptr(), stats.data_ptr(),
-          g_loss.data_ptr(), grad.data_ptr())
+    _call(x.device, _lib.lib().dw_distill_bwd, plan.ref, x.data_ptr(), teacher.data_ptr(), index.data_ptr(),
+          stats.data_ptr(), g_loss.data_ptr(), grad.data_ptr())
     return grad
 
 
 def _ds_node_backward(ctx, g_loss):
     logits, teacher, index = ctx.saved_tensors
-    x = logits if ctx.in_place else logits.contiguous()
-    return _ds_backward(x, teacher, index, ctx.stats, g_loss, ctx.ref), None, None, None, None, None
+    return _ds_backward(logits, teacher, index, ctx.stats, g_loss, ctx.plan), None, None, None
 
 
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher, index, dim, scale, renormalise):
-        x, teacher, index, (ctx.ref, nbytes) = _ds_desc(logits, teacher, index, dim, scale, renormalise)
-        loss, ctx.stats = _ds_forward(x, teacher, index, dim, True, ctx.ref, nbytes)
+    def forward(ctx, logits, teacher, index, plan):
+        loss, ctx.stats = _ds_forward(logits, teacher, index, plan, True)
         ctx.save_for_backward(logits, teacher, index)
-        ctx.in_place = x is logits
+        ctx.plan = plan
         return loss
 
     backward = staticmethod(_once(_ds_node_backward))
@@ -345,26 +426,26 @@ class _DistillFunction(torch.autograd.Function):
 @torch.library.custom_op("depthwarp::distill_loss", mutates_args=())
 def _distill_op(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale: float,
                 renormalise: bool) -> Tuple[Tensor, Tensor]:
-    x, teacher, index, plan = _ds_desc(logits, teacher, index, dim, scale, renormalise)
-    return _ds_forward(x, teacher, index, dim, True, *plan)
+    return _ds_forward(logits, teacher, index, _ds_plan_of(logits, teacher, index, dim, scale, renormalise), True)
 
 
 @_distill_op.register_fake
 def _(logits, teacher, index, dim, scale, renormalise):
-    rows = _rows_shape(logits, dim)
+    dim %= logits.dim()
+    rows = logits.shape[:dim] + logits.shape[dim + 1:]
     return logits.new_empty(rows, dtype=torch.float32), logits.new_empty(rows + (4,), dtype=torch.float32)
 
 
 @torch.library.custom_op("depthwarp::distill_loss_bwd", mutates_args=())
 def _distill_bwd_op(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, g_loss: Tensor, dim: int,
                     scale: float, renormalise: bool) -> Tensor:
-    x, teacher, index, (ref, _) = _ds_desc(logits, teacher, index, dim, scale, renormalise)
-    return _ds_backward(x, teacher, index, stats, g_loss, ref)
+    return _ds_backward(logits, teacher, index, stats, g_loss,
+                        _ds_plan_of(logits, teacher, index, dim, scale, renormalise))
 
 
 @_distill_bwd_op.register_fake
 def _(logits, teacher, index, stats, g_loss, dim, scale, renormalise):
-    return torch.empty_like(_place(logits, dim)[0])
+    return _fake_grad(logits, dim)
 
 
 def _ds_setup(ctx, inputs, output):
@@ -397,24 +478,15 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
     without entries has loss and gradient 0.  A class listed twice counts with both entries.  The loss
     is +inf where the teacher lists a class the student has at -inf.
     """
-    dim, scale = _check_logits(logits, dim, scale)
-    if teacher.dtype not in _TEACHER_FLAGS:
-        raise TypeError(f"teacher: expected float32, bfloat16 or float16, got {teacher.dtype}")
-    k = teacher.shape[dim] if teacher.dim() == logits.dim() else 0
-    shape = logits.shape[:dim] + (k,) + logits.shape[dim + 1:]
-    if not 1 <= k <= _lib.DW_DIST_MAX_ENTRIES or teacher.shape != shape:
-        raise ValueError(f"teacher: expected the shape of the logits {tuple(logits.shape)} with 1 to "
-                         f"{_lib.DW_DIST_MAX_ENTRIES} entries along axis {dim}, got {tuple(teacher.shape)}")
-    if teacher.device != logits.device:
-        raise ValueError(f"teacher: expected a tensor on {logits.device}, got {teacher.device}")
-    _check_index("teacher_index", teacher_index, teacher.shape, logits.device)
-    grad = torch.is_grad_enabled()
-    if grad and teacher.requires_grad:
+    _check_device(logits, teacher=teacher, teacher_index=teacher_index)
+    scale, renormalise = float(scale), bool(renormalise)
+    if teacher.requires_grad and torch.is_grad_enabled():
         raise ValueError("teacher: no gradient flows to the teacher; pass teacher.detach()")
-    renormalise = bool(renormalise)
     if torch.compiler.is_compiling():
+        dim = _ds_check(logits.shape, logits.dtype, teacher.shape, teacher.dtype, teacher_index.shape,
+                        teacher_index.dtype, dim, scale)
         return _distill_op(logits, teacher, teacher_index, dim, scale, renormalise)[0]
-    if grad and logits.requires_grad:
-        return _DistillFunction.apply(logits, teacher, teacher_index, dim, scale, renormalise)
-    x, teacher, teacher_index, plan = _ds_desc(logits, teacher, teacher_index, dim, scale, renormalise)
-    return _ds_forward(x, teacher, teacher_index, dim, False, *plan)[0]
+    plan = _ds_plan_of(logits, teacher, teacher_index, dim, scale, renormalise)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _DistillFunction.apply(logits, teacher, teacher_index, plan)
+    return _ds_forward(logits, teacher, teacher_index, plan, False)[0]
