@@ -27,6 +27,7 @@ using namespace dw;
 constexpr float kInf = __builtin_inff();
 constexpr float kLn2 = 0x1.62e43p-1f;      // fl(ln 2)
 constexpr float kLog2e = 0x1.715476p+0f;   // fl(log2 e)
+constexpr float kLog2eRest = 0x1.4ae0cp-26f;  // log2 e - fl(log2 e)
 constexpr float kFloor = -1e30f;           // stands in for an exponent of -inf where 0 * -inf would be NaN
 constexpr int kMaxEntries = 64;
 
@@ -155,6 +156,13 @@ struct Side {
   }
 };
 __device__ __forceinline__ float exp2_(float t) { return __builtin_amdgcn_exp2f(t); }
+// e^x: the rounding of x log2 e is put right to first order, so the error stays at two steps for any x.  (For
+// |x| so large that the correction is infinite or NaN the power is 0, inf or NaN by itself.)
+__device__ __forceinline__ float exp_(float x) {
+  const float t = x * kLog2e, p = exp2_(t);
+  const float r = fmaf(x, kLog2e, -t) + x * kLog2eRest;
+  return p == 0.f || p == kInf ? p : fmaf(p, r * kLn2, p);
+}
 
 // Hides where a value comes from, so that addresses are formed from it where they are used, not kept in a
 // register pair each across the loop
@@ -199,8 +207,9 @@ using Stats3 = Acc;  // what the backward pass gets of a row; m is 0 in an empty
 __device__ __forceinline__ float entropy_of(float s, float w, float ln_s) { return s == 0.f ? 0.f : ln_s - kLn2 * w / s; }
 __device__ __forceinline__ Acc acc_empty(const Side& z) { return Acc{z.far(), 0.f, 0.f}; }
 
+// top: best_of(v); nothing possible stands behind the n-th value
 template <bool ENT, int N>
-__device__ __forceinline__ void absorb(Acc& a, const float (&v)[N], float top, const Side& z) {  // top: best_of(v)
+__device__ __forceinline__ void absorb(Acc& a, const float (&v)[N], int n, float top, const Side& z) {
   const float m = z.best(a.m, top);
   const float b = m == z.far() ? 0.f : m;
   const float d = fmaxf((a.m - b) * z.c, kFloor), al = exp2_(d);
@@ -208,6 +217,7 @@ __device__ __forceinline__ void absorb(Acc& a, const float (&v)[N], float top, c
   a.s *= al;
 #pragma unroll
   for (int i = 0; i < N; i += 8) {
+    if (i >= n) break;
     float t[8], e[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) t[k] = (v[i + k] - b) * z.c;
@@ -419,8 +429,20 @@ __device__ __forceinline__ Place place(const Prob& p, unsigned block) {
     q.skip = (int)(own - q.first);
     q.row = q.first + q.lane;
     q.live = q.lane >= q.skip;
-    q.o = p.inner == 1 ? q.row : q.row / p.inner;
-    q.i = p.inner == 1 ? 0 : q.row - q.o * p.inner;
+    if (p.inner == 1) {
+      q.o = q.row;
+      q.i = 0;
+    } else if (p.inner >= 64) {  // the block's rows lie in one or two outer ones: one division, a scalar one
+      q.o = q.first / p.inner;
+      q.i = q.first - q.o * p.inner + q.lane;
+      if (q.i >= p.inner) {
+        q.i -= p.inner;
+        q.o += 1;
+      }
+    } else {
+      q.o = q.row / p.inner;
+      q.i = q.row - q.o * p.inner;
+    }
   } else {
     const unsigned tiles = (unsigned)((p.inner + 63) / 64);
     q.o = block / tiles;
@@ -472,8 +494,13 @@ struct Feed<T, true> {  // 64 row segments of classes [c0, c0 + n), 8 lanes a ro
     } else {
 #pragma unroll
       for (int it = 0; it < PER; ++it) {
-        if (j + T::VEC <= n) v[it] = load_vec<T>(x + off, at);
-        else v[it] = load_some<T>(x + off, at, n - j);
+        // what a vector reaches of the next row is read and not used; behind the last row nothing is read
+        const int64_t left = (p.rows - q.first - it * (64 / PER) - q.lane / PER) * p.V - c0 - j;
+        v[it].d = u32x4{0, 0, 0, 0};
+        if (j < n) {
+          if (left >= T::VEC) v[it] = load_vec<T>(x + off, at);
+          else v[it] = load_some<T>(x + off, at, n - j);
+        }
         off = fresh_uniform(off + (64 / PER) * p.V);
       }
     }
@@ -553,7 +580,7 @@ __device__ __forceinline__ void stage_write(char* lds, int lane, int h, const fl
 }
 template <class T>
 __device__ __forceinline__ void planes_out(typename T::S* g, const Prob& p, const Place& q, int c0, int n,
-                                           const float (&v)[32]) {
+                                           const typename T::S (&v)[32]) {
   using S = typename T::S;
   Global<S> plane = (Global<S>)(g + (q.o * p.V + c0) * p.inner + q.first);
   const unsigned at = fresh((unsigned)(q.i - q.first) * (unsigned)sizeof(S));
@@ -562,7 +589,7 @@ __device__ __forceinline__ void planes_out(typename T::S* g, const Prob& p, cons
 #pragma unroll
     for (int u = 0; u < 32; ++u) {
       plane = scalar_base(plane);
-      *at_byte<S>(plane, at) = T::down(v[u]);
+      *at_byte<S>(plane, at) = v[u];
       plane += p.inner;
     }
   } else {
@@ -570,7 +597,7 @@ __device__ __forceinline__ void planes_out(typename T::S* g, const Prob& p, cons
 #pragma unroll
     for (int u = 0; u < 32; ++u) {
       plane = scalar_base(plane);
-      if (u < m) *at_byte<S>(plane, at) = T::down(v[u]);
+      if (u < m) *at_byte<S>(plane, at) = v[u];
       plane += p.inner;
     }
   }
@@ -603,8 +630,11 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
 
   // the given class, on its way while the classes are read
-  const int given = index ? valid_index(load_index(index, q.row, p.flags), p.V) : -1;
-  const float x_given = given >= 0 ? T::up(x[element<LAST>(p, q, given)]) : 0.f;
+  const int64_t given_raw = index ? load_index(index, q.row, p.flags) : -1;
+  Feed<T, LAST> feed;
+  if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
+  const int given = valid_index(given_raw, p.V);
+  const typename T::S x_given = given >= 0 ? x[element<LAST>(p, q, given)] : typename T::S(0);
 
   Acc a = acc_empty(z);
   double limit = 0.0;
@@ -613,8 +643,7 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
     double top[K ? K : 1];
 #pragma unroll
     for (int i = 0; i < K; ++i) top[i] = kKeyNone;
-    Feed<T, LAST> feed;
-    if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
+    if (done > 0 && c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
     for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
       const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
       float v[32];
@@ -629,7 +658,7 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
       for (int h = 0; h < n; h += 32) {
         if (LAST) stage_read<T>(stage, q.lane, h, v);
         settle(v, z.far(), n - h);
-        if (done == 0) absorb<true>(a, v, z.best_of(v), z);
+        if (done == 0) absorb<true>(a, v, n - h, z.best_of(v), z);
         if constexpr (K > 0) {
           const bool nan = __any(a.s != a.s);  // NaN or +inf in some row
 #pragma unroll
@@ -684,7 +713,7 @@ __global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
       base = a.m == z.far() ? 0.f : a.m;
       ln_s = logf(a.s);
       if (q.wave == 0 && q.live) {
-        const float lp = given >= 0 ? log_p(x_given, base, ln_s, p.scale) : 0.f;
+        const float lp = given >= 0 ? log_p(T::up(x_given), base, ln_s, p.scale) : 0.f;
         if (log_prob) log_prob[q.row] = lp;
         if (entropy) entropy[q.row] = entropy_of(a.s, a.w, ln_s);
         if (stats) stats[q.row] = Stats3{base, a.s, a.w};
@@ -744,11 +773,11 @@ __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
   char* stage = smem + q.wave * kStageBytes;
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
-  const LpCoef r = lp_coef<ENT>(p, q.row, index, stats, g_lp, g_ent);
-  const bool any_dead = __any(r.dead);
   constexpr int CH = stage_classes<T, LAST>();
   Feed<T, LAST> feed;
   if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
+  const LpCoef r = lp_coef<ENT>(p, q.row, index, stats, g_lp, g_ent);
+  const bool any_dead = __any(r.dead);
   for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
     const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
     float v[32];
@@ -776,7 +805,10 @@ __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
       if (LAST) {
         stage_write<T>(stage, q.lane, h, v);
       } else {
-        planes_out<T>(g, p, q, c0, n, v);
+        typename T::S raw[32];
+#pragma unroll
+        for (int u = 0; u < 32; ++u) raw[u] = T::down(v[u]);
+        planes_out<T>(g, p, q, c0, n, raw);
       }
     }
     if (LAST) {
@@ -809,12 +841,12 @@ __device__ __forceinline__ float4 distill_stats(const RowSums& r, float c, float
   return st;
 }
 
-// Column of this lane's row inside the stage: planes [class][64] float32, or the row's own bytes.  What a
+// Column of this lane's row inside the stage: planes [class][64], or the row's own bytes.  What a
 // lane does for a listed class that is not in the stage goes to a place of its own behind the column.
 template <class T, bool LAST>
 struct Column {
-  using S = std::conditional_t<LAST, typename T::S, float>;
-  using M = std::conditional_t<LAST, T, F32>;
+  using S = typename T::S;
+  using M = T;
   static constexpr int kNowhere = LAST ? kSegBytes / (int)sizeof(S) : 32;
   char* lds;
   int lane;
@@ -822,13 +854,12 @@ struct Column {
     return LAST ? (S*)(lds + lane * kRowBytes) + u : (S*)lds + u * 64 + lane;
   }
 };
-template <bool LAST>
-constexpr int distill_stage_bytes() { return LAST ? kStageBytes : 33 * 64 * 4; }
+constexpr int distill_stage_bytes(bool last, int esize) { return last ? kStageBytes : 33 * 64 * esize; }
 constexpr int kGroup = 8;  // entries handled at once: their LDS accesses overlap
 __host__ __device__ constexpr int padded(int k) { return (k + kGroup - 1) / kGroup * kGroup; }
 // LDS of a block besides the stages: columns of 64 lanes, of list entries and of the waves' sums
 __host__ __device__ constexpr size_t distill_lds(int nw, int k, bool backward) {
-  return (size_t)256 * (padded(k) * 3 + 1 + (backward ? 0 : 2 * nw));
+  return (size_t)256 * (padded(k) * (backward ? 3 : 2) + 1 + (backward || nw == 1 ? 0 : 2 * nw));
 }
 
 template <class S>
@@ -837,21 +868,22 @@ __device__ __forceinline__ void read_group(const S* column, int e0, S (&v)[kGrou
   for (int i = 0; i < kGroup; ++i) v[i] = column[(e0 + i) * 64];
 }
 // Natural log of what the listed values' exponentials sum to (0 where that is nothing): the shift that
-// makes log-probabilities of them.  Padding holds -inf.
-__device__ __forceinline__ float list_shift(const float* tl, int KP) {
+// makes log-probabilities of them.  group(e0, l) gives eight of the values, -inf for padding.
+template <class G>
+__device__ __forceinline__ float list_shift(int KP, G group) {
   float tm = -kInf, ts = 0.f;  // fmaxf drops a NaN; the sum brings it back
   for (int e0 = 0; e0 < KP; e0 += kGroup) {
     float l[kGroup];
-    read_group(tl, e0, l);
+    group(e0, l);
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) tm = fmaxf(tm, l[i]);
   }
   if (tm == -kInf) tm = 0.f;
   for (int e0 = 0; e0 < KP; e0 += kGroup) {
     float l[kGroup];
-    read_group(tl, e0, l);
+    group(e0, l);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) ts += expf(l[i] - tm);
+    for (int i = 0; i < kGroup; ++i) ts += exp_(l[i] - tm);
   }
   return ts == 0.f ? 0.f : tm + logf(ts);
 }
@@ -895,12 +927,11 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   extern __shared__ __align__(16) char smem[];
   const Place q = place<LAST>(p, blockIdx.x);
   const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
-  char* stage = smem + q.wave * distill_stage_bytes<LAST>();
-  char* rest = smem + nw * distill_stage_bytes<LAST>();
+  char* stage = smem + q.wave * distill_stage_bytes(LAST, sizeof(typename T::S));
+  char* rest = smem + nw * distill_stage_bytes(LAST, sizeof(typename T::S));
   int* idx = (int*)rest + q.lane;                            // [KP][64]
-  float* tl = (float*)rest + KP * 64 + q.lane;               // [KP][64]: the teacher's values, -inf for padding
-  float* xs = (float*)rest + 2 * KP * 64 + q.lane;           // [KP + 1][64]: the listed classes' values
-  float* red = (float*)rest + (3 * KP + 1) * 64 + q.lane;    // [2][nw][64]
+  float* xs = (float*)rest + KP * 64 + q.lane;               // [KP + 1][64]: the listed classes' values
+  float* red = (float*)rest + (2 * KP + 1) * 64 + q.lane;    // [2][nw][64], where there are several waves
   const Column<T, LAST> col{stage, q.lane};
   constexpr int CH = stage_classes<T, LAST>();
   const Side z = side(p);
@@ -911,16 +942,15 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
 
   for (int e0 = q.wave * kGroup; e0 < KP; e0 += nw * kGroup) {
     int i8[kGroup];
-    float l8[kGroup];
     load_indices(p, index, t0, e0, i8);
-    load_teachers(p, teacher, t0, e0, l8);
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
       idx[(e0 + i) * 64] = i8[i];
-      tl[(e0 + i) * 64] = i8[i] >= 0 ? l8[i] : -kInf;
       xs[(e0 + i) * 64] = z.far();
     }
   }
+  float first[kGroup];  // the teacher's first values: in most lists all of them
+  load_teachers(p, teacher, t0, 0, first);
   __syncthreads();
   bool alive = false;
   for (int e0 = 0; e0 < KP; e0 += kGroup) {
@@ -938,9 +968,8 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
       if constexpr (LAST) {
         feed.to_lds(q, stage);
       } else {
-        feed.take(v);
 #pragma unroll
-        for (int u = 0; u < 32; ++u) *(float*)col.at(u) = v[u];
+        for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
       }
       if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
       wave_sync();
@@ -951,19 +980,31 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
           stage_read<T>(stage, q.lane, h, v);
         } else {
 #pragma unroll
-          for (int u = 0; u < 32; ++u) v[u] = *(const float*)col.at(u);
+          for (int u = 0; u < 32; ++u) v[u] = T::up(*col.at(u));
         }
         settle(v, z.far(), n - h);
-        absorb<false>(a, v, z.best_of(v), z);
+        absorb<false>(a, v, n - h, z.best_of(v), z);
       }
     }
   }
-  red[q.wave * 64] = a.m;
-  red[(nw + q.wave) * 64] = a.s;
-  __syncthreads();
-  if (q.wave != 0 || !q.live) return;
-  a = Acc{red[0], red[nw * 64], 0.f};
-  for (int w = 1; w < nw; ++w) a = acc_join(a, Acc{red[w * 64], red[(nw + w) * 64], 0.f}, z);
+  if (nw > 1) {
+    red[q.wave * 64] = a.m;
+    red[(nw + q.wave) * 64] = a.s;
+    __syncthreads();
+    if (q.wave != 0) return;
+    a = Acc{red[0], red[nw * 64], 0.f};
+    for (int w = 1; w < nw; ++w) a = acc_join(a, Acc{red[w * 64], red[(nw + w) * 64], 0.f}, z);
+  } else {
+    wave_sync();
+  }
+  if (!q.live) return;
+  const auto values = [&](int e0, float (&l)[kGroup]) {
+    int i8[kGroup];
+    read_group(idx, e0, i8);
+    if (e0 > 0) load_teachers(p, teacher, t0, e0, l);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) l[i] = i8[i] < 0 ? -kInf : e0 > 0 ? l[i] : first[i];
+  };
 
   RowSums r;
   r.m_r = a.m;
@@ -984,15 +1025,15 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
     for (int i = 0; i < kGroup; ++i) r.s += exp2_((v[i] - r.b) * p.c);
   }
   r.ln_s = logf(r.s);
-  const float shift = (p.flags & kRenorm) ? list_shift(tl, KP) : 0.f;
+  const float shift = (p.flags & kRenorm) ? list_shift(KP, values) : 0.f;
   float mass = 0.f, l = 0.f;
   for (int e0 = 0; e0 < KP; e0 += kGroup) {
     float v[kGroup], t[kGroup];
     read_group(xs, e0, v);
-    read_group(tl, e0, t);
+    values(e0, t);
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
-      const float lq = t[i] - shift, qe = expf(lq);  // 0 for padding
+      const float lq = t[i] - shift, qe = exp_(lq);  // 0 for padding
       mass += qe;
       if (v[i] == z.far() && idx[(e0 + i) * 64] >= 0) v[i] = xs[listed_before(idx, e0 + i) * 64];
       if (qe != 0.f) l = fmaf(qe, lq - log_p(v[i], r.b, r.ln_s, p.scale), l);
@@ -1012,8 +1053,8 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
   extern __shared__ __align__(16) char smem[];
   const Place q = place<LAST>(p, block_from_end());
   const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
-  char* stage = smem + q.wave * distill_stage_bytes<LAST>();
-  char* rest = smem + nw * distill_stage_bytes<LAST>();
+  char* stage = smem + q.wave * distill_stage_bytes(LAST, sizeof(typename T::S));
+  char* rest = smem + nw * distill_stage_bytes(LAST, sizeof(typename T::S));
   int* idx = (int*)rest + q.lane;                    // [KP][64]
   float* gq = (float*)rest + KP * 64 + q.lane;       // [KP][64]: upstream gradient * scale * teacher's probability
   float* gv = (float*)rest + 2 * KP * 64 + q.lane;   // [KP + 1][64]: the listed classes' gradients
@@ -1040,16 +1081,16 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
     for (int i = 0; i < kGroup; ++i) {
       if (dead) i8[i] = -1;
       idx[(e0 + i) * 64] = i8[i];
-      gq[(e0 + i) * 64] = i8[i] < 0 ? (renorm ? -kInf : 0.f) : renorm ? l8[i] : gs * expf(l8[i]);
+      gq[(e0 + i) * 64] = i8[i] < 0 ? (renorm ? -kInf : 0.f) : renorm ? l8[i] : gs * exp_(l8[i]);
     }
   }
   if (renorm) {  // values first, probabilities when their sum is known
     __syncthreads();
-    const float shift = list_shift(gq, KP);
+    const float shift = list_shift(KP, [&](int e0, float (&l)[kGroup]) { read_group(gq, e0, l); });
     __syncthreads();
     for (int e0 = q.wave * kGroup; e0 < KP; e0 += nw * kGroup) {
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) gq[(e0 + i) * 64] = gs * expf(gq[(e0 + i) * 64] - shift);
+      for (int i = 0; i < kGroup; ++i) gq[(e0 + i) * 64] = gs * exp_(gq[(e0 + i) * 64] - shift);
     }
   }
   __syncthreads();
@@ -1063,7 +1104,7 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
     } else {
       feed.take(v);
 #pragma unroll
-      for (int u = 0; u < 32; ++u) *(float*)col.at(u) = v[u];
+      for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
     }
     if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
     wave_sync();
@@ -1093,7 +1134,7 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
         stage_write<T>(stage, q.lane, h, v);
       } else {
 #pragma unroll
-        for (int u = 0; u < 32; ++u) *(float*)col.at(u) = v[u];
+        for (int u = 0; u < 32; ++u) *col.at(u) = T::down(v[u]);
       }
     }
     wave_sync();
@@ -1108,9 +1149,10 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
     if (LAST) {
       stage_out<T>(g, p, q, c0, n, stage);
     } else {
+      typename T::S raw[32];
 #pragma unroll
-      for (int u = 0; u < 32; ++u) v[u] = *(const float*)col.at(u);
-      planes_out<T>(g, p, q, c0, n, v);
+      for (int u = 0; u < 32; ++u) raw[u] = *col.at(u);
+      planes_out<T>(g, p, q, c0, n, raw);
     }
   }
 }
@@ -1121,20 +1163,6 @@ constexpr int kWaveTile = 64 * 32;
 template <class T>
 __device__ __forceinline__ int tile_class(int lane, int u) {  // class of a lane's u-th value inside the wave's tile
   return (u / T::VEC) * 64 * T::VEC + lane * T::VEC + u % T::VEC;
-}
-template <class T>
-__device__ __forceinline__ void row_in(const typename T::S* row, int base, int end, int lane, float far, float (&v)[32]) {
-  const unsigned first = fresh((unsigned)(base + lane * T::VEC));
-#pragma unroll
-  for (int u = 0; u < 32 / T::VEC; ++u) {
-    const unsigned j = first + u * 64 * T::VEC;
-    const int n = end - (int)j;
-    const Vec<T> w = n >= T::VEC ? load_vec<T>(row, j * (unsigned)sizeof(typename T::S))
-                                 : load_some<T>(row, j * (unsigned)sizeof(typename T::S), n);
-#pragma unroll
-    for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = e < n ? w.get(e) : far;
-    __builtin_amdgcn_sched_barrier(0);
-  }
 }
 template <class T>
 __device__ __forceinline__ void row_out(typename T::S* row, int base, int end, int lane, const float (&v)[32]) {
@@ -1179,27 +1207,53 @@ struct RowFeed {
 #pragma unroll
     for (int u = 0; u < 32; ++u) v[u] = w[u / T::VEC].get(u % T::VEC);
   }
+  __device__ __forceinline__ void issue_some(const typename T::S* row, int base, int end, int lane) {
+    const unsigned first = fresh((unsigned)(base + lane * T::VEC));
+#pragma unroll
+    for (int u = 0; u < 32 / T::VEC; ++u) {
+      const unsigned j = first + u * 64 * T::VEC;
+      const int n = end - (int)j;
+      w[u].d = u32x4{0, 0, 0, 0};
+      if (n >= T::VEC) w[u] = load_vec<T>(row, j * (unsigned)sizeof(typename T::S));
+      else if (n > 0) w[u] = load_some<T>(row, j * (unsigned)sizeof(typename T::S), n);
+    }
+  }
+  __device__ __forceinline__ void take_some(int base, int end, int lane, float far, float (&v)[32]) const {
+#pragma unroll
+    for (int u = 0; u < 32 / T::VEC; ++u) {
+      const int n = end - (base + lane * T::VEC + u * 64 * T::VEC);
+#pragma unroll
+      for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = e < n ? w[u].get(e) : far;
+    }
+  }
 };
-// f(v, base, it, full) for every block-wide step `it` of [begin, end): first the steps that are full for every
-// wave, then at most one that is not (v is all `far` for a wave that has nothing left)
+// f(v, base, it, full) for every block-wide step `it` of [begin, end) (v is all `far` for a wave that has nothing
+// in a step).  The step that is not full for every wave comes second: its loads are on their way early.
 template <class T, int NT, class F>
 __device__ __forceinline__ void walk_row(const typename T::S* row, int begin, int end, int lane, int wave, float far, F f) {
   const int full = (end - begin) / (NT * 32);
   int base = begin + wave * kWaveTile;
+  const int rest = base + full * NT * 32;
+  const bool some = begin + full * NT * 32 < end;
+  RowFeed<T> feed, part;
+  if (full > 0) feed.issue(row, base, lane);
+  if (some) part.issue_some(row, rest, end, lane);
+  float v[32];
   if (full > 0) {
-    RowFeed<T> feed;
-    feed.issue(row, base, lane);
-    for (int it = 0; it < full; ++it, base += NT * 32) {
-      float v[32];
-      feed.take(v);
-      if (it + 1 < full) feed.issue(row, base + NT * 32, lane);
-      f(v, base, it, std::true_type{});
-    }
+    feed.take(v);
+    if (full > 1) feed.issue(row, base + NT * 32, lane);
+    f(v, base, 0, std::true_type{});
   }
-  if (begin + full * NT * 32 < end) {
-    float v[32];
-    row_in<T>(row, base, end, lane, far, v);
-    f(v, base, full, std::false_type{});
+  if (some) {
+    part.take_some(rest, end, lane, far, v);
+    f(v, rest, full > 0 ? 1 : 0, std::false_type{});
+  }
+  for (int it = 1; it < full; ++it) {
+    base += NT * 32;
+    float w[32];
+    feed.take(w);
+    if (it + 1 < full) feed.issue(row, base + NT * 32, lane);
+    f(w, base, some ? it + 1 : it, std::true_type{});
   }
 }
 template <int NT>
@@ -1216,14 +1270,17 @@ __device__ __forceinline__ Acc acc_block(Acc a, const Side& z, Acc* red) {
 
 // ---- top classes of a stretch of a row ---------------------------------------------------------------------
 // The k-th largest of the threads' own maxima so far is a bound that at least k classes reach, and few others
-// do.  It is raised after steps 1, 2, 4, 8, ... of the walk, and what reaches it is put down in LDS from the
-// registers: about k classes for each doubling, no second look at the row.  At the end the last bound
-// thins the candidates out and the rest is ranked by counting.
+// do.  It is raised after steps 1, 8, 64, ... of the walk (1, 4, 16, ... for long lists), and what reaches it
+// is put down in LDS from the registers: about k classes in each step that is as long as the ones before the
+// last raise together, no second look at the row.  At the
+// end they are ranked by counting; where there are many, a last bound thins them out first.
 // More candidates than LDS holds (rows that are constant, or masked but for a few classes), and rows
 // with NaN, take row_top_again(), which goes back to the row: the classes above the bound, then the ones
 // at it from the first on; and k rounds of "largest below the last" where that does not fit either.
 constexpr int kCand = 1024;
-constexpr int kBoundBits = 20;  // of a maximum's 32 order bits: a bound a little too low only lets a few more in
+constexpr int kFewCandidates = 128;
+// of a maximum's 32 order bits: a bound a little too low only lets a few more in
+constexpr int kRoughBits = 12, kFineBits = 20;
 struct TopShared {
   unsigned long long cand[kCand];
   float maxima[256];
@@ -1236,7 +1293,7 @@ __device__ __forceinline__ unsigned order_bits(float v) {
   return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 // (just below) the k-th largest of the block's maxima, the same in every thread; two barriers
-template <int NT>
+template <int NT, int BITS>
 __device__ __forceinline__ float raise_bound(float my_max, int k, TopShared& sh) {
   unsigned o[NT / 64];
   if (NT == 64) {
@@ -1250,7 +1307,7 @@ __device__ __forceinline__ float raise_bound(float my_max, int k, TopShared& sh)
   }
   unsigned t = 0;
 #pragma unroll
-  for (int bit = 31; bit > 31 - kBoundBits; --bit) {
+  for (int bit = 31; bit > 31 - BITS; --bit) {
     const unsigned c = t | 1u << bit;
     int n = 0;
 #pragma unroll
@@ -1264,21 +1321,38 @@ template <class T>
 __device__ __forceinline__ void put_down(const float (&v)[32], float sign, int base, int end, int lane, float bound,
                                          TopShared& sh) {
 #pragma unroll
-  for (int u = 0; u < 32; ++u) {
-    const int j = base + tile_class<T>(lane, u);
-    if (v[u] * sign >= bound && j < end) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kCand) sh.cand[at] = key_u64(v[u] * sign, j);
+  for (int g = 0; g < 32; g += 8) {  // eight values at a time: in most of them there is nothing
+    float m = vmax(v[g] * sign, v[g + 1] * sign);
+#pragma unroll
+    for (int e = 2; e < 8; e += 2) m = vmax3(m, v[g + e] * sign, v[g + e + 1] * sign);
+    if (m >= bound) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = base + tile_class<T>(lane, g + e);
+        if (v[g + e] * sign >= bound && j < end) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCand) sh.cand[at] = key_u64(v[g + e] * sign, j);
+        }
+      }
     }
   }
+}
+// how many of the n keys are larger; eight are read at a time
+__device__ __forceinline__ int rank_of(unsigned long long mine, const unsigned long long* keys, int n) {
+  int rank = 0, j = 0;
+  for (; j + 8 <= n; j += 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rank += keys[j + i] > mine ? 1 : 0;
+  }
+  for (; j < n; ++j) rank += keys[j] > mine ? 1 : 0;
+  return rank;
 }
 // ranks the candidates; out: the `want` largest, descending
 template <int NT>
 __device__ __forceinline__ void rank_candidates(int n, int want, unsigned long long* out, const TopShared& sh) {
   for (int i = threadIdx.x; i < n; i += NT) {
     const unsigned long long mine = sh.cand[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.cand[j] > mine ? 1 : 0;
+    const int rank = rank_of(mine, sh.cand, n);
     if (rank < want) out[rank] = mine;
   }
 }
@@ -1289,7 +1363,7 @@ __device__ __noinline__ void row_top_again(const typename T::S* row, int begin, 
   const int want = min(k, end - begin);
   __syncthreads();
   if (tid == 0) sh.count = 0;
-  const float bound = raise_bound<NT>(my_max, k, sh);
+  const float bound = raise_bound<NT, kFineBits>(my_max, k, sh);
   __syncthreads();
   bool slow = bad;
   int n = 0;
@@ -1298,7 +1372,9 @@ __device__ __noinline__ void row_top_again(const typename T::S* row, int begin, 
     if (my_max > bound) {
       for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) {
         float v[32];
-        row_in<T>(row, base, end, lane, -kInf, v);
+        RowFeed<T> feed;
+        feed.issue_some(row, base, end, lane);
+        feed.take_some(base, end, lane, -kInf, v);
 #pragma unroll
         for (int u = 0; u < 32; ++u) {
           const int j = base + tile_class<T>(lane, u);
@@ -1363,16 +1439,11 @@ struct LpOut {
   Stats3* stats;
 };
 template <class T>
-__device__ __forceinline__ void lp_row_write(const Prob& p, int64_t row, const typename T::S* xr, const void* index,
-                                             const Acc& a, const LpOut& o) {
+__device__ __forceinline__ void lp_row_write(const Prob& p, int64_t row, int given, typename T::S x_given, const Acc& a,
+                                             const LpOut& o) {
   const Side z = side(p);
   const float base = a.m == z.far() ? 0.f : a.m, ln_s = logf(a.s);
-  const int t = index ? valid_index(load_index(index, row, p.flags), p.V) : -1;
-  float lp = 0.f;
-  if (t >= 0) {
-    const float v = T::up(xr[t]);
-    lp = log_p(v, base, ln_s, p.scale);
-  }
+  const float lp = given >= 0 ? log_p(T::up(x_given), base, ln_s, p.scale) : 0.f;
   if (o.log_prob) o.log_prob[row] = lp;
   if (o.entropy) o.entropy[row] = entropy_of(a.s, a.w, ln_s);
   if (o.stats) o.stats[row] = Stats3{base, a.s, a.w};
@@ -1409,20 +1480,24 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
     if (threadIdx.x == 0) shared_top.count = 0;
     __syncthreads();
   }
+  // the given class, on its way while the row is read
+  const int given = index && p.chunks == 1 ? valid_index(load_index(index, row, p.flags), p.V) : -1;
+  const typename T::S x_given = given >= 0 ? xr[given] : typename T::S(0);
   Acc a = acc_empty(z);
   float bound = -kInf;
+  const int steps = p.k > 32 ? 0x55555555 : 0x49249249;  // powers of 4 or of 8
   walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](const float (&v)[32], int base, int it, auto) {
     const float top = z.best_of(v);
-    absorb<true>(a, v, top, z);
+    absorb<true>(a, v, 32, top, z);
     if constexpr (TOP) {
-      if (((it + 1) & it) == 0) bound = raise_bound<NT>(a.m * z.sign, p.k, shared_top);
+      if (((it + 1) & it) == 0 && ((it + 1) & steps)) bound = raise_bound<NT, kRoughBits>(a.m * z.sign, p.k, shared_top);
       if (top * z.sign >= bound) put_down<T>(v, z.sign, base, end, lane, bound, shared_top);
     }
   });
   const float my_max = a.m * z.sign;
   a = acc_block<NT>(a, z, red);
   if (p.chunks == 1) {
-    if (threadIdx.x == 0) lp_row_write<T>(p, row, xr, index, a, o);
+    if (threadIdx.x == 0) lp_row_write<T>(p, row, given, x_given, a, o);
   } else if (threadIdx.x == 0) {
     parts[row * p.chunks + chunk] = Part{a.m, a.s, a.w, 0.f};
   }
@@ -1430,11 +1505,12 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
     TopShared& sh = shared_top;
     __shared__ unsigned long long best[kMaxEntries];
     const int want = min(p.k, end - begin);
-    bound = raise_bound<NT>(my_max, p.k, sh);
     __syncthreads();
-    int n = sh.count;
+    const int n = sh.count;
     if (n > kCand || a.s != a.s) {
       row_top_again<T, NT>(xr, begin, end, p.k, z.sign, my_max, a.s != a.s, best, sh);
+    } else if (n <= kFewCandidates) {
+      rank_candidates<NT>(n, want, best, sh);
     } else {
       unsigned long long mine[kCand / NT];
 #pragma unroll
@@ -1442,6 +1518,7 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
         const int at = threadIdx.x + i * NT;
         mine[i] = at < n ? sh.cand[at] : 0;
       }
+      bound = raise_bound<NT, kFineBits>(my_max, p.k, sh);
       __syncthreads();
       if (threadIdx.x == 0) sh.count = 0;
       __syncthreads();
@@ -1472,19 +1549,21 @@ __global__ __launch_bounds__(256) void lp_row_join(Prob p, const typename T::S* 
   __shared__ unsigned long long keys[kCand];
   const int64_t row = blockIdx.x;
   const Side z = side(p);
+  const int given = index ? valid_index(load_index(index, row, p.flags), p.V) : -1;
+  const typename T::S x_given = given >= 0 ? x[row * p.V + given] : typename T::S(0);
+  const int n = p.chunks * p.k;  // at most kCand
+  for (int i = threadIdx.x; i < n; i += 256) keys[i] = part_keys[row * n + i];
   Acc a = acc_empty(z);
-  for (int i = 0; i < p.chunks; ++i) {
+  for (int i = threadIdx.x & 63; i < p.chunks; i += 64) {
     const Part q = parts[row * p.chunks + i];
     a = acc_join(a, Acc{q.m, q.s, q.w}, z);
   }
-  if (threadIdx.x == 0) lp_row_write<T>(p, row, x + row * p.V, index, a, o);
-  const int n = p.chunks * p.k;  // at most kCand
-  for (int i = threadIdx.x; i < n; i += 256) keys[i] = part_keys[row * n + i];
+  a = acc_wave(a, z);
+  if (threadIdx.x == 0) lp_row_write<T>(p, row, given, x_given, a, o);
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += 256) {
     const unsigned long long mine = keys[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += keys[j] > mine ? 1 : 0;
+    const int rank = rank_of(mine, keys, n);
     if (mine != 0 && rank < p.k) lp_row_top_write(p, row, rank, mine, a, o);
   }
 }
@@ -1541,7 +1620,7 @@ __device__ __forceinline__ Entry load_entry(const Prob& p, int64_t row, const vo
       float tm = e.value;
 #pragma unroll
       for (int k = 1; k < 64; k <<= 1) tm = fmaxf(tm, shfl_xor(tm, k));
-      const float ts = wave_sum_all(expf(e.value - (tm == -kInf ? 0.f : tm)));
+      const float ts = wave_sum_all(exp_(e.value - (tm == -kInf ? 0.f : tm)));
       if (ts != 0.f) e.value -= tm + logf(ts);
     }
   }
@@ -1572,10 +1651,10 @@ __device__ __forceinline__ void patch_tile(float (&v)[32], int base, int lane, i
 }
 // loss and statistics of a row from the sums over its unlisted classes; one wave
 template <class T>
-__device__ __forceinline__ void ds_row_write(const Prob& p, int64_t row, const typename T::S* xr, const Entry& e,
+__device__ __forceinline__ void ds_row_write(const Prob& p, int64_t row, const Entry& e, typename T::S x_listed,
                                              const Acc& a, float* loss, float4* stats) {
   const Side z = side(p);
-  const float v = e.idx >= 0 ? T::up(xr[e.idx]) : z.far();
+  const float v = e.idx >= 0 ? T::up(x_listed) : z.far();
   const float first = e.again ? z.far() : v;
   RowSums r;
   r.m_r = a.m;
@@ -1585,7 +1664,7 @@ __device__ __forceinline__ void ds_row_write(const Prob& p, int64_t row, const t
   r.s = fmaf(a.s, exp2_((a.m - r.b) * p.c), wave_sum_all(exp2_((first - r.b) * p.c)));
   r.ln_s = logf(r.s);
   const bool alive = __any(e.idx >= 0);
-  const float qe = e.idx >= 0 ? expf(e.value) : 0.f;
+  const float qe = e.idx >= 0 ? exp_(e.value) : 0.f;
   const float mass = wave_sum_all(qe);
   float l = wave_sum_all(qe != 0.f ? qe * (e.value - log_p(v, r.b, r.ln_s, p.scale)) : 0.f);
   const float rr = (alive && !(p.flags & kRenorm) && r.s_r != 0.f) ? fmaxf(1.f - mass, 0.f) : 0.f;
@@ -1609,19 +1688,20 @@ __global__ __launch_bounds__(NT, 4) void ds_row_fwd(Prob p, const typename T::S*
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
   const Side z = side(p);
   const Entry e = load_entry(p, row, p.chunks == 1 ? teacher : nullptr, index, lane);
+  const typename T::S x_listed = p.chunks == 1 && e.idx >= 0 ? xr[e.idx] : typename T::S(0);
   Acc a = acc_empty(z);
   if (__any(e.idx >= 0)) {  // the same in every wave
     walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, auto full) {
       (void)full;
       patch_tile<T>(v, base, lane, e.idx, z.far());
-      absorb<false>(a, v, z.best_of(v), z);
+      absorb<false>(a, v, 32, z.best_of(v), z);
     });
   }
   a = acc_block<NT>(a, z, red);
   if (p.chunks > 1) {
     if (threadIdx.x == 0) parts[row * p.chunks + chunk] = Part{a.m, a.s, 0.f, 0.f};
   } else if (wave == 0) {
-    ds_row_write<T>(p, row, xr, e, a, loss, stats);
+    ds_row_write<T>(p, row, e, x_listed, a, loss, stats);
   }
 }
 template <class T>
@@ -1632,13 +1712,14 @@ __global__ __launch_bounds__(64) void ds_row_join(Prob p, const typename T::S* _
   const int64_t row = blockIdx.x;
   const Side z = side(p);
   const Entry e = load_entry(p, row, teacher, index, threadIdx.x);
+  const typename T::S x_listed = e.idx >= 0 ? x[row * p.V + e.idx] : typename T::S(0);
   Acc a = acc_empty(z);
   for (int i = threadIdx.x; i < p.chunks; i += 64) {
     const Part q = parts[row * p.chunks + i];
     a = acc_join(a, Acc{q.m, q.s, 0.f}, z);
   }
   a = acc_wave(a, z);
-  ds_row_write<T>(p, row, x + row * p.V, e, a, loss, stats);
+  ds_row_write<T>(p, row, e, x_listed, a, loss, stats);
 }
 
 template <class T, int NT>
@@ -1665,7 +1746,7 @@ __global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S*
   Entry e = load_entry(p, row, teacher, index, lane);
   float with = 0.f;
   {
-    float qe = e.idx >= 0 ? expf(e.value) : 0.f;
+    float qe = e.idx >= 0 ? exp_(e.value) : 0.f;
     float sum = qe;  // of all entries of this class
     for (int k = 0; k < p.k; ++k) {
       const int other = __builtin_amdgcn_readlane(e.idx, k);
@@ -1743,9 +1824,22 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
     const int stages = (p.V + stage - 1) / stage;
     P.nw = 1;
     while (P.nw < 16 && tiles * P.nw < kWantWaves && P.nw * 2 <= stages) P.nw *= 2;
-    const size_t per_wave = kStageBytes + (distill ? 512 : 64 * (12 + 8 * 16));
-    const size_t shared = distill ? distill_lds(0, p.k, true) : 0;
-    while (P.nw > 1 && P.nw * per_wave + shared > kLdsBudget) P.nw /= 2;
+    if (distill) {
+      // The list is the block's, a stage each wave's, so more waves a block are more waves in the LDS of a compute
+      // unit.  The forward pass ends with one wave's work: it takes that only where fewer than 8 waves would fit
+      // (channels_last f16, 128 classes, 8 entries: 35 us with one wave a block, 39 with two; bf16 planes, 256
+      // classes, 64 entries: 210 and 116 with one and 8).  The backward pass does not (bf16 planes, 256 classes,
+      // 8 entries: 118 us with one, 105 with two).
+      const auto waves = [&](int nw) {
+        const size_t lds = nw * (size_t)distill_stage_bytes(P.last, esize) + distill_lds(nw, p.k, false);
+        return lds > kLdsBudget ? 0 : (int)(kLdsBudget / lds) * nw;
+      };
+      for (int nw = P.nw * 2; nw <= 16 && nw <= stages; nw *= 2)
+        if (waves(nw) > waves(P.nw) && waves(P.nw) < (backward ? 16 : 8)) P.nw = nw;
+      while (P.nw > 1 && waves(P.nw) == 0) P.nw /= 2;
+    } else {
+      while (P.nw > 1 && P.nw * (kStageBytes + 64 * (12 + 8 * 16)) > (int)kLdsBudget) P.nw /= 2;
+    }
     p.cpw = (stages + P.nw - 1) / P.nw * stage;
     if (tiles > 0x7fffffff) return DW_ERR_SHAPE;
     P.grid = (unsigned)tiles;
@@ -1844,7 +1938,7 @@ template <class T, bool LAST>
 int ds_tile_launch(const Plan& P, bool backward, const void* x, const void* teacher, const void* index, float* loss,
                    float4* stats, const float* g_loss, void* g, hipStream_t st) {
   using S = typename T::S;
-  const size_t lds = P.nw * (size_t)distill_stage_bytes<LAST>() + distill_lds(P.nw, P.p.k, backward);
+  const size_t lds = P.nw * (size_t)distill_stage_bytes(LAST, sizeof(S)) + distill_lds(P.nw, P.p.k, backward);
   if (backward) {
     if (int rc = allow_lds(ds_tile_bwd<T, LAST>, lds)) return rc;
     ds_tile_bwd<T, LAST><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, stats, g_loss, (S*)g);
