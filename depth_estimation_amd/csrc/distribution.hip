@@ -1192,10 +1192,11 @@ __device__ __forceinline__ void row_zero(typename T::S* row, int begin, int end,
   for (int u = 0; u < 32; ++u) v[u] = 0.f;
   for (int base = begin + wave * kWaveTile; base < end; base += NT * 32) row_out<T>(row, base, end, lane, v);
 }
-template <class T, class FULL>
+template <class T>
 __device__ __forceinline__ void row_put(typename T::S* row, int base, int end, int lane, const float (&v)[32], bool past,
-                                             FULL) {
-  if (!FULL::value) {
+                                        bool full) {
+  if (!full) {
+    rare();
     row_out<T>(row, base, end, lane, v);
     return;
   }
@@ -1237,42 +1238,40 @@ struct RowFeed {
       else if (n > 0) w[u] = load_some<T>(row, j * (unsigned)sizeof(typename T::S), n);
     }
   }
-  __device__ __forceinline__ void take_some(int base, int end, int lane, float far, float (&v)[32]) const {
-#pragma unroll
-    for (int u = 0; u < 32 / T::VEC; ++u) {
-      const int n = end - (base + lane * T::VEC + u * 64 * T::VEC);
-#pragma unroll
-      for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = e < n ? w[u].get(e) : far;
-    }
-  }
 };
-// f(v, base, it, full) for every block-wide step `it` of [begin, end) (v is all `far` for a wave that has nothing
-// in a step).  The step that is not full for every wave comes second: its loads are on their way early.
+template <class T>
+__device__ __forceinline__ void mask_tail(float (&v)[32], int base, int end, int lane, float far) {
+  const int n = end - (int)fresh((unsigned)(base + lane * T::VEC));
+#pragma unroll
+  for (int u = 0; u < 32; ++u) v[u] = tile_class<T>(0, u) < n ? v[u] : far;
+}
+// f(v, base, it, full) for every block-wide step `it` of [begin, end); v is all `far` for a wave that has nothing in
+// the last one.  The body is there once: three copies of it (first step, last step, loop) spilled, and waiting
+// for a spilled value waits for the loads that are on their way.
 template <class T, int NT, class F>
 __device__ __forceinline__ void walk_row(const typename T::S* row, int begin, int end, int lane, int wave, float far, F f) {
-  const int full = (end - begin) / (NT * 32);
+  const int steps = (end - begin + NT * 32 - 1) / (NT * 32), full = (end - begin) / (NT * 32);
   int base = begin + wave * kWaveTile;
-  const int rest = base + full * NT * 32;
-  const bool some = begin + full * NT * 32 < end;
-  RowFeed<T> feed, part;
+  RowFeed<T> feed;
   if (full > 0) feed.issue(row, base, lane);
-  if (some) part.issue_some(row, rest, end, lane);
-  float v[32];
-  if (full > 0) {
+  else feed.issue_some(row, base, end, lane);
+#pragma clang loop unroll(disable)
+  for (int it = 0; it < steps; ++it) {
+    float v[32];
     feed.take(v);
-    if (full > 1) feed.issue(row, base + NT * 32, lane);
-    f(v, base, 0, std::true_type{});
-  }
-  if (some) {
-    part.take_some(rest, end, lane, far, v);
-    f(v, rest, full > 0 ? 1 : 0, std::false_type{});
-  }
-  for (int it = 1; it < full; ++it) {
-    base += NT * 32;
-    float w[32];
-    feed.take(w);
-    if (it + 1 < full) feed.issue(row, base + NT * 32, lane);
-    f(w, base, some ? it + 1 : it, std::true_type{});
+    if (it >= full) {
+      rare();
+      mask_tail<T>(v, base, end, lane, far);
+    }
+    const int next = base + NT * 32;
+    if (it + 1 < full) {
+      feed.issue(row, next, lane);
+    } else if (it + 1 < steps) {
+      rare();
+      feed.issue_some(row, next, end, lane);
+    }
+    f(v, base, it, it < full);
+    base = next;
   }
 }
 template <int NT>
@@ -1288,23 +1287,25 @@ __device__ __forceinline__ Acc acc_block(Acc a, const Side& z, Acc* red) {
 }
 
 // ---- top classes of a stretch of a row ---------------------------------------------------------------------
-// The k-th largest of the threads' own maxima so far is a bound that at least k classes reach, and few others
-// do.  It is raised after steps 1, 8, 64, ... of the walk (1, 4, 16, ... for long lists), and what reaches it
-// is put down in LDS from the registers: about k classes in each step that is as long as the ones before the
-// last raise together, no second look at the row.  At the
-// end they are ranked by counting; where there are many, a last bound thins them out first.
-// More candidates than LDS holds (rows that are constant, or masked but for a few classes), and rows
-// with NaN, take row_top_again(), which goes back to the row: the classes above the bound, then the ones
-// at it from the first on; and k rounds of "largest below the last" where that does not fit either.
-constexpr int kCand = 1024;
-constexpr int kFewCandidates = 128;
-// of a maximum's 32 order bits: a bound a little too low only lets a few more in
-constexpr int kRoughBits = 12, kFineBits = 20;
+// While the row is read, each thread only puts down the best of its 32 classes of every step (a cell; of
+// several steps where there are more than 16), in LDS.
+// The k-th largest of the threads' own maxima is then a bound that at least k classes reach, and few
+// others do: the cells that reach it, hardly more than k of them, are read again, 32 lanes a cell, and the
+// classes that reach it are ranked by counting.  (Collecting them from the registers in the loop, with a
+// bound raised on the way, cost more than it saved: 45 us against 31 without a list, 1023 x 50001 f16.)
+// Rows with more such cells or classes than LDS holds (constant ones, or masked but for a few classes), and
+// rows with NaN, take row_top_again(): the classes above the bound, then the ones at it from the first
+// on; and k rounds of "largest below the last" where that does not fit either.
+constexpr int kCand = 1024, kCells = 512;
+constexpr int kCellRows = 16;   // at most so many cells a thread
+__host__ __device__ constexpr int cell_span(int steps) { return (steps + kCellRows - 1) / kCellRows; }  // steps a cell
+constexpr int kBoundBits = 20;  // of a maximum's 32 order bits: a bound a little too low only lets a few more in
 struct TopShared {
   unsigned long long cand[kCand];
   float maxima[256];
   unsigned long long best[4];
-  int count, total[4];
+  unsigned cells[kCells];
+  int count, cell_count, total[4];
   float bound;
 };
 __device__ __forceinline__ unsigned order_bits(float v) {
@@ -1312,7 +1313,7 @@ __device__ __forceinline__ unsigned order_bits(float v) {
   return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 // (just below) the k-th largest of the block's maxima, the same in every thread; two barriers
-template <int NT, int BITS>
+template <int NT>
 __device__ __forceinline__ float raise_bound(float my_max, int k, TopShared& sh) {
   unsigned o[NT / 64];
   if (NT == 64) {
@@ -1325,8 +1326,8 @@ __device__ __forceinline__ float raise_bound(float my_max, int k, TopShared& sh)
     for (int w = 0; w < NT / 64; ++w) o[w] = order_bits(sh.maxima[w * 64 + (threadIdx.x & 63)]);
   }
   unsigned t = 0;
-#pragma unroll
-  for (int bit = 31; bit > 31 - BITS; --bit) {
+#pragma unroll 4
+  for (int bit = 31; bit > 31 - kBoundBits; --bit) {
     const unsigned c = t | 1u << bit;
     int n = 0;
 #pragma unroll
@@ -1335,26 +1336,6 @@ __device__ __forceinline__ float raise_bound(float my_max, int k, TopShared& sh)
   }
   if (t <= 0x007fffffu) return -kInf;  // at or below the order bits of -inf
   return __builtin_bit_cast(float, (t >> 31) ? (t ^ 0x80000000u) : ~t);
-}
-template <class T>
-__device__ __forceinline__ void put_down(const float (&v)[32], float sign, int base, int end, int lane, float bound,
-                                         TopShared& sh) {
-#pragma unroll
-  for (int g = 0; g < 32; g += 8) {  // eight values at a time: in most of them there is nothing
-    float m = vmax(v[g] * sign, v[g + 1] * sign);
-#pragma unroll
-    for (int e = 2; e < 8; e += 2) m = vmax3(m, v[g + e] * sign, v[g + e + 1] * sign);
-    if (m >= bound) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = base + tile_class<T>(lane, g + e);
-        if (v[g + e] * sign >= bound && j < end) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCand) sh.cand[at] = key_u64(v[g + e] * sign, j);
-        }
-      }
-    }
-  }
 }
 // how many of the n keys are larger; eight are read at a time
 __device__ __forceinline__ int rank_of(unsigned long long mine, const unsigned long long* keys, int n) {
@@ -1376,13 +1357,13 @@ __device__ __forceinline__ void rank_candidates(int n, int want, unsigned long l
   }
 }
 template <class T, int NT>
-__device__ __noinline__ void row_top_again(const typename T::S* row, int begin, int end, int k, float sign, float my_max,
+__device__ __forceinline__ void row_top_again(const typename T::S* row, int begin, int end, int k, float sign, float my_max,
                                            bool bad, unsigned long long* out, TopShared& sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int want = min(k, end - begin);
   __syncthreads();
   if (tid == 0) sh.count = 0;
-  const float bound = raise_bound<NT, kFineBits>(my_max, k, sh);
+  const float bound = raise_bound<NT>(my_max, k, sh);
   __syncthreads();
   bool slow = bad;
   int n = 0;
@@ -1393,7 +1374,7 @@ __device__ __noinline__ void row_top_again(const typename T::S* row, int begin, 
         float v[32];
         RowFeed<T> feed;
         feed.issue_some(row, base, end, lane);
-        feed.take_some(base, end, lane, -kInf, v);
+        feed.take(v);
 #pragma unroll
         for (int u = 0; u < 32; ++u) {
           const int j = base + tile_class<T>(lane, u);
@@ -1494,24 +1475,26 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
   const typename T::S* xr = x + row * p.V;
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
   const Side z = side(p);
-  __shared__ std::conditional_t<TOP, TopShared, char> shared_top;
-  if constexpr (TOP) {
-    if (threadIdx.x == 0) shared_top.count = 0;
-    __syncthreads();
-  }
+  extern __shared__ float cell_best[];  // [cell][thread]
+  const int steps = (end - begin + NT * 32 - 1) / (NT * 32), span = cell_span(steps);
+  float so_far = -kInf;
+  int cell = 0, in_cell = 0;
   // the given class, on its way while the row is read
   const int given = index && p.chunks == 1 ? valid_index(load_index(index, row, p.flags), p.V) : -1;
   const typename T::S x_given = given >= 0 ? xr[given] : typename T::S(0);
   Acc a = acc_empty(z);
-  float bound = -kInf;
-  const int steps = p.k > 32 ? 0x55555555 : 0x49249249;  // powers of 4 or of 8
-  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](const float (&v)[32], int base, int it, auto) {
+  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](const float (&v)[32], int, int, bool) {
     const float top = z.best_of(v);
-    absorb<true>(a, v, 32, top, z);
     if constexpr (TOP) {
-      if (((it + 1) & it) == 0 && ((it + 1) & steps)) bound = raise_bound<NT, kRoughBits>(a.m * z.sign, p.k, shared_top);
-      if (top * z.sign >= bound) put_down<T>(v, z.sign, base, end, lane, bound, shared_top);
+      so_far = vmax(so_far, top * z.sign);
+      cell_best[cell * NT + threadIdx.x] = so_far;
+      if (++in_cell == span) {
+        in_cell = 0;
+        ++cell;
+        so_far = -kInf;
+      }
     }
+    absorb<true>(a, v, 32, top, z);
   });
   const float my_max = a.m * z.sign;
   a = acc_block<NT>(a, z, red);
@@ -1521,33 +1504,40 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
     parts[row * p.chunks + chunk] = Part{a.m, a.s, a.w, 0.f};
   }
   if constexpr (TOP) {
-    TopShared& sh = shared_top;
+    __shared__ TopShared sh;
     __shared__ unsigned long long best[kMaxEntries];
-    const int want = min(p.k, end - begin);
+    const int want = min(p.k, end - begin), rows = (steps + span - 1) / span;
+    if (threadIdx.x == 0) sh.count = sh.cell_count = 0;
+    const float bound = raise_bound<NT>(my_max, p.k, sh);
     __syncthreads();
-    const int n = sh.count;
-    if (n > kCand || a.s != a.s) {
-      row_top_again<T, NT>(xr, begin, end, p.k, z.sign, my_max, a.s != a.s, best, sh);
-    } else if (n <= kFewCandidates) {
-      rank_candidates<NT>(n, want, best, sh);
-    } else {
-      unsigned long long mine[kCand / NT];
-#pragma unroll
-      for (int i = 0; i < kCand / NT; ++i) {
-        const int at = threadIdx.x + i * NT;
-        mine[i] = at < n ? sh.cand[at] : 0;
+    for (int r = 0; r < rows; ++r) {
+      if (cell_best[r * NT + threadIdx.x] >= bound) {
+        const int at = atomicAdd(&sh.cell_count, 1);
+        if (at < kCells) sh.cells[at] = r * NT + threadIdx.x;
       }
-      bound = raise_bound<NT, kFineBits>(my_max, p.k, sh);
-      __syncthreads();
-      if (threadIdx.x == 0) sh.count = 0;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kCand / NT; ++i) {
-        if (mine[i] != 0 && key_value(mine[i]) >= bound) sh.cand[atomicAdd(&sh.count, 1)] = mine[i];
-      }
-      __syncthreads();
-      rank_candidates<NT>(sh.count, want, best, sh);
     }
+    __syncthreads();
+    const int cells = sh.cell_count;
+    bool again = cells > kCells || a.s != a.s;
+    if (!again) {
+      for (int c = threadIdx.x / 32; c < cells * span; c += NT / 32) {
+        const int which = sh.cells[c / span], t = which % NT, it = which / NT * span + c % span;
+        const int j = begin + it * NT * 32 + t / 64 * kWaveTile + tile_class<T>(t % 64, threadIdx.x % 32);
+        if (it < steps && j < end) {
+          const float v = T::up(xr[j]) * z.sign;
+          if (v >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kCand) sh.cand[at] = key_u64(v, j);
+          }
+        }
+      }
+      __syncthreads();
+      again = sh.count > kCand;
+    }
+    if (again)
+      row_top_again<T, NT>(xr, begin, end, p.k, z.sign, my_max, a.s != a.s, best, sh);
+    else
+      rank_candidates<NT>(sh.count, want, best, sh);
     __syncthreads();
     if ((int)threadIdx.x < p.k) {
       const unsigned long long key = (int)threadIdx.x < want ? best[threadIdx.x] : 0;
@@ -1605,7 +1595,7 @@ __global__ __launch_bounds__(NT, 4) void lp_row_bwd(Prob p, const typename T::S*
     row_zero<T, NT>(gr, begin, end, lane, wave);
     return;
   }
-  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, auto full) {
+  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, bool full) {
 #pragma unroll
     for (int u = 0; u < 32; ++u) {
       v[u] = lp_grad<ENT>(r, v[u], p.c, 0.f);
@@ -1709,7 +1699,7 @@ __global__ __launch_bounds__(NT, 4) void ds_row_fwd(Prob p, const typename T::S*
   const typename T::S x_listed = p.chunks == 1 && e.idx >= 0 ? xr[e.idx] : typename T::S(0);
   Acc a = acc_empty(z);
   if (__any(e.idx >= 0)) {  // the same in every wave
-    walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, auto full) {
+    walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, bool full) {
       (void)full;
       patch_tile<T>(v, base, lane, e.idx, z.far());
       absorb<false>(a, v, 32, z.best_of(v), z);
@@ -1777,7 +1767,7 @@ __global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S*
     }
     if (e.again) e.idx = -1;
   }
-  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, auto full) {
+  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, bool full) {
 #pragma unroll
     for (int u = 0; u < 32; ++u) {
       v[u] = exp2_((v[u] - st.x) * p.c) * rest_f;
@@ -1935,11 +1925,13 @@ int lp_fwd(const Plan& P, const void* x, const void* index, const LpOut& o, void
   Part* parts = (Part*)ws;
   unsigned long long* keys = (unsigned long long*)((char*)ws + parts_bytes(P.p.rows, P.p.chunks));
   const typename T::S* xs = (const typename T::S*)x;
+  const int steps = (P.p.chunk + P.nt * 32 - 1) / (P.nt * 32), span = cell_span(steps);
+  const size_t cells = k ? (size_t)(steps + span - 1) / span * P.nt * sizeof(float) : 0;
   if (P.nt == 64) {
-    if (k) lp_row_fwd<T, 64, true><<<P.grid, 64, 0, st>>>(P.p, xs, index, o, parts, keys);
+    if (k) lp_row_fwd<T, 64, true><<<P.grid, 64, cells, st>>>(P.p, xs, index, o, parts, keys);
     else lp_row_fwd<T, 64, false><<<P.grid, 64, 0, st>>>(P.p, xs, index, o, parts, keys);
   } else {
-    if (k) lp_row_fwd<T, 256, true><<<P.grid, 256, 0, st>>>(P.p, xs, index, o, parts, keys);
+    if (k) lp_row_fwd<T, 256, true><<<P.grid, 256, cells, st>>>(P.p, xs, index, o, parts, keys);
     else lp_row_fwd<T, 256, false><<<P.grid, 256, 0, st>>>(P.p, xs, index, o, parts, keys);
   }
   if (P.p.chunks > 1) lp_row_join<T><<<(unsigned)P.p.rows, 256, 0, st>>>(P.p, xs, index, o, parts, keys);
