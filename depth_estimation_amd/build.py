@@ -1,4 +1,5 @@
-"""Builds libdepthwarp.so (the HIP kernels + C ABI) in-tree with hipcc.
+"""Builds libdepthwarp.so (the HIP kernels + C ABI) in-tree with hipcc, and libdepthwarp_torch.so (the autograd
+nodes that are written in C++; host code only) with the host compiler.
 
     python -m depth_estimation_amd.build [--force]
 
@@ -18,6 +19,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libdepthwarp.so"
+TORCH_LIB = PKG / "libdepthwarp_torch.so"   # autograd nodes in C++ (host code): csrc/distribution_autograd.cpp
+TORCH_SOURCE = CSRC / "distribution_autograd.cpp"
 SOURCES = ["photometric.hip", "compute_loss.hip", "modules.hip", "soft_argmin.hip", "cost_volume.hip", "lidar.hip",
            "distribution.hip", "abi.hip"]
 # per-source options: the tile kernel runs 1 % faster with the scheduler's max-ILP strategy
@@ -33,11 +36,22 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
+def _torch_command() -> list:
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-I{ROOT / 'include'}", "-isystem", str(root / "include"),
+            "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+            "-isystem", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), str(TORCH_SOURCE),
+            "-o", str(TORCH_LIB), f"-L{root / 'lib'}", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip"]
+
+
 def stale() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not TORCH_LIB.exists():
         return True
-    t = LIB.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES if (CSRC / s).exists()] + HEADERS
+    t = min(LIB.stat().st_mtime, TORCH_LIB.stat().st_mtime)
+    deps = [CSRC / s for s in SOURCES if (CSRC / s).exists()] + [TORCH_SOURCE] + HEADERS
     return any(d.stat().st_mtime > t for d in deps)
 
 
@@ -60,6 +74,10 @@ def build(force: bool = False, verbose: bool = True) -> Path:
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((cmd, obj, subprocess.Popen(cmd)))
+    torch_cmd = _torch_command()
+    if verbose:
+        print(" ".join(torch_cmd), flush=True)
+    torch_proc = subprocess.Popen(torch_cmd)
     objs = []
     for cmd, obj, proc in procs:
         if proc.wait() != 0:
@@ -69,6 +87,8 @@ def build(force: bool = False, verbose: bool = True) -> Path:
     if verbose:
         print(" ".join(link), flush=True)
     subprocess.run(link, check=True)
+    if torch_proc.wait() != 0:
+        raise subprocess.CalledProcessError(torch_proc.returncode, torch_cmd)
     return LIB
 
 

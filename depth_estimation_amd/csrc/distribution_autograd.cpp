@@ -1,0 +1,200 @@
+// Eager calls of the distribution operators as torch autograd nodes (host code only).
+//
+// The kernels are reached through the C ABI (depthwarp.h) like everywhere else; this file holds what an eager call
+// does around them -- outputs, workspace, stream, and the node of the backward pass.  It is C++ because small
+// training steps are bound by it: a node written in Python runs in the autograd engine's own thread, where the
+// interpreter's lock and cold caches took about half of such a step (80 to 90 us, 4 x 64 x 4 x 4).
+//
+// The library's functions and descriptors come from Python as addresses: which build of the library is in use, and
+// what the shapes and types decide, is settled there (distribution.py).
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include <cstring>
+#include <optional>
+#include <string>
+#include <vector>
+
+#include "depthwarp.h"
+
+namespace {
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Library {
+  decltype(&dw_strerror) strerror;
+  decltype(&dw_log_probs_fwd) log_probs_fwd;
+  decltype(&dw_log_probs_bwd) log_probs_bwd;
+  decltype(&dw_distill_fwd) distill_fwd;
+  decltype(&dw_distill_bwd) distill_bwd;
+} lib{};
+
+void bind(int64_t strerror, int64_t lp_fwd, int64_t lp_bwd, int64_t ds_fwd, int64_t ds_bwd) {
+  lib.strerror = reinterpret_cast<decltype(lib.strerror)>(strerror);
+  lib.log_probs_fwd = reinterpret_cast<decltype(lib.log_probs_fwd)>(lp_fwd);
+  lib.log_probs_bwd = reinterpret_cast<decltype(lib.log_probs_bwd)>(lp_bwd);
+  lib.distill_fwd = reinterpret_cast<decltype(lib.distill_fwd)>(ds_fwd);
+  lib.distill_bwd = reinterpret_cast<decltype(lib.distill_bwd)>(ds_bwd);
+}
+void check(int code, const char* what) {
+  TORCH_CHECK(code == DW_OK, what, " failed: ", lib.strerror(code), " (code ", code, ")");
+}
+void* stream_of(const Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+template <class T>
+T* data(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// the tensor as the kernels read it: its own memory (which may have the classes last), or a copy
+Tensor in_place(const Tensor& logits, bool copy) { return copy ? logits.contiguous() : logits; }
+Tensor workspace(const Tensor& x, int64_t bytes) {
+  // allocated for each call: calls on other streams, or captured into other graphs, have their own
+  return bytes ? at::empty({bytes}, x.options().dtype(at::kByte)) : Tensor();
+}
+std::vector<int64_t> with(at::IntArrayRef rows, int64_t at, int64_t n) {
+  std::vector<int64_t> s(rows.begin(), rows.end());
+  s.insert(s.begin() + at, n);
+  return s;
+}
+
+// The descriptor travels with the node as its bytes: the Python object it came from may be gone by then.
+std::string keep(int64_t address) { return std::string(reinterpret_cast<const char*>(address), sizeof(dw_dist_desc)); }
+dw_dist_desc kept(AutogradContext* ctx) {
+  dw_dist_desc d;
+  std::memcpy(&d, ctx->saved_data["desc"].toStringRef().data(), sizeof d);
+  return d;
+}
+// The gradients are differentiable once.  Where a pass builds a graph of itself, using that graph is an error.
+Tensor once(Tensor grad) {
+  if (!at::GradMode::is_enabled()) return grad;
+  grad = grad.detach();
+  grad.requires_grad_(true);
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with @once_differentiable", 1);
+  return (*node)({grad})[0];
+}
+
+// layout: 0 in memory order, 1 classes last, 2 neither (copied)
+struct LogProbs : torch::autograd::Function<LogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& given,
+                               int64_t desc, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout,
+                               bool train) {
+    const Tensor x = in_place(logits, layout == 2), index_in = given ? *given : Tensor(), index = contiguous(index_in);
+    const c10::OptionalDeviceGuard guard(x.device());
+    const auto f32 = x.options().dtype(at::kFloat).memory_format(std::nullopt);
+    Tensor ent = at::empty(rows, f32), lp, stats, top_lp, top_idx;
+    if (index.defined()) lp = at::empty(rows, f32);
+    if (train) stats = at::empty(with(rows, rows.size(), 3), f32);
+    if (top && layout == 1) {  // the kernels write the list of a row together, too
+      top_lp = at::empty(with(rows, rows.size(), top), f32).movedim(-1, dim);
+      top_idx = at::empty(with(rows, rows.size(), top), f32.dtype(at::kInt)).movedim(-1, dim);
+    } else if (top) {
+      top_lp = at::empty(with(rows, dim, top), f32);
+      top_idx = at::empty(with(rows, dim, top), f32.dtype(at::kInt));
+    }
+    const Tensor ws = workspace(x, nbytes);
+    check(lib.log_probs_fwd(reinterpret_cast<const dw_dist_desc*>(desc), data(x), data(index), data<float>(lp),
+                            data<float>(ent), data<float>(top_lp), data<int32_t>(top_idx), data<float>(stats), data(ws),
+                            nbytes, stream_of(x)),
+          "dw_log_probs_fwd");
+    variable_list out;
+    if (index.defined()) out.push_back(lp);
+    out.push_back(ent);
+    if (top) {
+      out.push_back(top_lp);
+      out.push_back(top_idx);
+    }
+    if (train) {
+      ctx->set_materialize_grads(false);
+      if (top) ctx->mark_non_differentiable({top_lp, top_idx});
+      ctx->save_for_backward({logits, index_in, stats});
+      ctx->saved_data["desc"] = keep(desc);
+      ctx->saved_data["copy"] = layout == 2;
+    }
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor index = contiguous(saved[1]);
+    Tensor g_lp, g_ent;
+    if (index.defined()) g_lp = contiguous(g[0]);
+    g_ent = contiguous(g[index.defined() ? 1 : 0]);
+    variable_list out(9);
+    if (!g_lp.defined() && !g_ent.defined()) return out;
+    const Tensor x = in_place(saved[0], ctx->saved_data["copy"].toBool());
+    const c10::OptionalDeviceGuard guard(x.device());
+    Tensor grad = at::empty_like(x);
+    const dw_dist_desc d = kept(ctx);
+    check(lib.log_probs_bwd(&d, data(x), data(index), data<float>(saved[2]), data<float>(g_lp), data<float>(g_ent),
+                            data(grad), stream_of(x)),
+          "dw_log_probs_bwd");
+    out[0] = once(grad);
+    return out;
+  }
+};
+
+struct Distill : torch::autograd::Function<Distill> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher_in, const Tensor& index_in,
+                        int64_t desc, int64_t nbytes, at::IntArrayRef rows, int64_t layout, bool copy_list, bool train) {
+    const Tensor x = in_place(logits, layout == 2), teacher = in_place(teacher_in, copy_list),
+                 index = in_place(index_in, copy_list);
+    const c10::OptionalDeviceGuard guard(x.device());
+    const auto f32 = x.options().dtype(at::kFloat).memory_format(std::nullopt);
+    Tensor loss = at::empty(rows, f32), stats;
+    if (train) stats = at::empty(with(rows, rows.size(), 4), f32);
+    const Tensor ws = workspace(x, nbytes);
+    check(lib.distill_fwd(reinterpret_cast<const dw_dist_desc*>(desc), data(x), data(teacher), data(index),
+                          data<float>(loss), data<float>(stats), data(ws), nbytes, stream_of(x)),
+          "dw_distill_fwd");
+    if (train) {
+      ctx->set_materialize_grads(false);
+      ctx->save_for_backward({logits, teacher_in, index_in, stats});
+      ctx->saved_data["desc"] = keep(desc);
+      ctx->saved_data["copy"] = layout == 2;
+      ctx->saved_data["copy_list"] = copy_list;
+    }
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(9);
+    if (!g[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const bool copy_list = ctx->saved_data["copy_list"].toBool();
+    const Tensor x = in_place(saved[0], ctx->saved_data["copy"].toBool()), teacher = in_place(saved[1], copy_list),
+                 index = in_place(saved[2], copy_list), up = contiguous(g[0]);
+    const c10::OptionalDeviceGuard guard(x.device());
+    Tensor grad = at::empty_like(x);
+    const dw_dist_desc d = kept(ctx);
+    check(lib.distill_bwd(&d, data(x), data(teacher), data(index), data<float>(saved[3]), data<float>(up), data(grad),
+                          stream_of(x)),
+          "dw_distill_bwd");
+    out[0] = once(grad);
+    return out;
+  }
+};
+
+// [log_prob if there is an index, entropy, and the two top lists if top > 0]
+std::vector<Tensor> log_probs(const Tensor& logits, const std::optional<Tensor>& index, int64_t desc, int64_t nbytes,
+                              at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout) {
+  const bool train = logits.requires_grad() && at::GradMode::is_enabled();
+  return LogProbs::apply(logits, index, desc, nbytes, rows, dim, top, layout, train);
+}
+Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, int64_t desc, int64_t nbytes,
+               at::IntArrayRef rows, int64_t layout, bool copy_list) {
+  const bool train = logits.requires_grad() && at::GradMode::is_enabled();
+  return Distill::apply(logits, teacher, index, desc, nbytes, rows, layout, copy_list, train);
+}
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(depthwarp, m) {
+  m.def("_bind_distribution(int strerror, int lp_fwd, int lp_bwd, int ds_fwd, int ds_bwd) -> ()", &bind);
+  m.def("_log_probs_eager(Tensor logits, Tensor? index, int desc, int nbytes, int[] rows, int dim, int top, "
+        "int layout) -> Tensor[]", &log_probs);
+  m.def("_distill_eager(Tensor logits, Tensor teacher, Tensor index, int desc, int nbytes, int[] rows, int layout, "
+        "bool copy_list) -> Tensor", &distill);
+}

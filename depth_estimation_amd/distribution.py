@@ -25,7 +25,6 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -43,26 +42,31 @@ class LogProbs(NamedTuple):
     top_index: Optional[Tensor]      # their indices, int32; ties: the lowest first
 
 
-# Host time counts: a small training step is bound by it, and the interpreter runs cold in the autograd
-# engine's own thread.  What a call's shapes and types decide -- every check, the descriptor, the workspace's
-# size -- is worked out once and kept by them (`_lp_plan`, `_ds_plan`); the backward passes get it from the
-# forward's; and the device and stream are read without building torch.cuda.Stream objects where torch
-# has the calls its own compiler uses.
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
-    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+# Host time counts: a small training step is bound by it.  What a call's shapes and types decide -- every check,
+# the descriptor, the workspace's size -- is worked out once and kept by them (`_lp_plan`, `_ds_plan`), and an eager
+# call's outputs, launches and autograd node are made in C++ (csrc/distribution_autograd.cpp).
+
+@functools.lru_cache(maxsize=None)
+def _eager():
+    """The two eager calls of libdepthwarp_torch.so, bound to the library in use."""
+    path = _lib.LIB_PATH.parent / "libdepthwarp_torch.so"
+    if not path.exists():
+        path = _lib._PKG / "libdepthwarp_torch.so"
+    if not path.exists():
+        raise _lib.DepthwarpError(f"{path} is missing: build it with `python -m depth_estimation_amd.build`. "
+                                  "There is no Python fallback for these calls.")
+    torch.ops.load_library(str(path))
+    lib = _lib.lib()
+    torch.ops.depthwarp._bind_distribution(*(C.cast(getattr(lib, n), C.c_void_p).value for n in (
+        "dw_strerror", "dw_log_probs_fwd", "dw_log_probs_bwd", "dw_distill_fwd", "dw_distill_bwd")))
+    return torch.ops.depthwarp._log_probs_eager.default, torch.ops.depthwarp._distill_eager.default
 
 
 def _call(device: torch.device, fn, *args) -> None:
     """One library call on the device's current stream (the library launches on the current device)."""
-    index = device.index
-    if _current_device() == index:
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        _lib.check(rc, fn.__name__)
+    with torch.cuda.device(device):
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, fn.__name__)
 
 
 def _workspace(x: Tensor, nbytes: int) -> Optional[Tensor]:
@@ -76,6 +80,7 @@ class _Plan(NamedTuple):
     dim: int
     rows: tuple        # shape without the class axis
     ref: object        # descriptor, for ctypes
+    address: int       # the same for C++
     nbytes: int        # workspace
     top: int = 0
     copy_list: bool = False   # distillation: the teacher's tensors have no common order
@@ -115,7 +120,7 @@ def _descriptor(workspace_of: str, shape, dim: int, last: bool, dtype, scale: fl
     nbytes = getattr(_lib.lib(), workspace_of)(ref)
     if nbytes < 0:
         _lib.check(int(nbytes), f"{workspace_of}(shape={tuple(shape)}, entries={entries}, scale={scale})")
-    return ref, nbytes
+    return ref, C.addressof(d), nbytes
 
 
 def _check_problem(shape, dtype, dim: int, scale: float) -> int:
@@ -148,12 +153,6 @@ def _check_device(logits: Tensor, **others: Optional[Tensor]) -> None:
             raise ValueError(f"{name}: expected a tensor on {logits.device}, got {t.device}")
 
 
-def _once(backward):
-    """`once_differentiable`, whose bookkeeping only a pass that builds a graph has to pay for."""
-    guarded = once_differentiable(backward)
-    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
-
-
 # ------------------------------------------------------------------------------ log-probabilities
 
 def _lp_check(shape, dtype, index_dtype, index_shape, dim: int, scale: float, top: int) -> int:
@@ -170,8 +169,8 @@ def _make_lp_plan(shape, stride, dtype, index_dtype, index_shape, dim: int, scal
     dim = _lp_check(shape, dtype, index_dtype, index_shape, dim, scale, top)
     layout = _layout(shape, stride, dim)
     flags = 0 if index_dtype is None else _INDEX_FLAGS[index_dtype]
-    ref, nbytes = _descriptor("dw_log_probs_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, top, flags)
-    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, nbytes, top)
+    ref, address, nbytes = _descriptor("dw_log_probs_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, top, flags)
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, address, nbytes, top)
 
 
 _lp_plan = functools.lru_cache(maxsize=512)(_make_lp_plan)
@@ -183,19 +182,17 @@ def _plan_of(logits: Tensor, index: Optional[Tensor], dim: int, scale: float, to
     return _lp_plan(logits.shape, logits.stride(), logits.dtype, index.dtype, index.shape, dim, scale, top)
 
 
-def _lp_forward(logits: Tensor, index: Optional[Tensor], plan: _Plan, need_stats: bool):
+def _lp_forward(logits: Tensor, index: Optional[Tensor], plan: _Plan):
     x = logits.contiguous() if plan.layout == _COPY else logits
     dev, rows, top = x.device, plan.rows, plan.top
     ent = torch.empty(rows, dtype=torch.float32, device=dev)
-    lp = lp_ptr = index_ptr = stats = stats_ptr = top_lp = top_lp_ptr = top_idx = top_idx_ptr = ws = None
+    stats = torch.empty(rows + (3,), dtype=torch.float32, device=dev)
+    lp = lp_ptr = index_ptr = top_lp = top_lp_ptr = top_idx = top_idx_ptr = None
     if index is not None:
         index = index.contiguous()
         index_ptr = index.data_ptr()
         lp = torch.empty(rows, dtype=torch.float32, device=dev)
         lp_ptr = lp.data_ptr()
-    if need_stats:
-        stats = torch.empty(rows + (3,), dtype=torch.float32, device=dev)
-        stats_ptr = stats.data_ptr()
     if top:
         if plan.layout == _LAST:   # the kernels write the list of a row together, too
             top_lp = torch.empty(rows + (top,), dtype=torch.float32, device=dev).movedim(-1, plan.dim)
@@ -205,11 +202,9 @@ def _lp_forward(logits: Tensor, index: Optional[Tensor], plan: _Plan, need_stats
             top_lp = torch.empty(shape, dtype=torch.float32, device=dev)
             top_idx = torch.empty(shape, dtype=torch.int32, device=dev)
         top_lp_ptr, top_idx_ptr = top_lp.data_ptr(), top_idx.data_ptr()
-        ws = _workspace(x, plan.nbytes)
-    elif plan.nbytes:
-        ws = _workspace(x, plan.nbytes)
+    ws = _workspace(x, plan.nbytes)
     _call(dev, _lib.lib().dw_log_probs_fwd, plan.ref, x.data_ptr(), index_ptr, lp_ptr, ent.data_ptr(), top_lp_ptr,
-          top_idx_ptr, stats_ptr, None if ws is None else ws.data_ptr(), plan.nbytes)
+          top_idx_ptr, stats.data_ptr(), None if ws is None else ws.data_ptr(), plan.nbytes)
     return lp, ent, top_lp, top_idx, stats
 
 
@@ -232,37 +227,13 @@ def _lp_backward(logits: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: O
     return grad
 
 
-def _lp_node_backward(ctx, g_lp, g_ent, *_g_top):
-    if g_lp is None and g_ent is None:
-        return None, None, None
-    logits, index = ctx.saved_tensors
-    return _lp_backward(logits, index, ctx.stats, g_lp, g_ent, ctx.plan), None, None
-
-
-class _LogProbsFunction(torch.autograd.Function):
-    """Eager calls with a gradient skip the operator dispatcher."""
-
-    @staticmethod
-    def forward(ctx, logits, index, plan):
-        lp, ent, top_lp, top_idx, ctx.stats = _lp_forward(logits, index, plan, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, index)
-        ctx.plan = plan
-        if not plan.top:
-            return lp, ent
-        ctx.mark_non_differentiable(top_lp, top_idx)
-        return lp, ent, top_lp, top_idx
-
-    backward = staticmethod(_once(_lp_node_backward))
-
-
-# The same as torch operators, which is what torch.compile traces.  An operator always returns tensors:
+# Torch operators with the same results, which is what torch.compile traces.  An operator always returns tensors:
 # without an index, log_prob is empty; the last result is for the backward pass.
 
 @torch.library.custom_op("depthwarp::log_probs", mutates_args=())
 def _log_probs_op(logits: Tensor, index: Optional[Tensor], dim: int, scale: float,
                   top: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    lp, ent, top_lp, top_idx, stats = _lp_forward(logits, index, _plan_of(logits, index, dim, scale, top), True)
+    lp, ent, top_lp, top_idx, stats = _lp_forward(logits, index, _plan_of(logits, index, dim, scale, top))
     if lp is None:
         lp = ent.new_empty((0,))
     if not top:
@@ -332,7 +303,8 @@ def log_probs(logits: Tensor, index: Optional[Tensor] = None, *, dim: int = 1, s
     gradient 0.  A row with NaN (or +inf) has NaN results.  A row that gets no upstream gradient gets
     zeros whatever it holds.
     """
-    _check_device(logits, index=index)
+    if not logits.is_cuda or (index is not None and index.device != logits.device):
+        _check_device(logits, index=index)
     scale, top = float(scale), int(top)
     if torch.compiler.is_compiling():
         dim = _lp_check(logits.shape, logits.dtype, None if index is None else index.dtype,
@@ -340,10 +312,10 @@ def log_probs(logits: Tensor, index: Optional[Tensor] = None, *, dim: int = 1, s
         lp, ent, top_lp, top_idx, _ = _log_probs_op(logits, index, dim, scale, top)
         return LogProbs(None if index is None else lp, ent, top_lp if top else None, top_idx if top else None)
     plan = _plan_of(logits, index, dim, scale, top)
-    if logits.requires_grad and torch.is_grad_enabled():
-        out = _LogProbsFunction.apply(logits, index, plan)
-        return LogProbs(*out) if top else LogProbs(*out, None, None)
-    return LogProbs(*_lp_forward(logits, index, plan, False)[:4])
+    out = _eager()[0](logits, index, plan.address, plan.nbytes, plan.rows, plan.dim, top, plan.layout)
+    if index is None:
+        return LogProbs(None, *out) if top else LogProbs(None, out[0], None, None)
+    return LogProbs(*out) if top else LogProbs(*out, None, None)
 
 
 # --------------------------------------------------------------------------------- distillation
@@ -371,8 +343,8 @@ def _make_ds_plan(shape, stride, dtype, t_shape, t_stride, t_dtype, i_shape, i_s
     strides = (k * inner, 1, k) if not copy and t_layout == _LAST else (k * inner, inner, 1)
     layout = _layout(shape, stride, dim)
     flags = _INDEX_FLAGS[i_dtype] | _TEACHER_FLAGS[t_dtype] | (_lib.DW_DIST_RENORMALISE if renormalise else 0)
-    ref, nbytes = _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k, flags, strides)
-    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, nbytes, copy_list=copy)
+    ref, address, nbytes = _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k, flags, strides)
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, address, nbytes, copy_list=copy)
 
 
 _ds_plan = functools.lru_cache(maxsize=512)(_make_ds_plan)
@@ -383,16 +355,15 @@ def _ds_plan_of(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale:
                     index.shape, index.stride(), index.dtype, dim, scale, renormalise)
 
 
-def _ds_forward(logits: Tensor, teacher: Tensor, index: Tensor, plan: _Plan, need_stats: bool):
+def _ds_forward(logits: Tensor, teacher: Tensor, index: Tensor, plan: _Plan):
     x = logits.contiguous() if plan.layout == _COPY else logits
     if plan.copy_list:
         teacher, index = teacher.contiguous(), index.contiguous()
     loss = torch.empty(plan.rows, dtype=torch.float32, device=x.device)
-    stats = torch.empty(plan.rows + (4,), dtype=torch.float32, device=x.device) if need_stats else None
+    stats = torch.empty(plan.rows + (4,), dtype=torch.float32, device=x.device)
     ws = _workspace(x, plan.nbytes)
     _call(x.device, _lib.lib().dw_distill_fwd, plan.ref, x.data_ptr(), teacher.data_ptr(), index.data_ptr(),
-          loss.data_ptr(), None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(),
-          plan.nbytes)
+          loss.data_ptr(), stats.data_ptr(), None if ws is None else ws.data_ptr(), plan.nbytes)
     return loss, stats
 
 
@@ -407,26 +378,10 @@ def _ds_backward(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, 
     return grad
 
 
-def _ds_node_backward(ctx, g_loss):
-    logits, teacher, index = ctx.saved_tensors
-    return _ds_backward(logits, teacher, index, ctx.stats, g_loss, ctx.plan), None, None, None
-
-
-class _DistillFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher, index, plan):
-        loss, ctx.stats = _ds_forward(logits, teacher, index, plan, True)
-        ctx.save_for_backward(logits, teacher, index)
-        ctx.plan = plan
-        return loss
-
-    backward = staticmethod(_once(_ds_node_backward))
-
-
 @torch.library.custom_op("depthwarp::distill_loss", mutates_args=())
 def _distill_op(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale: float,
                 renormalise: bool) -> Tuple[Tensor, Tensor]:
-    return _ds_forward(logits, teacher, index, _ds_plan_of(logits, teacher, index, dim, scale, renormalise), True)
+    return _ds_forward(logits, teacher, index, _ds_plan_of(logits, teacher, index, dim, scale, renormalise))
 
 
 @_distill_op.register_fake
@@ -478,7 +433,8 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
     without entries has loss and gradient 0.  A class listed twice counts with both entries.  The loss
     is +inf where the teacher lists a class the student has at -inf.
     """
-    _check_device(logits, teacher=teacher, teacher_index=teacher_index)
+    if not (logits.is_cuda and teacher.device == logits.device == teacher_index.device):
+        _check_device(logits, teacher=teacher, teacher_index=teacher_index)
     scale, renormalise = float(scale), bool(renormalise)
     if teacher.requires_grad and torch.is_grad_enabled():
         raise ValueError("teacher: no gradient flows to the teacher; pass teacher.detach()")
@@ -487,6 +443,4 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
                         teacher_index.dtype, dim, scale)
         return _distill_op(logits, teacher, teacher_index, dim, scale, renormalise)[0]
     plan = _ds_plan_of(logits, teacher, teacher_index, dim, scale, renormalise)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _DistillFunction.apply(logits, teacher, teacher_index, plan)
-    return _ds_forward(logits, teacher, teacher_index, plan, False)[0]
+    return _eager()[1](logits, teacher, teacher_index, plan.address, plan.nbytes, plan.rows, plan.layout, plan.copy_list)
