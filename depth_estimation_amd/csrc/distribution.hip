@@ -1484,7 +1484,8 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
   const int begin = chunk * p.chunk, end = min(p.V, begin + p.chunk);
   const Side z = side(p);
   extern __shared__ float cell_best[];  // [cell][thread]
-  const int steps = (end - begin + NT * 32 - 1) / (NT * 32), span = cell_span(steps);
+  // (the span is that of a whole chunk, which the launch makes room for: a short last one could have more cells)
+  const int steps = (end - begin + NT * 32 - 1) / (NT * 32), span = cell_span((p.chunk + NT * 32 - 1) / (NT * 32));
   float so_far = -kInf;
   int cell = 0, in_cell = 0;
   // the given class, on its way while the row is read
@@ -1788,6 +1789,7 @@ __global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S*
 
 // ---- host side -----------------------------------------------------------------------------------------------
 constexpr int64_t kMaxClasses = 1 << 28;   // the order keys hold 29 bits of index
+constexpr int64_t kMaxThreads = 0xffffffff; // of a launch
 constexpr int kWantWaves = 2048;           // 8 a compute unit: enough loads in flight
 // A gradient from this size on is stored past the caches.  It would fill half of the 256 MB last-level cache or
 // more, and what comes next would have to wait while that is written back: the next forward pass over 4096 x
@@ -1864,7 +1866,7 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
       while (P.nw > 1 && P.nw * (kStageBytes + 64 * (12 + 8 * 16)) > (int)kLdsBudget) P.nw /= 2;
     }
     p.cpw = (stages + P.nw - 1) / P.nw * stage;
-    if (tiles > 0x7fffffff) return DW_ERR_SHAPE;
+    if (tiles > kMaxThreads / (P.nw * 64)) return DW_ERR_SHAPE;
     P.grid = (unsigned)tiles;
     return DW_OK;
   }
@@ -1880,7 +1882,7 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
   const int64_t tiles_each = (most + chunks - 1) / chunks;
   p.chunk = (int)(tiles_each * block_tile < p.V ? tiles_each * block_tile : p.V);
   p.chunks = (int)((p.V + (int64_t)p.chunk - 1) / p.chunk);
-  if (p.rows > 0x7fffffff / p.chunks) return DW_ERR_SHAPE;
+  if (p.rows > kMaxThreads / P.nt / p.chunks) return DW_ERR_SHAPE;
   P.grid = (unsigned)(p.rows * p.chunks);
   if (!backward && p.chunks > 1) {
     P.ws = parts_bytes(p.rows, p.chunks);

@@ -89,7 +89,10 @@ def _desc(outer=2, classes=8, inner=1, scale=1.0, dtype=0, entries=2, flags=0):
 BAD = [(dict(classes=0), -2), (dict(classes=(1 << 28) + 1), -2), (dict(outer=-1), -2), (dict(inner=-1), -2),
        (dict(entries=-1), -2), (dict(entries=65), -2), (dict(dtype=3), -5), (dict(dtype=-1), -5), (dict(flags=64), -5),
        (dict(scale=0.0), -5), (dict(scale=INF), -5), (dict(scale=float("nan")), -5),
-       (dict(outer=1 << 41), -2), (dict(outer=1 << 39, inner=1 << 39), -2), (dict(outer=1 << 30, classes=1 << 27), -2)]
+       (dict(outer=1 << 41), -2), (dict(outer=1 << 39, inner=1 << 39), -2), (dict(outer=1 << 30, classes=1 << 27), -2),
+       # more threads than a launch can have
+       (dict(outer=1 << 24, classes=5000), -2), (dict(outer=1 << 26, classes=2100), -2), (dict(outer=1 << 38, classes=8), -2),
+       (dict(outer=1 << 26, inner=64, classes=1), -2)]
 
 
 @pytest.mark.parametrize("kw,code", BAD)

@@ -176,6 +176,30 @@ def test_top_of_rows_whose_large_values_lie_in_one_threads_classes(n):
         _check_log_probs(x.to(dtype), torch.zeros(n, dtype=torch.long), "rows", 1.0, 64, with_grad=False)
 
 
+# blocks of more than 16 steps: a kept maximum stands for several; the last block of a row is shorter, so that
+# it alone would need more of them (17 and 16 steps)
+@pytest.mark.parametrize("n,V,top", [(300, 33 * 8192, 64), (300, 33 * 8192 - 5, 3), (520, 140001, 64)])
+def test_top_of_blocks_of_many_steps(n, V, top):
+    from depth_estimation_amd.distribution import log_probs
+    g = torch.Generator(device="cuda").manual_seed(n + V)
+    x = torch.randn(n, V, generator=g, device="cuda").bfloat16()
+    x[3] = 1.0                               # constant
+    x[4, :-2] = -INF                         # two classes left
+    x[5, V // 2:] += 3                       # the large values in the last half
+    out = log_probs(x, top=top)
+    for i in (0, 1, 2, 3, 4, 5, n - 1):
+        row = x[i].cpu().double()
+        _, want = torch.sort(row, descending=True, stable=True)
+        assert torch.equal(out.top_index[i].cpu().long(), want[:top])
+        lp = torch.log_softmax(row, 0)[want[:top]]
+        t = (row.amax() - row[want[:top]]).nan_to_num(0, 0, 0)
+        _close(out.top_log_prob[i], lp, _factor(V) + 4 * U * t, "top_log_prob")
+    # every list is descending, and no class comes twice
+    assert (out.top_log_prob[:, 1:] <= out.top_log_prob[:, :-1]).all()
+    listed = out.top_index.long().sort(1).values
+    assert (listed[:, 1:] > listed[:, :-1]).all()
+
+
 @pytest.mark.parametrize("layout", ["volume", "last", "rows", "many"])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_log_probs_masks_and_special_values(layout, dtype):
@@ -632,6 +656,74 @@ def test_forward_and_backward_in_two_captured_graphs(shape):
         for p, o in ((a, outs[0]), (b, outs[1])):
             for got, want in zip(o, _both(*p)):
                 assert torch.equal(got, want)
+
+
+def test_two_threads_on_their_own_streams_give_the_same_bits():
+    import threading
+    problems = [_problem((3, 40000), 0), _problem((1, 64, 24, 80), 1)]
+    wants = [_both(*p) for p in problems]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(p, want):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got = _both(*p)
+                    s.synchronize()
+                    bad.extend(1 for a, b in zip(got, want) if not torch.equal(a, b))
+        except Exception as e:   # noqa: BLE001  (a thread's error has to reach the test)
+            bad.append(e)
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(problems, wants)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad[:2]
+
+
+def test_autograd_modes():
+    from torch.utils.checkpoint import checkpoint
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x, idx, t, ti = _problem((2, 20, 4, 6), 0)
+
+    def f(v):
+        o = log_probs(v, idx, scale=-1.0, top=2)
+        return o.log_prob.sum() + o.entropy.sum() + distill_loss(v, t, ti).sum()
+
+    want = f(x)
+    gw, = torch.autograd.grad(want, x)
+    for use_reentrant in (False, True):
+        y = checkpoint(f, x, use_reentrant=use_reentrant)
+        y.backward()
+        assert torch.equal(y, want) and torch.equal(x.grad, gw)
+        x.grad = None
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            y = f(x)
+        assert torch.equal(y, want) and not y.requires_grad
+    # a result that is not used takes no part
+    g, = torch.autograd.grad(log_probs(x, idx).entropy.sum(), x)
+    h, = torch.autograd.grad(log_probs(x).entropy.sum(), x)
+    assert torch.equal(g, h)
+    # what the backward pass needs must not be overwritten before it
+    for tensor in (x.detach(), idx):
+        y = log_probs(x, idx).log_prob.sum()
+        tensor.add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    for tensor in (t, ti):
+        y = distill_loss(x, t, ti).sum()
+        tensor.add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    # function transforms do not reach the kernels
+    with pytest.raises(RuntimeError):
+        torch.func.grad(f)(x.detach())
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda v: log_probs(v, dim=0).entropy)(x.detach())
 
 
 def test_registered_operators():
