@@ -126,14 +126,14 @@ def test_log_probs_rows(n, V, dtype):
 
 # enough rows that a thread takes one; the last tile is not full
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V,top", [(1, 1), (7, 4), (31, 3), (32, 8), (33, 9), (63, 0), (64, 16), (65, 17), (129, 33)])
+@pytest.mark.parametrize("V,top", [(1, 1), (7, 4), (31, 3), (32, 8), (33, 9), (63, 0), (64, 16), (65, 17), (129, 33), (96, 64)])
 def test_log_probs_many_short_rows(V, top, dtype):
     x, _ = _make("rows", (8200, V), dtype, seed=V)
     _check_log_probs(x, _index((8200,), V, V), "rows", [1.0, -0.5][V % 2], top)
 
 
 VOLUMES = [(1, 1, 1, 1), (1, 5, 1, 3), (2, 31, 3, 5), (1, 32, 8, 8), (2, 33, 5, 13), (1, 64, 9, 7), (3, 65, 1, 65),
-           (1, 96, 24, 80), (2, 193, 11, 17), (1, 256, 16, 40), (1, 1025, 3, 30)]
+           (1, 96, 24, 80), (2, 193, 11, 17), (1, 256, 16, 40), (1, 1025, 3, 30), (1, 8192, 2, 7), (1, 8193, 3, 5), (1, 8230, 1, 70)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
