@@ -657,8 +657,11 @@ __device__ __forceinline__ void settle(float (&v)[32], float far, int n) {
 // ---- log-probabilities, forward, tile ---------------------------------------------------------------
 // K: top classes kept in registers as keys of kind P (0: none).  More than K wanted: further passes over the data,
 // each for the next K below the last key of the pass before.
+// Turning rows and keeping their lists takes up to 180 registers: those blocks have at most 8 waves, so that they get
+// them (192 classes of 2 x 192 x 320 pixels f32: the top 8 in 31 us, 41 with 128 registers; bf16 the same either way).
+constexpr int list_waves(bool last, bool list) { return last && list ? 8 : 16; }
 template <class T, bool LAST, class P, int K>
-__global__ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
+__global__ __launch_bounds__(64 * list_waves(LAST, K > 0)) void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
                             float* __restrict__ log_prob, float* __restrict__ entropy, float* __restrict__ top_lp,
                             int32_t* __restrict__ top_idx, Stats3* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
@@ -1870,8 +1873,9 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
   if (P.tile) {
     const int stage = P.last ? kSegBytes / esize : 32;
     const int stages = (p.V + stage - 1) / stage;
+    const int most = distill || backward ? 16 : list_waves(P.last, p.k > 0);
     P.nw = 1;
-    while (P.nw < 16 && tiles * P.nw < kWantWaves && P.nw * 2 <= stages) P.nw *= 2;
+    while (P.nw < most && tiles * P.nw < kWantWaves && P.nw * 2 <= stages) P.nw *= 2;
     if (distill) {
       // The list is the block's, a stage each wave's, so more waves a block are more waves in the LDS of a compute
       // unit.  The forward pass ends with one wave's work: it takes that only where fewer than 8 waves would fit
