@@ -17,6 +17,10 @@
 //         load); rows whose classes lie together are turned through LDS, 128 bytes of each row at
 //         a time.  No cross-lane work at all, and the top classes stay sorted in registers.
 //   row   a block (or a few, joined by a second kernel) for each row, for rows that are long or few.
+//
+// Every pass reads the logits once and a backward pass writes as much again, so the bound is memory: a large copy
+// moves 4.8 TB/s on this chip, a large read 5.4.  Next to it stands the vector pipe, with 11 instructions a class in
+// the forward pass and a quarter-rate exp2 among them.  The figures at the kernels are times of the kernel alone.
 #include <type_traits>
 
 #include "dw_common.h"
@@ -335,7 +339,8 @@ struct Narrow {
 __device__ __forceinline__ void order_nans(float (&v)[32]) {
 #pragma unroll
   for (int u = 0; u < 32; ++u)
-    asm volatile("v_cmp_u_f32 vcc, %0, %0\n\ts_nop 1\n\tv_cndmask_b32 %0, %0, %1, vcc" : "+v"(v[u]) : "v"(__builtin_nanf("")) : "vcc");
+    asm volatile("v_cmp_u_f32 vcc, %0, %0\n\ts_nop 1\n\tv_cndmask_b32 %0, %0, %1, vcc"
+                 : "+v"(v[u]) : "v"(__builtin_nanf("")) : "vcc");
 }
 template <class P>
 __device__ __forceinline__ void order2(typename P::Key& hi, typename P::Key& lo) {
@@ -655,13 +660,19 @@ __device__ __forceinline__ void settle(float (&v)[32], float far, int n) {
 }
 
 // ---- log-probabilities, forward, tile ---------------------------------------------------------------
+// A thread a row keeps the whole soft-max in its own registers: a block a row, as in the row kernels, would spend a
+// reduction over 64 lanes on every few hundred classes.  The waves of a block split the classes where there are
+// too few rows to fill the chip, and join through LDS.  Loads of the next 32 classes are issued before the ones at
+// hand are worked on.  12 x 64 x 96 x 320 bf16 (47 MB): 15.8 us, 3.0 TB/s, the vector pipe; 1 x 256 x 256 x 512 f32 with
+// the top 8 (134 MB): 34 us, 4.0 TB/s; 4 x 193 x 96 x 320 f16, classes last (47 MB): 18.4 us.
 // K: top classes kept in registers as keys of kind P (0: none).  More than K wanted: further passes over the data,
 // each for the next K below the last key of the pass before.
 // Turning rows and keeping their lists takes up to 180 registers: those blocks have at most 8 waves, so that they get
 // them (192 classes of 2 x 192 x 320 pixels f32: the top 8 in 31 us, 41 with 128 registers; bf16 the same either way).
 constexpr int list_waves(bool last, bool list) { return last && list ? 8 : 16; }
 template <class T, bool LAST, class P, int K>
-__global__ __launch_bounds__(64 * list_waves(LAST, K > 0)) void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
+__global__ __launch_bounds__(64 * list_waves(LAST, K > 0))
+void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
                             float* __restrict__ log_prob, float* __restrict__ entropy, float* __restrict__ top_lp,
                             int32_t* __restrict__ top_idx, Stats3* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
@@ -806,6 +817,9 @@ __device__ __forceinline__ float lp_grad(const LpCoef& r, float v, float c, floa
   return fmaf(e, ENT ? fmaf(vmax(t, kFloor), r.k1, r.k0) : r.k0, add);
 }
 
+// The rows' sums come from the forward pass, so this is one read and one write: dx_j = e_j (k0 + k1 t_j), and the
+// given class on top.  12 x 64 x 96 x 320 bf16 (94 MB): 20.0 us, 4.7 TB/s, what a copy takes.  4 x 193 x 96 x 320 f16, classes
+// last (95 MB): 28 us; rows of 386 bytes begin inside the memory's lines, and 66 MB are written for 47.
 template <class T, bool LAST, bool ENT>
 __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
                             const Stats3* __restrict__ stats, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
@@ -962,7 +976,10 @@ __device__ __forceinline__ void take_listed(const C& col, const int* idx, int K,
 // ---- distillation, forward, tile ------------------------------------------------------------------------
 // Each listed class is taken out of its column before the running soft-max sees the column, so the
 // unlisted classes are summed on their own (1 - sum of the listed would cancel where the list holds
-// nearly everything).
+// nearly everything).  The list lies in LDS, a column a lane, so that 64 entries cost no registers; every
+// entry is looked up in every stage, eight at a time, which is what long lists cost (192 classes of 2 x 192 x 640
+// pixels bf16: 36 us with 8 entries, 49 with 16).  4 x 256 x 192 x 640 bf16, 8 entries (252 + 31 MB): 68 us, 4.2 TB/s;
+// 12 x 128 x 96 x 320 f16, classes last (94 + 25 MB): 32 us, 3.7 TB/s; 1 x 64 x 24 x 80: 6.6 us, the launch's latency.
 template <class T, bool LAST>
 __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ teacher,
                             const void* __restrict__ index, float* __restrict__ loss, float4* __restrict__ stats) {
@@ -1088,6 +1105,9 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
 }
 
 // ---- distillation, backward, tile -------------------------------------------------------------------------
+// The stage becomes gradients in place: the listed classes' values are taken out and their gradients worked out in
+// the list's columns, the others' are e_j times one factor, and the listed ones are put back last, a class that is
+// listed twice with the sum.  4 x 256 x 192 x 640 bf16, 8 entries (503 + 31 MB): 112 us, 4.8 TB/s, what a copy takes.
 template <class T, bool LAST>
 __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ teacher,
                             const void* __restrict__ index, const float4* __restrict__ stats,
@@ -1200,7 +1220,11 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
 }
 
 // ---- row kernels -------------------------------------------------------------------------------------------
-// A wave takes 2048 neighbouring classes at a time, 32 a lane in 16-byte pieces.
+// A wave takes 2048 neighbouring classes at a time, 32 a lane in 16-byte pieces: every instruction moves 1 KB
+// of neighbouring bytes, whatever the row's alignment.  64 threads a block up to 4096 classes, else 256; few rows are split
+// until 2048 waves are at work, and joined in a fixed order, so that a result does not depend on which block
+// ends first.  Forward, 4096 x 32768 bf16 (268 MB): 56 us, 4.8 TB/s.  Backward (537 MB): 85 us, 6.3 TB/s, part of the logits
+// still in the last-level cache.  One row of 32768: 8.4 us with its top 20 and 4.6 for the join, both latency.
 constexpr int kWaveTile = 64 * 32;
 template <class T>
 __device__ __forceinline__ int tile_class(int lane, int u) {  // class of a lane's u-th value inside the wave's tile
@@ -1646,6 +1670,9 @@ __global__ __launch_bounds__(NT, 4) void lp_row_bwd(Prob p, const typename T::S*
 }
 
 // ---- distillation over long rows: every wave holds the whole list, one entry a lane --------------------
+// Which of a wave's 2048 classes are listed is one ballot; what is listed, hardly one in a tile, is patched in
+// registers.  2048 x 131072 bf16, 64 entries: forward (537 MB) 107 us, 5.0 TB/s, backward (1.07 GB) 194 us, 5.5 TB/s.
+// 333 x 50001 f32, 20 entries: 19.4 us + 6.0 (join), backward 27; 5 x 131072: 7.5 + 6.3 and 8.0, latency.
 struct Entry {
   int idx;      // -1: none
   float value;  // the teacher's, after the shift (a log-probability)

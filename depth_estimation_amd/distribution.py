@@ -15,6 +15,10 @@ Logits are float32, bfloat16 or float16; the class axis is `dim` (1, as in a (B,
 temperature.  Tensors in memory order, or with the class axis last in memory (torch's channels_last),
 are read where they are; any other order is copied first.  Sums and results are float32, gradients
 have the type and the memory order of the logits.
+
+Calls can be captured into a graph, backward passes with them; workspaces belong to the call, so graphs do
+not share them.  While a backward pass is captured, no eager graph of the same leaves may be alive (torch
+ends the process): drop the eager results first, or capture `torch.autograd.grad`.
 """
 from __future__ import annotations
 

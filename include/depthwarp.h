@@ -387,7 +387,8 @@ DW_API int dw_lidar_project(int32_t B, int32_t n_max, int32_t H, int32_t W, cons
  *   Rows behind the last, and bytes between rows, are neither read nor written.
  * ------------------------------------------------------------------------- */
 typedef struct dw_dist_desc {
-  int64_t outer, classes, inner; /* 1 <= classes <= 2^28; outer or inner may be 0: nothing to do */
+  int64_t outer, classes, inner; /* 1 <= classes <= 2^28; outer or inner may be 0: nothing to do.  More rows than one
+                                    launch takes (2^24 long ones, 2^32 of at most 2048 classes) are DW_ERR_SHAPE */
   int64_t entry_stride[3];       /* distillation: element strides of the teacher's list along outer, entry, inner */
   float scale;                   /* finite, not 0 */
   int32_t dtype;                 /* of the logits and their gradient: DW_DTYPE_* */
