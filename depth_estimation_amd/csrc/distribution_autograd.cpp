@@ -49,9 +49,17 @@ void* stream_of(const Tensor& t) {
 template <class T>
 T* data(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// (a tensor may stand for its memory's values with the other sign: at::_neg_view)
+Tensor contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 // the tensor as the kernels read it: its own memory (which may have the classes last), or a copy
-Tensor in_place(const Tensor& logits, bool copy) { return copy ? logits.contiguous() : logits; }
+Tensor in_place(const Tensor& t, bool copy) { return copy ? contiguous(t) : t.resolve_neg(); }
+// The same in the backward pass.  What was saved has its own strides there, unless hooks for saved tensors brought it
+// back in another order: then it is put into the one the descriptor tells of.
+Tensor saved_in_place(const Tensor& t, bool copy, at::IntArrayRef strides) {
+  const Tensor x = in_place(t, copy);
+  if (copy || x.strides() == strides) return x;
+  return at::empty_strided(x.sizes(), strides, x.options()).copy_(x);
+}
 Tensor workspace(const Tensor& x, int64_t bytes) {
   // allocated for each call: calls on other streams, or captured into other graphs, have their own
   return bytes ? at::empty({bytes}, x.options().dtype(at::kByte)) : Tensor();
@@ -115,22 +123,23 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
       ctx->save_for_backward({logits, index_in, stats});
       ctx->saved_data["desc"] = keep(desc);
       ctx->saved_data["copy"] = layout == 2;
+      ctx->saved_data["strides"] = x.strides().vec();
     }
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor index = contiguous(saved[1]);
+    const Tensor index = contiguous(saved[1]), stats = contiguous(saved[2]);
     Tensor g_lp, g_ent;
     if (index.defined()) g_lp = contiguous(g[0]);
     g_ent = contiguous(g[index.defined() ? 1 : 0]);
     variable_list out(9);
     if (!g_lp.defined() && !g_ent.defined()) return out;
-    const Tensor x = in_place(saved[0], ctx->saved_data["copy"].toBool());
-    const c10::OptionalDeviceGuard guard(x.device());
+    const c10::OptionalDeviceGuard guard(saved[0].device());
+    const Tensor x = saved_in_place(saved[0], ctx->saved_data["copy"].toBool(), ctx->saved_data["strides"].toIntVector());
     Tensor grad = at::empty_like(x);
     const dw_dist_desc d = kept(ctx);
-    check(lib.log_probs_bwd(&d, data(x), data(index), data<float>(saved[2]), data<float>(g_lp), data<float>(g_ent),
+    check(lib.log_probs_bwd(&d, data(x), data(index), data<float>(stats), data<float>(g_lp), data<float>(g_ent),
                             data(grad), stream_of(x)),
           "dw_log_probs_bwd");
     out[0] = once(grad);
@@ -157,6 +166,9 @@ struct Distill : torch::autograd::Function<Distill> {
       ctx->saved_data["desc"] = keep(desc);
       ctx->saved_data["copy"] = layout == 2;
       ctx->saved_data["copy_list"] = copy_list;
+      ctx->saved_data["strides"] = x.strides().vec();
+      ctx->saved_data["teacher_strides"] = teacher.strides().vec();
+      ctx->saved_data["index_strides"] = index.strides().vec();
     }
     return loss;
   }
@@ -165,12 +177,15 @@ struct Distill : torch::autograd::Function<Distill> {
     if (!g[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const bool copy_list = ctx->saved_data["copy_list"].toBool();
-    const Tensor x = in_place(saved[0], ctx->saved_data["copy"].toBool()), teacher = in_place(saved[1], copy_list),
-                 index = in_place(saved[2], copy_list), up = contiguous(g[0]);
-    const c10::OptionalDeviceGuard guard(x.device());
+    const c10::OptionalDeviceGuard guard(saved[0].device());
+    auto& data_of = ctx->saved_data;
+    const Tensor x = saved_in_place(saved[0], data_of["copy"].toBool(), data_of["strides"].toIntVector()),
+                 teacher = saved_in_place(saved[1], copy_list, data_of["teacher_strides"].toIntVector()),
+                 index = saved_in_place(saved[2], copy_list, data_of["index_strides"].toIntVector()),
+                 stats = contiguous(saved[3]), up = contiguous(g[0]);
     Tensor grad = at::empty_like(x);
     const dw_dist_desc d = kept(ctx);
-    check(lib.distill_bwd(&d, data(x), data(teacher), data(index), data<float>(saved[3]), data<float>(up), data(grad),
+    check(lib.distill_bwd(&d, data(x), data(teacher), data(index), data<float>(stats), data<float>(up), data(grad),
                           stream_of(x)),
           "dw_distill_bwd");
     out[0] = once(grad);

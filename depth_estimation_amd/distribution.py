@@ -215,7 +215,7 @@ def _lp_forward(logits: Tensor, index: Optional[Tensor], plan: _Plan):
 def _lp_backward(logits: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: Optional[Tensor],
                  g_ent: Optional[Tensor], plan: _Plan) -> Tensor:
     x = logits.contiguous() if plan.layout == _COPY else logits
-    grad = torch.empty_like(x)
+    grad, stats = torch.empty_like(x), stats.contiguous()
     index_ptr = g_lp_ptr = g_ent_ptr = None
     if index is not None:
         index = index.contiguous()
@@ -376,7 +376,7 @@ def _ds_backward(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, 
     if plan.copy_list:
         teacher, index = teacher.contiguous(), index.contiguous()
     grad = torch.empty_like(x)
-    g_loss = g_loss.contiguous()
+    stats, g_loss = stats.contiguous(), g_loss.contiguous()
     _call(x.device, _lib.lib().dw_distill_bwd, plan.ref, x.data_ptr(), teacher.data_ptr(), index.data_ptr(),
           stats.data_ptr(), g_loss.data_ptr(), grad.data_ptr())
     return grad

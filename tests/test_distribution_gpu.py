@@ -726,6 +726,62 @@ def test_autograd_modes():
         torch.vmap(lambda v: log_probs(v, dim=0).entropy)(x.detach())
 
 
+@pytest.mark.parametrize("layout", ["volume", "last"])
+def test_saved_tensors_that_come_back_in_another_order(layout):
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x, idx, t, ti = (_gpu(v.detach().cpu(), layout) if v.dim() == 4 else v for v in _problem((2, 20, 4, 6), 0))
+    x.requires_grad_(True)
+
+    def f(v):
+        o = log_probs(v, idx, scale=-1.0)
+        return o.log_prob.sum() + o.entropy.sum() + distill_loss(v, t, ti).sum()
+
+    want, = torch.autograd.grad(f(x), x)
+    for unpack in (lambda s: s.contiguous(), lambda s: s.cpu().contiguous().cuda(),
+                   lambda s: s.movedim(1, -1).contiguous().movedim(-1, 1) if s.dim() == 4 else s):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s.detach().clone(), unpack):
+            y = f(x)
+        got, = torch.autograd.grad(y, x)
+        assert torch.equal(got, want)
+    with torch.autograd.graph.save_on_cpu():
+        y = f(x)
+    got, = torch.autograd.grad(y, x)
+    assert torch.equal(got, want) and got.stride() == x.stride()
+
+
+def test_negated_views_and_indices_far_outside():
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x, idx, t, ti = _problem((2, 20, 4, 6), 0)
+    n, m = torch._neg_view(x.detach()).requires_grad_(True), (-x.detach()).requires_grad_(True)
+    idx = idx.clone()
+    idx[0, 0, 0], idx[0, 0, 1], idx[0, 0, 2] = 1 << 40, (1 << 32) + 3, -(1 << 33) + 3
+    a, b = log_probs(n, idx, top=3), log_probs(m, idx, top=3)
+    la, lb = distill_loss(n, torch._neg_view(-t), ti), distill_loss(m, t, ti)
+    for p, q in zip(a + (la,), b + (lb,)):
+        assert torch.equal(p, q)
+    assert (a.log_prob[0, 0, :3] == 0).all()
+    up = torch.rand_like(la)
+    ga, = torch.autograd.grad([a.log_prob, a.entropy, la], n, [torch._neg_view(-up), up, torch._neg_view(-up)])
+    gb, = torch.autograd.grad([b.log_prob, b.entropy, lb], m, [up, up, up])
+    assert torch.equal(ga, gb)
+
+
+def test_traced_calls_with_changing_sizes():
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+
+    def f(x, idx, t, ti):
+        o = log_probs(x, idx, scale=-1.0, top=2)
+        return o.log_prob.sum() + o.entropy.sum() + distill_loss(x, t, ti, renormalise=True).sum()
+
+    g = torch.compile(f, backend="aot_eager", dynamic=True)
+    for shape in ((2, 20, 4, 6), (3, 33, 5, 9), (1, 64, 7, 11)):
+        p = _problem(shape, 0)
+        want, got = f(*p), g(*p)
+        gw, = torch.autograd.grad(want, p[0])
+        gg, = torch.autograd.grad(got, p[0])
+        assert torch.equal(want, got) and torch.equal(gw, gg)
+
+
 def test_registered_operators():
     import depth_estimation_amd.distribution  # noqa: F401
     tests = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
