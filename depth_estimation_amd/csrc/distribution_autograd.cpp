@@ -51,14 +51,24 @@ T* data(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : 
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // (a tensor may stand for its memory's values with the other sign: at::_neg_view)
 Tensor contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
-// the tensor as the kernels read it: its own memory (which may have the classes last), or a copy
-Tensor in_place(const Tensor& t, bool copy) { return copy ? contiguous(t) : t.resolve_neg(); }
-// The same in the backward pass.  What was saved has its own strides there, unless hooks for saved tensors brought it
-// back in another order: then it is put into the one the descriptor tells of.
-Tensor saved_in_place(const Tensor& t, bool copy, at::IntArrayRef strides) {
-  const Tensor x = in_place(t, copy);
-  if (copy || x.strides() == strides) return x;
-  return at::empty_strided(x.sizes(), strides, x.options()).copy_(x);
+// How the kernels read a tensor: in memory order, with the classes (or entries) last in memory, or neither: a copy of it
+enum Layout : int64_t { kInOrder = 0, kLast = 1, kCopy = 2 };
+Tensor in_place(const Tensor& t, int64_t layout) { return layout == kCopy ? contiguous(t) : t.resolve_neg(); }
+bool has_last(const Tensor& t, int64_t dim) {
+  int64_t step = t.size(dim);
+  bool ok = step == 1 || t.stride(dim) == 1;
+  for (int64_t i = t.dim() - 1; i >= 0; --i) {
+    if (i == dim || t.size(i) == 1) continue;
+    ok = ok && t.stride(i) == step;
+    step *= t.size(i);
+  }
+  return ok;
+}
+// The same in the backward pass, where hooks for saved tensors may have brought them back in another order
+Tensor saved_in_place(const Tensor& saved, int64_t layout, int64_t dim) {
+  if (layout != kLast) return contiguous(saved);
+  const Tensor t = saved.resolve_neg();
+  return has_last(t, dim) ? t : t.movedim(dim, -1).contiguous().movedim(-1, dim);
 }
 Tensor workspace(const Tensor& x, int64_t bytes) {
   // allocated for each call: calls on other streams, or captured into other graphs, have their own
@@ -70,12 +80,20 @@ std::vector<int64_t> with(at::IntArrayRef rows, int64_t at, int64_t n) {
   return s;
 }
 
-// The descriptor travels with the node as its bytes: the Python object it came from may be gone by then.
-std::string keep(int64_t address) { return std::string(reinterpret_cast<const char*>(address), sizeof(dw_dist_desc)); }
-dw_dist_desc kept(AutogradContext* ctx) {
-  dw_dist_desc d;
-  std::memcpy(&d, ctx->saved_data["desc"].toStringRef().data(), sizeof d);
-  return d;
+// What the backward pass has to know travels with the node as its bytes: the Python object that the descriptor came
+// from may be gone by then.
+struct Kept {
+  dw_dist_desc desc;
+  int64_t dim, layout, list_layout;
+};
+void keep(AutogradContext* ctx, int64_t desc, int64_t dim, int64_t layout, int64_t list_layout) {
+  const Kept k{*reinterpret_cast<const dw_dist_desc*>(desc), dim, layout, list_layout};
+  ctx->saved_data["call"] = std::string(reinterpret_cast<const char*>(&k), sizeof k);
+}
+Kept kept(AutogradContext* ctx) {
+  Kept k;
+  std::memcpy(&k, ctx->saved_data["call"].toStringRef().data(), sizeof k);
+  return k;
 }
 // The gradients are differentiable once.  Where a pass builds a graph of itself, using that graph is an error.
 Tensor once(Tensor grad) {
@@ -87,18 +105,17 @@ Tensor once(Tensor grad) {
   return (*node)({grad})[0];
 }
 
-// layout: 0 in memory order, 1 classes last, 2 neither (copied)
 struct LogProbs : torch::autograd::Function<LogProbs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& given,
                                int64_t desc, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout,
                                bool train) {
-    const Tensor x = in_place(logits, layout == 2), index_in = given ? *given : Tensor(), index = contiguous(index_in);
+    const Tensor x = in_place(logits, layout), index_in = given ? *given : Tensor(), index = contiguous(index_in);
     const c10::OptionalDeviceGuard guard(x.device());
     const auto f32 = x.options().dtype(at::kFloat).memory_format(std::nullopt);
     Tensor ent = at::empty(rows, f32), lp, stats, top_lp, top_idx;
     if (index.defined()) lp = at::empty(rows, f32);
     if (train) stats = at::empty(with(rows, rows.size(), 3), f32);
-    if (top && layout == 1) {  // the kernels write the list of a row together, too
+    if (top && layout == kLast) {  // the kernels write the list of a row together, too
       top_lp = at::empty(with(rows, rows.size(), top), f32).movedim(-1, dim);
       top_idx = at::empty(with(rows, rows.size(), top), f32.dtype(at::kInt)).movedim(-1, dim);
     } else if (top) {
@@ -121,9 +138,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
       ctx->set_materialize_grads(false);
       if (top) ctx->mark_non_differentiable({top_lp, top_idx});
       ctx->save_for_backward({logits, index_in, stats});
-      ctx->saved_data["desc"] = keep(desc);
-      ctx->saved_data["copy"] = layout == 2;
-      ctx->saved_data["strides"] = x.strides().vec();
+      keep(ctx, desc, dim, layout, kInOrder);
     }
     return out;
   }
@@ -136,10 +151,10 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     variable_list out(9);
     if (!g_lp.defined() && !g_ent.defined()) return out;
     const c10::OptionalDeviceGuard guard(saved[0].device());
-    const Tensor x = saved_in_place(saved[0], ctx->saved_data["copy"].toBool(), ctx->saved_data["strides"].toIntVector());
+    const Kept k = kept(ctx);
+    const Tensor x = saved_in_place(saved[0], k.layout, k.dim);
     Tensor grad = at::empty_like(x);
-    const dw_dist_desc d = kept(ctx);
-    check(lib.log_probs_bwd(&d, data(x), data(index), data<float>(stats), data<float>(g_lp), data<float>(g_ent),
+    check(lib.log_probs_bwd(&k.desc, data(x), data(index), data<float>(stats), data<float>(g_lp), data<float>(g_ent),
                             data(grad), stream_of(x)),
           "dw_log_probs_bwd");
     out[0] = once(grad);
@@ -149,9 +164,10 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
 
 struct Distill : torch::autograd::Function<Distill> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher_in, const Tensor& index_in,
-                        int64_t desc, int64_t nbytes, at::IntArrayRef rows, int64_t layout, bool copy_list, bool train) {
-    const Tensor x = in_place(logits, layout == 2), teacher = in_place(teacher_in, copy_list),
-                 index = in_place(index_in, copy_list);
+                        int64_t desc, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t layout, int64_t list_layout,
+                        bool train) {
+    const Tensor x = in_place(logits, layout), teacher = in_place(teacher_in, list_layout),
+                 index = in_place(index_in, list_layout);
     const c10::OptionalDeviceGuard guard(x.device());
     const auto f32 = x.options().dtype(at::kFloat).memory_format(std::nullopt);
     Tensor loss = at::empty(rows, f32), stats;
@@ -163,29 +179,20 @@ struct Distill : torch::autograd::Function<Distill> {
     if (train) {
       ctx->set_materialize_grads(false);
       ctx->save_for_backward({logits, teacher_in, index_in, stats});
-      ctx->saved_data["desc"] = keep(desc);
-      ctx->saved_data["copy"] = layout == 2;
-      ctx->saved_data["copy_list"] = copy_list;
-      ctx->saved_data["strides"] = x.strides().vec();
-      ctx->saved_data["teacher_strides"] = teacher.strides().vec();
-      ctx->saved_data["index_strides"] = index.strides().vec();
+      keep(ctx, desc, dim, layout, list_layout);
     }
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    variable_list out(9);
+    variable_list out(10);
     if (!g[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
-    const bool copy_list = ctx->saved_data["copy_list"].toBool();
     const c10::OptionalDeviceGuard guard(saved[0].device());
-    auto& data_of = ctx->saved_data;
-    const Tensor x = saved_in_place(saved[0], data_of["copy"].toBool(), data_of["strides"].toIntVector()),
-                 teacher = saved_in_place(saved[1], copy_list, data_of["teacher_strides"].toIntVector()),
-                 index = saved_in_place(saved[2], copy_list, data_of["index_strides"].toIntVector()),
-                 stats = contiguous(saved[3]), up = contiguous(g[0]);
+    const Kept k = kept(ctx);
+    const Tensor x = saved_in_place(saved[0], k.layout, k.dim), teacher = saved_in_place(saved[1], k.list_layout, k.dim),
+                 index = saved_in_place(saved[2], k.list_layout, k.dim), stats = contiguous(saved[3]), up = contiguous(g[0]);
     Tensor grad = at::empty_like(x);
-    const dw_dist_desc d = kept(ctx);
-    check(lib.distill_bwd(&d, data(x), data(teacher), data(index), data<float>(stats), data<float>(up), data(grad),
+    check(lib.distill_bwd(&k.desc, data(x), data(teacher), data(index), data<float>(stats), data<float>(up), data(grad),
                           stream_of(x)),
           "dw_distill_bwd");
     out[0] = once(grad);
@@ -200,9 +207,9 @@ std::vector<Tensor> log_probs(const Tensor& logits, const std::optional<Tensor>&
   return LogProbs::apply(logits, index, desc, nbytes, rows, dim, top, layout, train);
 }
 Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, int64_t desc, int64_t nbytes,
-               at::IntArrayRef rows, int64_t layout, bool copy_list) {
+               at::IntArrayRef rows, int64_t dim, int64_t layout, int64_t list_layout) {
   const bool train = logits.requires_grad() && at::GradMode::is_enabled();
-  return Distill::apply(logits, teacher, index, desc, nbytes, rows, layout, copy_list, train);
+  return Distill::apply(logits, teacher, index, desc, nbytes, rows, dim, layout, list_layout, train);
 }
 }  // namespace
 
@@ -210,6 +217,6 @@ TORCH_LIBRARY_FRAGMENT(depthwarp, m) {
   m.def("_bind_distribution(int strerror, int lp_fwd, int lp_bwd, int ds_fwd, int ds_bwd) -> ()", &bind);
   m.def("_log_probs_eager(Tensor logits, Tensor? index, int desc, int nbytes, int[] rows, int dim, int top, "
         "int layout) -> Tensor[]", &log_probs);
-  m.def("_distill_eager(Tensor logits, Tensor teacher, Tensor index, int desc, int nbytes, int[] rows, int layout, "
-        "bool copy_list) -> Tensor", &distill);
+  m.def("_distill_eager(Tensor logits, Tensor teacher, Tensor index, int desc, int nbytes, int[] rows, int dim, "
+        "int layout, int list_layout) -> Tensor", &distill);
 }

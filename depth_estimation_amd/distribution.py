@@ -87,7 +87,7 @@ class _Plan(NamedTuple):
     address: int       # the same for C++
     nbytes: int        # workspace
     top: int = 0
-    copy_list: bool = False   # distillation: the teacher's tensors have no common order
+    list_layout: int = 0      # distillation: the same of the teacher's tensors (_COPY where they have no common order)
 
 
 _IN_PLACE, _LAST, _COPY = 0, 1, 2
@@ -343,12 +343,12 @@ def _make_ds_plan(shape, stride, dtype, t_shape, t_stride, t_dtype, i_shape, i_s
     k, inner = t_shape[dim], math.prod(t_shape[dim + 1:])
     # the list's element strides along outer, entry, inner: its tensors as they are if they share an order
     t_layout, i_layout = _layout(t_shape, t_stride, dim), _layout(i_shape, i_stride, dim)
-    copy = t_layout != i_layout or t_layout == _COPY
-    strides = (k * inner, 1, k) if not copy and t_layout == _LAST else (k * inner, inner, 1)
+    list_layout = t_layout if t_layout == i_layout else _COPY
+    strides = (k * inner, 1, k) if list_layout == _LAST else (k * inner, inner, 1)
     layout = _layout(shape, stride, dim)
     flags = _INDEX_FLAGS[i_dtype] | _TEACHER_FLAGS[t_dtype] | (_lib.DW_DIST_RENORMALISE if renormalise else 0)
     ref, address, nbytes = _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k, flags, strides)
-    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, address, nbytes, copy_list=copy)
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, address, nbytes, list_layout=list_layout)
 
 
 _ds_plan = functools.lru_cache(maxsize=512)(_make_ds_plan)
@@ -361,7 +361,7 @@ def _ds_plan_of(logits: Tensor, teacher: Tensor, index: Tensor, dim: int, scale:
 
 def _ds_forward(logits: Tensor, teacher: Tensor, index: Tensor, plan: _Plan):
     x = logits.contiguous() if plan.layout == _COPY else logits
-    if plan.copy_list:
+    if plan.list_layout == _COPY:
         teacher, index = teacher.contiguous(), index.contiguous()
     loss = torch.empty(plan.rows, dtype=torch.float32, device=x.device)
     stats = torch.empty(plan.rows + (4,), dtype=torch.float32, device=x.device)
@@ -373,7 +373,7 @@ def _ds_forward(logits: Tensor, teacher: Tensor, index: Tensor, plan: _Plan):
 
 def _ds_backward(logits: Tensor, teacher: Tensor, index: Tensor, stats: Tensor, g_loss: Tensor, plan: _Plan) -> Tensor:
     x = logits.contiguous() if plan.layout == _COPY else logits
-    if plan.copy_list:
+    if plan.list_layout == _COPY:
         teacher, index = teacher.contiguous(), index.contiguous()
     grad = torch.empty_like(x)
     stats, g_loss = stats.contiguous(), g_loss.contiguous()
@@ -447,4 +447,5 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
                         teacher_index.dtype, dim, scale)
         return _distill_op(logits, teacher, teacher_index, dim, scale, renormalise)[0]
     plan = _ds_plan_of(logits, teacher, teacher_index, dim, scale, renormalise)
-    return _eager()[1](logits, teacher, teacher_index, plan.address, plan.nbytes, plan.rows, plan.layout, plan.copy_list)
+    return _eager()[1](logits, teacher, teacher_index, plan.address, plan.nbytes, plan.rows, plan.dim, plan.layout,
+                       plan.list_layout)
