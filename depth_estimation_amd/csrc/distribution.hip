@@ -1542,8 +1542,9 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
   const int given = index && p.chunks == 1 ? valid_index(load_index(index, row, p.flags), p.V) : -1;
   const typename T::S x_given = given >= 0 ? xr[given] : typename T::S(0);
   Acc a = acc_empty(z);
-  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](const float (&v)[32], int, int, bool) {
-    const float top = z.best_of(v);
+  walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](const float (&v)[32], int base, int, bool) {
+    const bool mine = base < end;  // (a row's last step may leave waves without classes: 1023 x 50001 f16 33 -> 32 us)
+    const float top = mine ? z.best_of(v) : z.far();
     if constexpr (TOP) {
       so_far = vmax(so_far, top * z.sign);
       cell_best[cell * NT + threadIdx.x] = so_far;
@@ -1553,7 +1554,7 @@ __global__ __launch_bounds__(NT, 4) void lp_row_fwd(Prob p, const typename T::S*
         so_far = -kInf;
       }
     }
-    absorb<true>(a, v, 32, top, z);
+    if (mine) absorb<true>(a, v, 32, top, z);
   });
   const float my_max = a.m * z.sign;
   a = acc_block<NT>(a, z, red);
@@ -1763,6 +1764,7 @@ __global__ __launch_bounds__(NT, 4) void ds_row_fwd(Prob p, const typename T::S*
   if (__any(e.idx >= 0)) {  // the same in every wave
     walk_row<T, NT>(xr, begin, end, lane, wave, z.far(), [&](float (&v)[32], int base, int, bool full) {
       (void)full;
+      if (base >= end) return;
       patch_tile<T>(v, base, lane, e.idx, z.far());
       absorb<false>(a, v, 32, z.best_of(v), z);
     });
