@@ -438,6 +438,7 @@ __device__ __forceinline__ void load_teachers(const Prob& p, const void* teacher
 }
 
 // ---- tile kernels: where the 64 rows of a block are, and how their classes come in -----------------
+enum Layout { kPlanes, kTurned, kFlat };
 struct Place {
   int64_t row;    // this lane's row (planes: the last pixel again behind the end)
   int64_t o, i;   // its outer and inner index
@@ -511,14 +512,14 @@ constexpr int kRowBytes = kSegBytes + 16;      // LDS distance of two rows: spre
 constexpr int kStageBytes = 64 * kRowBytes;
 
 // classes a wave takes at a time
-template <class T, bool LAST>
-constexpr int stage_classes() { return LAST ? kSegBytes / (int)sizeof(typename T::S) : 32; }
+template <class T, int L>
+constexpr int stage_classes() { return L == kTurned ? kSegBytes / (int)sizeof(typename T::S) : 32; }
 
 // The next stage on its way: loads are issued a stage ahead, while the one before is worked on.
-template <class T, bool LAST>
+template <class T, int L>
 struct Feed;
 template <class T>
-struct Feed<T, true> {  // 64 row segments of classes [c0, c0 + n), 8 lanes a row
+struct Feed<T, kTurned> {  // 64 row segments of classes [c0, c0 + n), 8 lanes a row
   static constexpr int PER = kSegBytes / 16;
   Vec<T> v[PER];
   __device__ __forceinline__ void issue(const typename T::S* x, const Prob& p, const Place& q, int c0, int n) {
@@ -553,7 +554,7 @@ struct Feed<T, true> {  // 64 row segments of classes [c0, c0 + n), 8 lanes a ro
   }
 };
 template <class T>
-struct Feed<T, false> {  // 32 planes from class c0 on; the planes behind the n-th repeat it
+struct Feed<T, kPlanes> {  // 32 planes from class c0 on; the planes behind the n-th repeat it
   typename T::S v[32];
   __device__ __forceinline__ void issue(const typename T::S* x, const Prob& p, const Place& q, int c0, int n) {
     using S = typename T::S;
@@ -579,6 +580,99 @@ struct Feed<T, false> {  // 32 planes from class c0 on; the planes behind the n-
   __device__ __forceinline__ void take(float (&f)[32]) const {
 #pragma unroll
     for (int u = 0; u < 32; ++u) f[u] = T::up(v[u]);
+  }
+};
+template <class T>
+struct Feed<T, kFlat> {  // all there already
+  __device__ __forceinline__ void issue(const typename T::S*, const Prob&, const Place&, int, int) {}
+};
+
+// Rows of a flat tile: the 64 rows' bytes as they lie in memory, so that whole lines are read and written whatever the
+// rows' length; where rows are whole 16-byte pieces, each with 16 bytes behind it, which spreads them over the banks.
+constexpr int kFlatSlack = 128;  // behind the last row: a lane reads 32 classes at a time
+__host__ __device__ constexpr bool flat_padded(int row) { return row % 16 == 0 && row > 16; }
+__host__ __device__ constexpr int flat_row(int row) { return row + (flat_padded(row) ? 16 : 0); }
+__host__ __device__ constexpr int flat_bytes(int row) { return (64 * flat_row(row) + kFlatSlack + 15) / 16 * 16; }
+template <class T>
+struct FlatTile {
+  using S = typename T::S;
+  char* lds;
+  int row, step, threads;  // bytes of a row in memory, in LDS
+  unsigned pieces, inv;    // 16-byte pieces of the tile; 2^32 / pieces of a row, rounded up: exact below 2^16 pieces
+  __device__ __forceinline__ FlatTile(const Prob& p, char* smem)
+      : lds(smem), row(p.V * (int)sizeof(S)), step(flat_row(row)), threads(blockDim.x), pieces(4u * row),
+        inv(flat_padded(row) ? 0xffffffffu / (unsigned)(row / 16) + 1 : 0) {}
+  __device__ __forceinline__ u32x4* at(unsigned piece) const {
+    return (u32x4*)(lds + 16 * (piece + (flat_padded(row) ? __umulhi(piece, inv) : 0)));
+  }
+  __device__ __forceinline__ S* lane_row(int lane) const { return (S*)(lds + lane * step); }
+  // the whole block; ends with a barrier
+  __device__ __forceinline__ void in(const S* x, const Prob& p, const Place& q) const {
+    const S* base = x + q.first * p.V;
+    for (unsigned c0 = threadIdx.x; c0 < pieces; c0 += 8 * threads) {
+      Vec<T> w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned c = c0 + i * threads;
+        if (c < pieces) w[i] = load_vec<T>(base, c * 16);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned c = c0 + i * threads;
+        if (c < pieces) *at(c) = w[i].d;
+      }
+    }
+    __syncthreads();
+  }
+  // begins with a barrier
+  __device__ __forceinline__ void out(S* g, const Prob& p, const Place& q) const {
+    __syncthreads();
+    S* base = g + q.first * p.V;
+    const unsigned skip = (unsigned)(q.skip * row);
+    for (unsigned c = threadIdx.x; c < pieces; c += threads) {
+      const Vec<T> w{*at(c)};
+      if (c * 16 >= skip) {
+        store_vec<T>(base, c * 16, w);
+      } else if (c * 16 + 16 > skip) {
+        const S* e = (const S*)at(c);
+        for (unsigned b = skip; b < c * 16 + 16; b += sizeof(S)) at_byte(base, b) = e[(b - c * 16) / sizeof(S)];
+      }
+    }
+  }
+  // 32 classes from c on; what lies behind the row's last is anything
+  __device__ __forceinline__ void read(int lane, int c, float (&v)[32]) const {
+    const S* r = lane_row(lane) + c;
+    if (flat_padded(row)) {
+#pragma unroll
+      for (int u = 0; u < 32 / T::VEC; ++u) {
+        const Vec<T> w{((const u32x4*)r)[u]};
+#pragma unroll
+        for (int e = 0; e < T::VEC; ++e) v[u * T::VEC + e] = w.get(e);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 32; ++u) v[u] = T::up(r[u]);
+    }
+  }
+  // n of them (whole pieces, where rows are)
+  __device__ __forceinline__ void write(int lane, int c, int n, const float (&v)[32]) const {
+    S* r = lane_row(lane) + c;
+    if (flat_padded(row)) {
+#pragma unroll
+      for (int u = 0; u < 32 / T::VEC; ++u) {
+        Vec<T> w;
+        w.put(v + u * T::VEC);
+        if (u * T::VEC < n) ((u32x4*)r)[u] = w.d;
+      }
+    } else if (n == 32) {
+#pragma unroll
+      for (int u = 0; u < 32; ++u) r[u] = T::down(v[u]);
+    } else {
+      n = (int)fresh_uniform(n);
+#pragma unroll
+      for (int u = 0; u < 32; ++u)
+        if (u < n) r[u] = T::down(v[u]);
+    }
   }
 };
 template <class T>
@@ -670,30 +764,33 @@ __device__ __forceinline__ void settle(float (&v)[32], float far, int n) {
 // Turning rows and keeping their lists takes up to 180 registers: those blocks have at most 8 waves, so that they get
 // them (192 classes of 2 x 192 x 320 pixels f32: the top 8 in 31 us, 41 with 128 registers; bf16 the same either way).
 constexpr int list_waves(bool last, bool list) { return last && list ? 8 : 16; }
-template <class T, bool LAST, class P, int K>
-__global__ __launch_bounds__(64 * list_waves(LAST, K > 0))
+template <class T, int L, class P, int K>
+__global__ __launch_bounds__(64 * list_waves(L != kPlanes, K > 0))
 void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
                             float* __restrict__ log_prob, float* __restrict__ entropy, float* __restrict__ top_lp,
                             int32_t* __restrict__ top_idx, Stats3* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
+  constexpr bool LAST = L != kPlanes;
   const Place q = place<LAST>(p, blockIdx.x);
   const int nw = blockDim.x >> 6;
-  char* stage = smem + q.wave * kStageBytes;                       // LAST only
-  char* joint = smem + (LAST ? nw * kStageBytes : 0);
+  char* stage = smem + q.wave * kStageBytes;                       // kTurned only
+  const FlatTile<T> tile(p, smem);                                 // kFlat only
+  char* joint = smem + (L == kTurned ? nw * kStageBytes : L == kFlat ? flat_bytes(tile.row) : 0);
   float* red = (float*)joint;                                      // [3][nw][64]
   using Key = typename P::Key;
   Key* keys = (Key*)(joint + 3 * nw * 64 * sizeof(float));         // [nw][K][64]
-  constexpr int CH = stage_classes<T, LAST>();
+  constexpr int CH = stage_classes<T, L>();
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
 
   // the given class, on its way while the classes are read
   const int64_t given_raw = index ? load_index(index, q.row, p.flags) : -1;
-  Feed<T, LAST> feed;
+  Feed<T, L> feed;
   if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
   const int given = valid_index(given_raw, p.V);
   const typename T::S x_given = given >= 0 ? x[element<LAST>(p, q, given)] : typename T::S(0);
 
+  if constexpr (L == kFlat) tile.in(x, p, q);
   Acc a = acc_empty(z);
   Key limit = P::kNone;
   float ln_s = 0.f, base = 0.f;
@@ -705,16 +802,17 @@ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __rest
     for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
       const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
       float v[32];
-      if constexpr (LAST) {
+      if constexpr (L == kTurned) {
         wave_sync();
         feed.to_lds(q, stage);
         wave_sync();
-      } else {
+      } else if constexpr (L == kPlanes) {
         feed.take(v);
       }
       if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
       for (int h = 0; h < n; h += 32) {
-        if (LAST) stage_read<T>(stage, q.lane, h, v);
+        if constexpr (L == kTurned) stage_read<T>(stage, q.lane, h, v);
+        if constexpr (L == kFlat) tile.read(q.lane, c0 + h, v);
         settle(v, z.far(), n - h);
         if (done == 0) absorb<true>(a, v, n - h, z.best_of(v), z);
         if constexpr (K > 0) {
@@ -820,33 +918,37 @@ __device__ __forceinline__ float lp_grad(const LpCoef& r, float v, float c, floa
 // The rows' sums come from the forward pass, so this is one read and one write: dx_j = e_j (k0 + k1 t_j), and the
 // given class on top.  12 x 64 x 96 x 320 bf16 (94 MB): 20.0 us, 4.7 TB/s, what a copy takes.  4 x 193 x 96 x 320 f16, classes
 // last (95 MB): 28 us; rows of 386 bytes begin inside the memory's lines, and 66 MB are written for 47.
-template <class T, bool LAST, bool ENT>
+template <class T, int L, bool ENT>
 __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
                             const Stats3* __restrict__ stats, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
                             typename T::S* __restrict__ g) {
   extern __shared__ __align__(16) char smem[];
+  constexpr bool LAST = L != kPlanes;
   const Place q = place<LAST>(p, block_from_end());
   char* stage = smem + q.wave * kStageBytes;
+  const FlatTile<T> tile(p, smem);  // kFlat only
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
-  constexpr int CH = stage_classes<T, LAST>();
-  Feed<T, LAST> feed;
+  constexpr int CH = stage_classes<T, L>();
+  Feed<T, L> feed;
   if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
   const LpCoef r = lp_coef<ENT>(p, q.row, index, stats, g_lp, g_ent);
   const bool any_dead = __any(r.dead);
+  if constexpr (L == kFlat) tile.in(x, p, q);
   for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
     const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
     float v[32];
-    if constexpr (LAST) {
+    if constexpr (L == kTurned) {
       wave_sync();
       feed.to_lds(q, stage);
       wave_sync();
-    } else {
+    } else if constexpr (L == kPlanes) {
       feed.take(v);
     }
     if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
     for (int h = 0; h < n; h += 32) {
-      if (LAST) stage_read<T>(stage, q.lane, h, v);
+      if constexpr (L == kTurned) stage_read<T>(stage, q.lane, h, v);
+      if constexpr (L == kFlat) tile.read(q.lane, c0 + h, v);
       settle(v, z.far(), n - h);
       const int rel = r.target - c0 - h;
 #pragma unroll
@@ -858,8 +960,10 @@ __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
 #pragma unroll
         for (int u = 0; u < 32; ++u) v[u] = r.dead ? 0.f : v[u];
       }
-      if (LAST) {
+      if constexpr (L == kTurned) {
         stage_write<T>(stage, q.lane, h, v);
+      } else if constexpr (L == kFlat) {
+        tile.write(q.lane, c0, n, v);
       } else {
         typename T::S raw[32];
 #pragma unroll
@@ -867,11 +971,12 @@ __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
         planes_out<T>(g, p, q, c0, n, raw);
       }
     }
-    if (LAST) {
+    if constexpr (L == kTurned) {
       wave_sync();
       stage_out<T>(g, p, q, c0, n, stage);
     }
   }
+  if constexpr (L == kFlat) tile.out(g, p, q);
 }
 
 // ---- distillation: what both families share ---------------------------------------------------------
@@ -898,19 +1003,35 @@ __device__ __forceinline__ float4 distill_stats(const RowSums& r, float c, float
 }
 
 // Column of this lane's row inside the stage: planes [class][64], or the row's own bytes.  What a
-// lane does for a listed class that is not in the stage goes to a place of its own behind the column.
-template <class T, bool LAST>
+// lane does for a listed class that is not in the stage goes to a place of its own.
+template <class T, int L>
 struct Column {
   using S = typename T::S;
   using M = T;
-  static constexpr int kNowhere = LAST ? kSegBytes / (int)sizeof(S) : 32;
-  char* lds;
-  int lane;
-  __device__ __forceinline__ S* at(int u) const {
-    return LAST ? (S*)(lds + lane * kRowBytes) + u : (S*)lds + u * 64 + lane;
+  S *first, *nowhere;
+  __device__ __forceinline__ Column(char* stage, const FlatTile<T>& tile, int c_lo, int wave, int lane) {
+    if (L == kPlanes) {
+      first = (S*)stage + lane;
+      nowhere = first + 32 * 64;
+    } else if (L == kTurned) {
+      first = (S*)(stage + lane * kRowBytes);
+      nowhere = first + kSegBytes / (int)sizeof(S);
+    } else {
+      first = tile.lane_row(lane) + c_lo;
+      nowhere = (S*)(tile.lds + flat_bytes(tile.row)) + wave * 64 + lane;
+    }
   }
+  __device__ __forceinline__ S* at(int u) const { return first + (L == kPlanes ? u * 64 : u); }
+  __device__ __forceinline__ S* at(bool hit, int u) const { return hit ? at(u) : nowhere; }
 };
-constexpr int distill_stage_bytes(bool last, int esize) { return last ? kStageBytes : 33 * 64 * esize; }
+// LDS of the classes: a stage a wave, or the flat tile of the block
+__host__ __device__ inline size_t distill_stages(int layout, int nw, int V, int esize) {
+  if (layout == kFlat) return flat_bytes(V * esize) + (size_t)nw * 64 * 4;
+  return nw * (size_t)(layout == kTurned ? kStageBytes : 33 * 64 * esize);
+}
+__host__ __device__ constexpr int distill_stage_bytes(int layout, int esize) {
+  return layout == kTurned ? kStageBytes : layout == kPlanes ? 33 * 64 * esize : 0;
+}
 constexpr int kGroup = 8;  // entries handled at once: their LDS accesses overlap
 __host__ __device__ constexpr int padded(int k) { return (k + kGroup - 1) / kGroup * kGroup; }
 // LDS of a block besides the stages: columns of 64 lanes, of list entries and of the waves' sums
@@ -964,7 +1085,7 @@ __device__ __forceinline__ void take_listed(const C& col, const int* idx, int K,
     for (int i = 0; i < kGroup; ++i) {
       const int rel = idx[(e0 + i) * 64] - c0;
       hit[i] = (unsigned)rel < (unsigned)n;
-      typename C::S* at = col.at(hit[i] ? rel : C::kNowhere);
+      typename C::S* at = col.at(hit[i], rel);
       old[i] = C::M::up(*at);
       *at = C::M::down(far);
     }
@@ -980,23 +1101,25 @@ __device__ __forceinline__ void take_listed(const C& col, const int* idx, int K,
 // entry is looked up in every stage, eight at a time, which is what long lists cost (192 classes of 2 x 192 x 640
 // pixels bf16: 36 us with 8 entries, 49 with 16).  4 x 256 x 192 x 640 bf16, 8 entries (252 + 31 MB): 68 us, 4.2 TB/s;
 // 12 x 128 x 96 x 320 f16, classes last (94 + 25 MB): 32 us, 3.7 TB/s; 1 x 64 x 24 x 80: 6.6 us, the launch's latency.
-template <class T, bool LAST>
+template <class T, int L>
 __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ teacher,
                             const void* __restrict__ index, float* __restrict__ loss, float4* __restrict__ stats) {
   extern __shared__ __align__(16) char smem[];
+  constexpr bool LAST = L != kPlanes;
   const Place q = place<LAST>(p, blockIdx.x);
   const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
-  char* stage = smem + q.wave * distill_stage_bytes(LAST, sizeof(typename T::S));
-  char* rest = smem + nw * distill_stage_bytes(LAST, sizeof(typename T::S));
+  char* stage = smem + q.wave * distill_stage_bytes(L, sizeof(typename T::S));
+  char* rest = smem + distill_stages(L, nw, p.V, sizeof(typename T::S));
   int* idx = (int*)rest + q.lane;                            // [KP][64]
   float* xs = (float*)rest + KP * 64 + q.lane;               // [KP + 1][64]: the listed classes' values
   float* red = (float*)rest + (2 * KP + 1) * 64 + q.lane;    // [2][nw][64], where there are several waves
-  const Column<T, LAST> col{stage, q.lane};
-  constexpr int CH = stage_classes<T, LAST>();
+  constexpr int CH = stage_classes<T, L>();
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
+  const FlatTile<T> tile(p, smem);  // kFlat only
+  const Column<T, L> col(stage, tile, c_lo, q.wave, q.lane);
   const int64_t t0 = q.o * p.es[0] + q.i * p.es[2];
-  Feed<T, LAST> feed;
+  Feed<T, L> feed;
   if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
 
   for (int e0 = q.wave * kGroup; e0 < KP; e0 += nw * kGroup) {
@@ -1010,7 +1133,8 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   }
   float first[kGroup];  // the teacher's first values: in most lists all of them
   load_teachers(p, teacher, t0, 0, first);
-  __syncthreads();
+  if constexpr (L == kFlat) tile.in(x, p, q);  // with the barrier
+  else __syncthreads();
   bool alive = false;
   for (int e0 = 0; e0 < KP; e0 += kGroup) {
     int i8[kGroup];
@@ -1020,23 +1144,31 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   }
   Acc a = acc_empty(z);
   if (__any(alive)) {  // the same in every wave of the block
+    const auto take = [&](int c0, int n) {
+      take_listed(col, idx, K, c0, n, z.far(), [&](int e, bool hit, float old) { xs[(hit ? e : KP) * 64] = old; });
+      wave_sync();
+    };
+    if constexpr (L == kFlat) take(c_lo, max(c_hi - c_lo, 0));
     for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
       const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
       float v[32];
-      wave_sync();
-      if constexpr (LAST) {
-        feed.to_lds(q, stage);
-      } else {
+      if constexpr (L != kFlat) {
+        wave_sync();
+        if constexpr (L == kTurned) {
+          feed.to_lds(q, stage);
+        } else {
 #pragma unroll
-        for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
+          for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
+        }
+        if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
+        wave_sync();
+        take(c0, n);
       }
-      if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
-      wave_sync();
-      take_listed(col, idx, K, c0, n, z.far(), [&](int e, bool hit, float old) { xs[(hit ? e : KP) * 64] = old; });
-      wave_sync();
       for (int h = 0; h < n; h += 32) {
-        if (LAST) {
+        if constexpr (L == kTurned) {
           stage_read<T>(stage, q.lane, h, v);
+        } else if constexpr (L == kFlat) {
+          tile.read(q.lane, c0 + h, v);
         } else {
 #pragma unroll
           for (int u = 0; u < 32; ++u) v[u] = T::up(*col.at(u));
@@ -1108,30 +1240,31 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
 // The stage becomes gradients in place: the listed classes' values are taken out and their gradients worked out in
 // the list's columns, the others' are e_j times one factor, and the listed ones are put back last, a class that is
 // listed twice with the sum.  4 x 256 x 192 x 640 bf16, 8 entries (503 + 31 MB): 112 us, 4.8 TB/s, what a copy takes.
-template <class T, bool LAST>
+template <class T, int L>
 __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ teacher,
                             const void* __restrict__ index, const float4* __restrict__ stats,
                             const float* __restrict__ g_loss, typename T::S* __restrict__ g) {
   extern __shared__ __align__(16) char smem[];
+  constexpr bool LAST = L != kPlanes;
   const Place q = place<LAST>(p, block_from_end());
   const int nw = blockDim.x >> 6, K = p.k, KP = padded(K);
-  char* stage = smem + q.wave * distill_stage_bytes(LAST, sizeof(typename T::S));
-  char* rest = smem + nw * distill_stage_bytes(LAST, sizeof(typename T::S));
+  char* stage = smem + q.wave * distill_stage_bytes(L, sizeof(typename T::S));
+  char* rest = smem + distill_stages(L, nw, p.V, sizeof(typename T::S));
   int* idx = (int*)rest + q.lane;                    // [KP][64]
   float* gq = (float*)rest + KP * 64 + q.lane;       // [KP][64]: upstream gradient * scale * teacher's probability
   float* gv = (float*)rest + 2 * KP * 64 + q.lane;   // [KP + 1][64]: the listed classes' gradients
-  const Column<T, LAST> col{stage, q.lane};
-  using C = Column<T, LAST>;
-  constexpr int CH = stage_classes<T, LAST>();
+  constexpr int CH = stage_classes<T, L>();
   const Side z = side(p);
   const bool renorm = p.flags & kRenorm;
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
+  const FlatTile<T> tile(p, smem);  // kFlat only
+  const Column<T, L> col(stage, tile, c_lo, q.wave, q.lane);
   const int64_t t0 = q.o * p.es[0] + q.i * p.es[2];
   const float4 st = stats[q.row];
   const float up = g_loss[q.row];
   const bool dead = up == 0.f || st.w == 0.f;
   const float gs = up * p.scale, rest_f = gs * st.y, member_f = gs * st.w;
-  Feed<T, LAST> feed;
+  Feed<T, L> feed;
   if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
 
   for (int e0 = q.wave * kGroup; e0 < KP; e0 += nw * kGroup) {
@@ -1155,22 +1288,11 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
       for (int i = 0; i < kGroup; ++i) gq[(e0 + i) * 64] = gs * exp_(gq[(e0 + i) * 64] - shift);
     }
   }
-  __syncthreads();
+  if constexpr (L == kFlat) tile.in(x, p, q);  // with the barrier
+  else __syncthreads();
   const bool any_dead = __any(dead);
-  for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
-    const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
-    float v[32];
-    wave_sync();
-    if constexpr (LAST) {
-      feed.to_lds(q, stage);
-    } else {
-      feed.take(v);
-#pragma unroll
-      for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
-    }
-    if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
-    wave_sync();
-    // p Q - q of the listed classes; one that is listed again goes on from its earlier entry's value
+  // p Q - q of the listed classes; one that is listed again goes on from its earlier entry's value
+  const auto take = [&](int c0, int n) {
     take_listed(col, idx, K, c0, n, z.far(), [&](int e, bool hit, float old) {
       float f = fmaf(exp2_((old - st.z) * p.c), member_f, -gq[e * 64]);
       if (hit && old == z.far()) {
@@ -1180,8 +1302,39 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
       gv[(hit ? e : KP) * 64] = f;
     });
     wave_sync();
+  };
+  const auto put = [&](int c0, int n) {
+    wave_sync();
+    for (int e0 = 0; e0 < K; e0 += kGroup) {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const int rel = idx[(e0 + i) * 64] - c0;
+        *col.at((unsigned)rel < (unsigned)n, rel) = T::down(gv[(e0 + i) * 64]);
+      }
+    }
+    wave_sync();
+  };
+  const int mine = max(c_hi - c_lo, 0);
+  if constexpr (L == kFlat) take(c_lo, mine);
+  for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
+    const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
+    float v[32];
+    if constexpr (L != kFlat) {
+      wave_sync();
+      if constexpr (L == kTurned) {
+        feed.to_lds(q, stage);
+      } else {
+        feed.take(v);
+#pragma unroll
+        for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
+      }
+      if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
+      wave_sync();
+      take(c0, n);
+    }
     for (int h = 0; h < n; h += 32) {
-      if (LAST) stage_read<T>(stage, q.lane, h, v);
+      if constexpr (L == kTurned) stage_read<T>(stage, q.lane, h, v);
+      if constexpr (L == kFlat) tile.read(q.lane, c0 + h, v);
       settle(v, z.far(), n - h);
 #pragma unroll
       for (int u = 0; u < 32; ++u) {
@@ -1192,30 +1345,28 @@ __global__ void ds_tile_bwd(Prob p, const typename T::S* __restrict__ x, const v
 #pragma unroll
         for (int u = 0; u < 32; ++u) v[u] = dead ? 0.f : v[u];
       }
-      if (LAST) {
+      if constexpr (L == kTurned) {
         stage_write<T>(stage, q.lane, h, v);
+      } else if constexpr (L == kFlat) {
+        tile.write(q.lane, c0, n, v);
       } else {
 #pragma unroll
         for (int u = 0; u < 32; ++u) *col.at(u) = T::down(v[u]);
       }
     }
-    wave_sync();
-    for (int e0 = 0; e0 < K; e0 += kGroup) {
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        const int rel = idx[(e0 + i) * 64] - c0;
-        *col.at((unsigned)rel < (unsigned)n ? rel : C::kNowhere) = C::M::down(gv[(e0 + i) * 64]);
-      }
-    }
-    wave_sync();
-    if (LAST) {
+    if constexpr (L != kFlat) put(c0, n);
+    if constexpr (L == kTurned) {
       stage_out<T>(g, p, q, c0, n, stage);
-    } else {
+    } else if constexpr (L == kPlanes) {
       typename T::S raw[32];
 #pragma unroll
       for (int u = 0; u < 32; ++u) raw[u] = *col.at(u);
       planes_out<T>(g, p, q, c0, n, raw);
     }
+  }
+  if constexpr (L == kFlat) {
+    put(c_lo, mine);
+    tile.out(g, p, q);
   }
 }
 
@@ -1854,10 +2005,12 @@ constexpr int kWantWaves = 2048;           // 8 a compute unit: enough loads in 
 // instead of 96), turned rows never (193 classes f16: 45 instead of 29).
 constexpr int64_t kPastBytes = (int64_t)128 << 20;
 constexpr size_t kLdsBudget = 152 * 1024;  // of a block, of the compute unit's 160 KB
+constexpr int kMostFlat = 64 * 1024;       // of a flat tile
 
 struct Plan {
   Prob p;
   bool tile, last;
+  int layout;    // tile: kPlanes, kTurned, kFlat
   int nw;        // tile: waves a block
   int nt;        // row: threads a block
   unsigned grid;
@@ -1900,28 +2053,32 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
   const int esize = d->dtype == DW_DTYPE_F32 ? 4 : 2;
   P.tile = !P.last || (p.V <= 2048 && tiles * 4 >= kWantWaves / 4);
   if (P.tile) {
-    const int stage = P.last ? kSegBytes / esize : 32;
+    const int row = p.V * esize;
+    P.layout = !P.last ? kPlanes : row % kSegBytes != 0 && flat_bytes(row) <= kMostFlat ? kFlat : kTurned;
+    const int stage = P.layout == kTurned ? kSegBytes / esize : 32;
     const int stages = (p.V + stage - 1) / stage;
     const int most = distill || backward ? 16 : list_waves(P.last, p.k > 0);
     P.nw = 1;
     while (P.nw < most && tiles * P.nw < kWantWaves && P.nw * 2 <= stages) P.nw *= 2;
+    if (P.layout == kFlat)
+      while (P.nw < 4 && P.nw * 2 <= stages) P.nw *= 2;
+    const auto lds = [&](int nw) {
+      return distill ? distill_stages(P.layout, nw, p.V, esize) + distill_lds(nw, p.k, false)
+                     : (P.layout == kTurned ? (size_t)nw * kStageBytes : P.layout == kFlat ? flat_bytes(row) : 0) +
+                           (size_t)nw * 64 * (12 + 8 * 16);
+    };
     if (distill) {
       // The list is the block's, a stage each wave's, so more waves a block are more waves in the LDS of a compute
       // unit.  The forward pass ends with one wave's work: it takes that only where fewer than 8 waves would fit
       // (channels_last f16, 128 classes, 8 entries: 35 us with one wave a block, 39 with two; bf16 planes, 256
       // classes, 64 entries: 210 and 116 with one and 8).  The backward pass does not (bf16 planes, 256 classes,
       // 8 entries: 118 us with one, 105 with two).
-      const auto waves = [&](int nw) {
-        const size_t lds = nw * (size_t)distill_stage_bytes(P.last, esize) + distill_lds(nw, p.k, false);
-        return lds > kLdsBudget ? 0 : (int)(kLdsBudget / lds) * nw;
-      };
+      const auto waves = [&](int nw) { return lds(nw) > kLdsBudget ? 0 : (int)(kLdsBudget / lds(nw)) * nw; };
       for (int nw = P.nw * 2; nw <= 16 && nw <= stages; nw *= 2)
         if (waves(nw) > waves(P.nw) && waves(P.nw) < (backward ? 16 : 8)) P.nw = nw;
-      while (P.nw > 1 && waves(P.nw) == 0) P.nw /= 2;
-    } else {
-      while (P.nw > 1 && P.nw * (kStageBytes + 64 * (12 + 8 * 16)) > (int)kLdsBudget) P.nw /= 2;
     }
-    p.cpw = (stages + P.nw - 1) / P.nw * stage;
+    while (P.nw > 1 && lds(P.nw) > kLdsBudget) P.nw /= 2;
+    p.cpw = P.layout == kFlat ? (p.V + 8 * P.nw - 1) / (8 * P.nw) * 8 : (stages + P.nw - 1) / P.nw * stage;
     if (tiles > kMaxThreads / (P.nw * 64)) return DW_ERR_SHAPE;
     P.grid = (unsigned)tiles;
     return DW_OK;
@@ -1965,38 +2122,42 @@ int allow_lds(F f, size_t bytes) {  // more than 64 KB of LDS has to be asked fo
              ? DW_OK : DW_ERR_LAUNCH;
 }
 
-template <class T, bool LAST, class KP, int K>
+template <class T, int L, class KP, int K>
 int lp_tile_launch(const Plan& P, const void* x, const void* index, const LpOut& o, hipStream_t st) {
-  const size_t lds = (LAST ? P.nw * kStageBytes : 0) + (P.nw > 1 ? P.nw * 64 * (12 + sizeof(typename KP::Key) * K) : 0);
-  if (int rc = allow_lds(lp_tile_fwd<T, LAST, KP, K>, lds)) return rc;
-  lp_tile_fwd<T, LAST, KP, K><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const typename T::S*)x, index, o.log_prob, o.entropy,
+  const size_t lds = (L == kTurned ? P.nw * kStageBytes : L == kFlat ? flat_bytes(P.p.V * (int)sizeof(typename T::S)) : 0) +
+                     (P.nw > 1 ? P.nw * 64 * (12 + sizeof(typename KP::Key) * K) : 0);
+  if (int rc = allow_lds(lp_tile_fwd<T, L, KP, K>, lds)) return rc;
+  lp_tile_fwd<T, L, KP, K><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const typename T::S*)x, index, o.log_prob, o.entropy,
                                                               o.top_lp, o.top_idx, o.stats);
   return launched();
 }
 // the list in registers: the smallest that holds all of it, or the largest there is, several times
-template <class T, bool LAST>
+template <class T, int L>
 int lp_tile(const Plan& P, const void* x, const void* index, const LpOut& o, hipStream_t st) {
   const int k = P.p.k;
-  if (k == 0) return lp_tile_launch<T, LAST, Wide, 0>(P, x, index, o, st);
+  if (k == 0) return lp_tile_launch<T, L, Wide, 0>(P, x, index, o, st);
   if constexpr (sizeof(typename T::S) == 2) {
     if (P.p.V <= Narrow::kClasses) {
-      if (k <= 4) return lp_tile_launch<T, LAST, Narrow, 4>(P, x, index, o, st);
-      if (k <= 8) return lp_tile_launch<T, LAST, Narrow, 8>(P, x, index, o, st);
-      if (k <= 16) return lp_tile_launch<T, LAST, Narrow, 16>(P, x, index, o, st);
-      return lp_tile_launch<T, LAST, Narrow, 32>(P, x, index, o, st);
+      if (k <= 4) return lp_tile_launch<T, L, Narrow, 4>(P, x, index, o, st);
+      if (k <= 8) return lp_tile_launch<T, L, Narrow, 8>(P, x, index, o, st);
+      if (k <= 16) return lp_tile_launch<T, L, Narrow, 16>(P, x, index, o, st);
+      return lp_tile_launch<T, L, Narrow, 32>(P, x, index, o, st);
     }
   }
-  if constexpr (sizeof(typename T::S) == 4 || !LAST) {  // (rows of that many classes do not come here)
-    if (k <= 4) return lp_tile_launch<T, LAST, Wide, 4>(P, x, index, o, st);
-    if (k <= 8) return lp_tile_launch<T, LAST, Wide, 8>(P, x, index, o, st);
-    return lp_tile_launch<T, LAST, Wide, 16>(P, x, index, o, st);
+  if constexpr (sizeof(typename T::S) == 4 || L == kPlanes) {  // (rows of that many classes do not come here)
+    if (k <= 4) return lp_tile_launch<T, L, Wide, 4>(P, x, index, o, st);
+    if (k <= 8) return lp_tile_launch<T, L, Wide, 8>(P, x, index, o, st);
+    return lp_tile_launch<T, L, Wide, 16>(P, x, index, o, st);
   }
   return DW_ERR_SHAPE;
 }
 template <class T>
 int lp_fwd(const Plan& P, const void* x, const void* index, const LpOut& o, void* ws, hipStream_t st) {
   const int k = P.p.k;
-  if (P.tile) return P.last ? lp_tile<T, true>(P, x, index, o, st) : lp_tile<T, false>(P, x, index, o, st);
+  if (P.tile)
+    return P.layout == kPlanes  ? lp_tile<T, kPlanes>(P, x, index, o, st)
+           : P.layout == kFlat ? lp_tile<T, kFlat>(P, x, index, o, st)
+                               : lp_tile<T, kTurned>(P, x, index, o, st);
   Part* parts = (Part*)ws;
   unsigned long long* keys = (unsigned long long*)((char*)ws + parts_bytes(P.p.rows, P.p.chunks));
   const typename T::S* xs = (const typename T::S*)x;
@@ -2017,12 +2178,16 @@ int lp_bwd(const Plan& P, const void* x, const void* index, const Stats3* stats,
            const float* g_ent, void* g, hipStream_t st) {
   using S = typename T::S;
   if (P.tile) {
-    if (P.last) {
+    if (P.layout == kFlat) {
+      const size_t lds = flat_bytes(P.p.V * (int)sizeof(S));
+      if (int rc = allow_lds(lp_tile_bwd<T, kFlat, ENT>, lds)) return rc;
+      lp_tile_bwd<T, kFlat, ENT><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
+    } else if (P.layout == kTurned) {
       const size_t lds = P.nw * kStageBytes;
-      if (int rc = allow_lds(lp_tile_bwd<T, true, ENT>, lds)) return rc;
-      lp_tile_bwd<T, true, ENT><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
+      if (int rc = allow_lds(lp_tile_bwd<T, kTurned, ENT>, lds)) return rc;
+      lp_tile_bwd<T, kTurned, ENT><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
     } else {
-      lp_tile_bwd<T, false, ENT><<<P.grid, P.nw * 64, 0, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
+      lp_tile_bwd<T, kPlanes, ENT><<<P.grid, P.nw * 64, 0, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
     }
   } else if (P.nt == 64) {
     lp_row_bwd<T, 64, ENT><<<P.grid, 64, 0, st>>>(P.p, (const S*)x, index, stats, g_lp, g_ent, (S*)g);
@@ -2031,17 +2196,17 @@ int lp_bwd(const Plan& P, const void* x, const void* index, const Stats3* stats,
   }
   return launched();
 }
-template <class T, bool LAST>
+template <class T, int L>
 int ds_tile_launch(const Plan& P, bool backward, const void* x, const void* teacher, const void* index, float* loss,
                    float4* stats, const float* g_loss, void* g, hipStream_t st) {
   using S = typename T::S;
-  const size_t lds = P.nw * (size_t)distill_stage_bytes(LAST, sizeof(S)) + distill_lds(P.nw, P.p.k, backward);
+  const size_t lds = distill_stages(L, P.nw, P.p.V, sizeof(S)) + distill_lds(P.nw, P.p.k, backward);
   if (backward) {
-    if (int rc = allow_lds(ds_tile_bwd<T, LAST>, lds)) return rc;
-    ds_tile_bwd<T, LAST><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, stats, g_loss, (S*)g);
+    if (int rc = allow_lds(ds_tile_bwd<T, L>, lds)) return rc;
+    ds_tile_bwd<T, L><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, stats, g_loss, (S*)g);
   } else {
-    if (int rc = allow_lds(ds_tile_fwd<T, LAST>, lds)) return rc;
-    ds_tile_fwd<T, LAST><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, loss, stats);
+    if (int rc = allow_lds(ds_tile_fwd<T, L>, lds)) return rc;
+    ds_tile_fwd<T, L><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, loss, stats);
   }
   return launched();
 }
@@ -2050,8 +2215,9 @@ int ds_run(const Plan& P, bool backward, const void* x, const void* teacher, con
            float4* stats, const float* g_loss, void* g, void* ws, hipStream_t st) {
   using S = typename T::S;
   if (P.tile)
-    return P.last ? ds_tile_launch<T, true>(P, backward, x, teacher, index, loss, stats, g_loss, g, st)
-                  : ds_tile_launch<T, false>(P, backward, x, teacher, index, loss, stats, g_loss, g, st);
+    return P.layout == kPlanes  ? ds_tile_launch<T, kPlanes>(P, backward, x, teacher, index, loss, stats, g_loss, g, st)
+           : P.layout == kFlat ? ds_tile_launch<T, kFlat>(P, backward, x, teacher, index, loss, stats, g_loss, g, st)
+                               : ds_tile_launch<T, kTurned>(P, backward, x, teacher, index, loss, stats, g_loss, g, st);
   const S* xs = (const S*)x;
   if (backward) {
     if (P.nt == 64) ds_row_bwd<T, 64><<<P.grid, 64, 0, st>>>(P.p, xs, teacher, index, stats, g_loss, (S*)g);
