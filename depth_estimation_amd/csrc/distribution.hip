@@ -15,7 +15,8 @@
 //   tile  one thread a row, 64 rows a wave; the waves of a block share the classes of their 64 rows.
 //         The classes of a volume (B, V, inner) are read plane by plane (64 neighbouring pixels a
 //         load); rows whose classes lie together are turned through LDS, 128 bytes of each row at
-//         a time.  No cross-lane work at all, and the top classes stay sorted in registers.
+//         a time, or all of the 64 rows at once, as one stretch of memory ("flat"), if they are not whole lines.
+//         No cross-lane work at all, and the top classes stay sorted in registers.
 //   row   a block (or a few, joined by a second kernel) for each row, for rows that are long or few.
 //
 // Every pass reads the logits once and a backward pass writes as much again, so the bound is memory: a large copy
@@ -631,7 +632,11 @@ struct FlatTile {
     const unsigned skip = (unsigned)(q.skip * row);
     for (unsigned c = threadIdx.x; c < pieces; c += threads) {
       const Vec<T> w{*at(c)};
-      if (c * 16 >= skip) {
+      if (c * 16 >= skip && p.past) {
+        rare();
+        store_vec<T, true>(base, c * 16, w);
+        rare();
+      } else if (c * 16 >= skip) {
         store_vec<T>(base, c * 16, w);
       } else if (c * 16 + 16 > skip) {
         const S* e = (const S*)at(c);
@@ -1116,8 +1121,7 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   constexpr int CH = stage_classes<T, L>();
   const Side z = side(p);
   const int c_lo = q.wave * p.cpw, c_hi = min(p.V, c_lo + p.cpw);
-  const FlatTile<T> tile(p, smem);  // kFlat only
-  const Column<T, L> col(stage, tile, c_lo, q.wave, q.lane);
+  const Column<T, L> col(stage, FlatTile<T>(p, smem), c_lo, q.wave, q.lane);
   const int64_t t0 = q.o * p.es[0] + q.i * p.es[2];
   Feed<T, L> feed;
   if (c_lo < c_hi) feed.issue(x, p, q, c_lo, min(CH, c_hi - c_lo));
@@ -1133,8 +1137,7 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   }
   float first[kGroup];  // the teacher's first values: in most lists all of them
   load_teachers(p, teacher, t0, 0, first);
-  if constexpr (L == kFlat) tile.in(x, p, q);  // with the barrier
-  else __syncthreads();
+  __syncthreads();
   bool alive = false;
   for (int e0 = 0; e0 < KP; e0 += kGroup) {
     int i8[kGroup];
@@ -1144,31 +1147,23 @@ __global__ void ds_tile_fwd(Prob p, const typename T::S* __restrict__ x, const v
   }
   Acc a = acc_empty(z);
   if (__any(alive)) {  // the same in every wave of the block
-    const auto take = [&](int c0, int n) {
-      take_listed(col, idx, K, c0, n, z.far(), [&](int e, bool hit, float old) { xs[(hit ? e : KP) * 64] = old; });
-      wave_sync();
-    };
-    if constexpr (L == kFlat) take(c_lo, max(c_hi - c_lo, 0));
     for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
       const int n = min(CH, c_hi - c0), ahead = min(CH, c_hi - c0 - CH);
       float v[32];
-      if constexpr (L != kFlat) {
-        wave_sync();
-        if constexpr (L == kTurned) {
-          feed.to_lds(q, stage);
-        } else {
+      wave_sync();
+      if constexpr (LAST) {
+        feed.to_lds(q, stage);
+      } else {
 #pragma unroll
-          for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
-        }
-        if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
-        wave_sync();
-        take(c0, n);
+        for (int u = 0; u < 32; ++u) *col.at(u) = feed.v[u];
       }
+      if (ahead > 0) feed.issue(x, p, q, c0 + CH, ahead);
+      wave_sync();
+      take_listed(col, idx, K, c0, n, z.far(), [&](int e, bool hit, float old) { xs[(hit ? e : KP) * 64] = old; });
+      wave_sync();
       for (int h = 0; h < n; h += 32) {
-        if constexpr (L == kTurned) {
+        if constexpr (LAST) {
           stage_read<T>(stage, q.lane, h, v);
-        } else if constexpr (L == kFlat) {
-          tile.read(q.lane, c0 + h, v);
         } else {
 #pragma unroll
           for (int u = 0; u < 32; ++u) v[u] = T::up(*col.at(u));
@@ -2001,8 +1996,8 @@ constexpr int kWantWaves = 2048;           // 8 a compute unit: enough loads in 
 // more, and what comes next would have to wait while that is written back: the next forward pass over 4096 x
 // 32768 bf16 takes 54 us instead of 80, over 4 x 256 x 192 x 640 bf16 66 instead of 86; the backward pass
 // itself 83 either way.  Smaller ones stay where the next operator finds them.  It takes whole 128-byte lines: rows
-// are written 1 KB at a time, planes only where 64 pixels are whole lines (255 bins of 131 x 641 pixels bf16: 165 us
-// instead of 96), turned rows never (193 classes f16: 45 instead of 29).
+// are written 1 KB at a time, flat tiles in one stretch, planes only where 64 pixels are whole lines (255 bins of 131 x 641
+// pixels bf16: 165 us instead of 96), turned rows never (193 classes f16: 45 instead of 29).
 constexpr int64_t kPastBytes = (int64_t)128 << 20;
 constexpr size_t kLdsBudget = 152 * 1024;  // of a block, of the compute unit's 160 KB
 constexpr int kMostFlat = 64 * 1024;       // of a flat tile
@@ -2054,26 +2049,33 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
   P.tile = !P.last || (p.V <= 2048 && tiles * 4 >= kWantWaves / 4);
   if (P.tile) {
     const int row = p.V * esize;
-    P.layout = !P.last ? kPlanes : row % kSegBytes != 0 && flat_bytes(row) <= kMostFlat ? kFlat : kTurned;
+    // Rows that are not whole lines lie in LDS as they do in memory, if 64 of them fit 64 KB (193 classes of 4 x 192 x 320
+    // pixels f16: forward 32 us, turned 35; backward 40 and 70; distillation backward 54 and 64; f32, 250 classes,
+    // half as many pixels: 37 and 45, 49 and 69, 55 and 76).  Not the distillation's forward pass, where one wave ends
+    // the work of a block: 193 classes 44 and 40, f32 42 and 38, 50 classes 39 and 42.
+    const bool flat = P.last && row % kSegBytes != 0 && flat_bytes(row) <= kMostFlat && (!distill || backward);
+    P.layout = !P.last ? kPlanes : flat ? kFlat : kTurned;
     const int stage = P.layout == kTurned ? kSegBytes / esize : 32;
     const int stages = (p.V + stage - 1) / stage;
     const int most = distill || backward ? 16 : list_waves(P.last, p.k > 0);
     P.nw = 1;
     while (P.nw < most && tiles * P.nw < kWantWaves && P.nw * 2 <= stages) P.nw *= 2;
-    if (P.layout == kFlat)
-      while (P.nw < 4 && P.nw * 2 <= stages) P.nw *= 2;
     const auto lds = [&](int nw) {
       return distill ? distill_stages(P.layout, nw, p.V, esize) + distill_lds(nw, p.k, false)
                      : (P.layout == kTurned ? (size_t)nw * kStageBytes : P.layout == kFlat ? flat_bytes(row) : 0) +
-                           (size_t)nw * 64 * (12 + 8 * 16);
+                           (size_t)nw * 64 * (backward ? 0 : 12 + (p.k ? 8 * 16 : 0));
     };
-    if (distill) {
+    const auto waves = [&](int nw) { return lds(nw) > kLdsBudget ? 0 : (int)(kLdsBudget / lds(nw)) * nw; };
+    if (flat) {
+      // The waves of a block share the tile; 16 or more should fit a compute unit (f16, 193 classes: 43 + 65 us with one
+      // wave a block, 35 + 53 with two, 33 + 39 with 4 and with 8; 50 classes: 24 + 36 with one, 27 + 34 with two).
+      while (P.nw * 2 <= (most < stages ? most : stages) && waves(P.nw) < 16) P.nw *= 2;
+    } else if (distill) {
       // The list is the block's, a stage each wave's, so more waves a block are more waves in the LDS of a compute
       // unit.  The forward pass ends with one wave's work: it takes that only where fewer than 8 waves would fit
       // (channels_last f16, 128 classes, 8 entries: 35 us with one wave a block, 39 with two; bf16 planes, 256
       // classes, 64 entries: 210 and 116 with one and 8).  The backward pass does not (bf16 planes, 256 classes,
       // 8 entries: 118 us with one, 105 with two).
-      const auto waves = [&](int nw) { return lds(nw) > kLdsBudget ? 0 : (int)(kLdsBudget / lds(nw)) * nw; };
       for (int nw = P.nw * 2; nw <= 16 && nw <= stages; nw *= 2)
         if (waves(nw) > waves(P.nw) && waves(P.nw) < (backward ? 16 : 8)) P.nw = nw;
     }
@@ -2106,7 +2108,7 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
 // g: where the gradient goes
 void choose_stores(Plan& P, int esize, const void* g) {
   if (P.p.rows * P.p.V * esize < kPastBytes) return;
-  P.p.past = P.tile ? !P.last && P.p.inner % 64 == 0 && ((uintptr_t)g & 127) == 0 : true;
+  P.p.past = P.tile ? (P.layout == kFlat || (P.layout == kPlanes && P.p.inner % 64 == 0)) && ((uintptr_t)g & 127) == 0 : true;
 }
 int check_ws(const Plan& P, const void* ws, size_t bytes) {
   if (P.ws == 0) return DW_OK;
@@ -2204,7 +2206,7 @@ int ds_tile_launch(const Plan& P, bool backward, const void* x, const void* teac
   if (backward) {
     if (int rc = allow_lds(ds_tile_bwd<T, L>, lds)) return rc;
     ds_tile_bwd<T, L><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, stats, g_loss, (S*)g);
-  } else {
+  } else if constexpr (L != kFlat) {
     if (int rc = allow_lds(ds_tile_fwd<T, L>, lds)) return rc;
     ds_tile_fwd<T, L><<<P.grid, P.nw * 64, lds, st>>>(P.p, (const S*)x, teacher, index, loss, stats);
   }

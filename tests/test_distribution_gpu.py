@@ -126,7 +126,8 @@ def test_log_probs_rows(n, V, dtype):
 
 # enough rows that a thread takes one; the last tile is not full
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V,top", [(1, 1), (7, 4), (31, 3), (32, 8), (33, 9), (63, 0), (64, 16), (65, 17), (129, 33), (96, 64)])
+@pytest.mark.parametrize("V,top", [(1, 1), (7, 4), (31, 3), (32, 8), (33, 9), (63, 0), (64, 16), (65, 17), (129, 33), (96, 64),
+                                   (200, 8), (255, 5), (511, 4), (513, 0)])
 def test_log_probs_many_short_rows(V, top, dtype):
     x, _ = _make("rows", (8200, V), dtype, seed=V)
     _check_log_probs(x, _index((8200,), V, V), "rows", [1.0, -0.5][V % 2], top)
@@ -321,7 +322,7 @@ def test_distill_rows(n, V, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V,k", [(1, 1), (7, 7), (31, 4), (33, 8), (64, 3), (65, 20), (129, 64)])
+@pytest.mark.parametrize("V,k", [(1, 1), (7, 7), (31, 4), (33, 8), (64, 3), (65, 20), (129, 64), (200, 16), (255, 8), (511, 64), (513, 4)])
 def test_distill_many_short_rows(V, k, dtype):
     x, g = _make("rows", (8201, V), dtype, seed=V)
     val, idx = _teacher((8201,), V, k, g)
