@@ -763,7 +763,7 @@ __device__ __forceinline__ void settle(float (&v)[32], float far, int n) {
 // reduction over 64 lanes on every few hundred classes.  The waves of a block split the classes where there are
 // too few rows to fill the chip, and join through LDS.  Loads of the next 32 classes are issued before the ones at
 // hand are worked on.  12 x 64 x 96 x 320 bf16 (47 MB): 15.8 us, 3.0 TB/s, the vector pipe; 1 x 256 x 256 x 512 f32 with
-// the top 8 (134 MB): 34 us, 4.0 TB/s; 4 x 193 x 96 x 320 f16, classes last (47 MB): 18.4 us.
+// the top 8 (134 MB): 34 us, 4.0 TB/s; 4 x 193 x 96 x 320 f16, classes last (47 MB): 18.1 us.
 // K: top classes kept in registers as keys of kind P (0: none).  More than K wanted: further passes over the data,
 // each for the next K below the last key of the pass before.
 // Turning rows and keeping their lists takes up to 180 registers: those blocks have at most 8 waves, so that they get
@@ -921,8 +921,9 @@ __device__ __forceinline__ float lp_grad(const LpCoef& r, float v, float c, floa
 }
 
 // The rows' sums come from the forward pass, so this is one read and one write: dx_j = e_j (k0 + k1 t_j), and the
-// given class on top.  12 x 64 x 96 x 320 bf16 (94 MB): 20.0 us, 4.7 TB/s, what a copy takes.  4 x 193 x 96 x 320 f16, classes
-// last (95 MB): 28 us; rows of 386 bytes begin inside the memory's lines, and 66 MB are written for 47.
+// given class on top.  12 x 64 x 96 x 320 bf16 (94 MB): 20.0 us, 4.7 TB/s, what a copy takes.  4 x 193 x 96 x 320 f16,
+// classes last (95 MB): 24 us; 28 where its rows of 386 bytes were turned 128 bytes at a time, and the halves of a line,
+// written long after each other, reached memory one by one (66 MB written for 47).
 template <class T, int L, bool ENT>
 __global__ void lp_tile_bwd(Prob p, const typename T::S* __restrict__ x, const void* __restrict__ index,
                             const Stats3* __restrict__ stats, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
