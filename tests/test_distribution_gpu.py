@@ -659,6 +659,33 @@ def test_forward_and_backward_in_two_captured_graphs(shape):
                 assert torch.equal(got, want)
 
 
+def test_capture_of_calls_that_never_ran_before():
+    # (the kernels of these shapes ask for more LDS than a launch gets by itself)
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    x = torch.randn(9001, 255, device="cuda", requires_grad=True)
+    y = torch.randn(1, 2048, 64, 3, device="cuda", dtype=torch.float16, requires_grad=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = []
+        for v in (x, y):
+            o = log_probs(v, top=37)
+            loss = distill_loss(v, o.top_log_prob, o.top_index, renormalise=True)
+            outs.append((o, loss) + torch.autograd.grad([o.entropy, loss], v, [torch.ones_like(loss), torch.ones_like(loss)]))
+    for seed in (1, 2):
+        for v in (x, y):
+            v.data.normal_(generator=torch.Generator(device="cuda").manual_seed(seed))
+        g.replay()
+        torch.cuda.synchronize()
+        for v, (o, loss, grad) in zip((x, y), outs):
+            want = log_probs(v, top=37)
+            assert torch.equal(o.entropy, want.entropy) and torch.equal(o.top_index, want.top_index)
+            wl = distill_loss(v, want.top_log_prob, want.top_index, renormalise=True)
+            assert torch.equal(loss, wl)
+            wg, = torch.autograd.grad([want.entropy, wl], v, [torch.ones_like(wl), torch.ones_like(wl)])
+            assert torch.equal(grad, wg)
+
+
 def test_two_threads_on_their_own_streams_give_the_same_bits():
     import threading
     problems = [_problem((3, 40000), 0), _problem((1, 64, 24, 80), 1)]
