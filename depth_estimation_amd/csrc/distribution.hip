@@ -1030,13 +1030,12 @@ struct Column {
   __device__ __forceinline__ S* at(int u) const { return first + (L == kPlanes ? u * 64 : u); }
   __device__ __forceinline__ S* at(bool hit, int u) const { return hit ? at(u) : nowhere; }
 };
-// LDS of the classes: a stage a wave, or the flat tile of the block
-__host__ __device__ inline size_t distill_stages(int layout, int nw, int V, int esize) {
-  if (layout == kFlat) return flat_bytes(V * esize) + (size_t)nw * 64 * 4;
-  return nw * (size_t)(layout == kTurned ? kStageBytes : 33 * 64 * esize);
-}
+// LDS of the classes: a stage a wave, or the flat tile of the block and the lanes' places of their own
 __host__ __device__ constexpr int distill_stage_bytes(int layout, int esize) {
   return layout == kTurned ? kStageBytes : layout == kPlanes ? 33 * 64 * esize : 0;
+}
+__host__ __device__ inline size_t distill_stages(int layout, int nw, int V, int esize) {
+  return layout == kFlat ? flat_bytes(V * esize) + (size_t)nw * 64 * 4 : nw * (size_t)distill_stage_bytes(layout, esize);
 }
 constexpr int kGroup = 8;  // entries handled at once: their LDS accesses overlap
 __host__ __device__ constexpr int padded(int k) { return (k + kGroup - 1) / kGroup * kGroup; }
