@@ -827,6 +827,11 @@ void lp_tile_fwd(Prob p, const typename T::S* __restrict__ x, const void* __rest
             Key nk[K];
 #pragma unroll
             for (int i = 0; i < K; ++i) nk[i] = P::of(v[g + i], z.sign, c0 + h + g + i);
+            if (L == kFlat && n < 32) {  // (c0 + n and on: the next wave's classes, which has them in its own list)
+              const int mine = (int)fresh_uniform(n);
+#pragma unroll
+              for (int i = 0; i < K; ++i) nk[i] = g + i < mine ? nk[i] : P::kNone;
+            }
             if (done > 0) {
 #pragma unroll
               for (int i = 0; i < K; ++i) nk[i] = nk[i] < limit ? nk[i] : P::kNone;

@@ -231,6 +231,30 @@ def test_log_probs_masks_and_special_values(layout, dtype):
     _check_log_probs(-x, idx, lay, -1.0, 20)
 
 
+# lists that reach into impossible classes, where the waves of a block share a row's classes and their shares end
+# inside a step of 32
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,top", [(33, 33), (40, 32), (40, 40), (70, 64), (72, 41), (100, 64), (193, 64), (250, 33)])
+@pytest.mark.parametrize("layout", ["rows", "last"])
+def test_lists_longer_than_the_possible_classes(layout, V, top, dtype):
+    shape = (8256, V) if layout == "rows" else (3, V, 43, 64)
+    x, g = _make(layout, shape, dtype, seed=V + top)
+    rows = _last(x).flatten(0, -2)
+    n = rows.shape[0]
+    # row r keeps r % (V + 1) of its classes, anywhere; every third row the first or the last ones
+    order = torch.rand(n, V, generator=g).argsort(1)
+    order[1::3] = torch.arange(V)
+    order[2::3] = torch.arange(V).flip(0)
+    keep = (torch.arange(n) % (V + 1))[:, None]
+    rows = torch.where(order < keep, rows, -INF)
+    rows[5::101, V // 2] = float("nan")
+    rows[7::103, 3] = INF
+    x = rows if layout == "rows" else rows.view(3, 43, 64, V).movedim(-1, 1).contiguous()
+    idx = _index((n,) if layout == "rows" else (3, 43, 64), V, 1)
+    _check_log_probs(x, idx, layout, 1.0, top, with_grad=False)
+    _check_log_probs(-x, idx, layout, -1.0, top, with_grad=False)
+
+
 @pytest.mark.parametrize("layout", ["volume", "last", "rows"])
 def test_rows_without_upstream_gradient_get_zeros_whatever_they_hold(layout):
     from depth_estimation_amd.distribution import distill_loss, log_probs
