@@ -272,18 +272,20 @@ __device__ __forceinline__ float log_p(float x, float m, float ln_s, float scale
 }
 
 // ---- order keys --------------------------------------------------------------------------------
-// 64-bit whole number that orders classes by value, then by lowest index; NaN above everything
+// 64-bit whole number that orders classes by value, then by lowest index; NaN above everything.  No key is all ones
+// (NaN at class 0 comes nearest) or 0: a search may begin above or below every key.
+constexpr unsigned kLowestFirst = 0xfffffffeu;
 __device__ __forceinline__ unsigned long long key_u64(float v, int idx) {
   unsigned b = __builtin_bit_cast(unsigned, v + 0.f);
   b = v != v ? 0xffffffffu : (b ^ ((unsigned)((int)b >> 31) | 0x80000000u));
-  return ((unsigned long long)b << 32) | (0xffffffffu - (unsigned)idx);
+  return ((unsigned long long)b << 32) | (kLowestFirst - (unsigned)idx);
 }
 __device__ __forceinline__ float key_value(unsigned long long k) {
   const unsigned b = (unsigned)(k >> 32);
   if (b == 0xffffffffu) return __builtin_nanf("");
   return __builtin_bit_cast(float, (b >> 31) ? (b ^ 0x80000000u) : ~b);
 }
-__device__ __forceinline__ int key_index(unsigned long long k) { return (int)(0xffffffffu - (unsigned)k); }
+__device__ __forceinline__ int key_index(unsigned long long k) { return (int)(kLowestFirst - (unsigned)k); }
 
 // Keys of the lists that are kept in registers: numbers of the same order.  A NaN has to be positive (order_nans()).
 //

@@ -255,6 +255,20 @@ def test_lists_longer_than_the_possible_classes(layout, V, top, dtype):
     _check_log_probs(-x, idx, layout, -1.0, top, with_grad=False)
 
 
+# rows of one block (64 and 256 threads), split rows, tiles; class 0 has the largest key a list knows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,top", [(3, 1, 1), (3, 10, 10), (3, 10, 3), (5, 64, 64), (2600, 4500, 5), (2, 4500, 8), (3, 50001, 64),
+                                     (8256, 40, 40), (8256, 64, 64)])
+def test_top_of_rows_with_nan_in_the_first_class(n, V, top, dtype):
+    x, _ = _make("rows", (n, V), dtype, seed=V)
+    x[0, 0] = float("nan")
+    x[1] = float("nan")
+    x[-1, 0] = x[-1, V // 2] = float("nan")
+    idx = _index((n,), V, 1)
+    _check_log_probs(x, idx, "rows", 1.0, top, with_grad=False)
+    _check_log_probs(x, idx, "rows", -1.0, top, with_grad=False)
+
+
 @pytest.mark.parametrize("layout", ["volume", "last", "rows"])
 def test_rows_without_upstream_gradient_get_zeros_whatever_they_hold(layout):
     from depth_estimation_amd.distribution import distill_loss, log_probs
