@@ -5,8 +5,10 @@
 // training steps are bound by it: a node written in Python runs in the autograd engine's own thread, where the
 // interpreter's lock and cold caches took about half of such a step (80 to 90 us, 4 x 64 x 4 x 4).
 //
-// The library's functions and descriptors come from Python as addresses: which build of the library is in use, and
-// what the shapes and types decide, is settled there (distribution.py).
+// The library's functions come from Python as addresses, descriptors as their words: which build of the library is in
+// use, and what the shapes and types decide, is settled there (distribution.py).  These calls launch by pointer, so
+// nothing that records or replaces tensor operations sees more of them than their outputs being made: distribution.py
+// calls the registered operators wherever something of the kind watches.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -80,14 +82,21 @@ std::vector<int64_t> with(at::IntArrayRef rows, int64_t at, int64_t n) {
   return s;
 }
 
-// What the backward pass has to know travels with the node as its bytes: the Python object that the descriptor came
-// from may be gone by then.
+// A descriptor by value: a call that is kept for later holds no address of this process.
+dw_dist_desc descriptor(at::IntArrayRef words) {
+  dw_dist_desc d;
+  static_assert(sizeof d % sizeof(int64_t) == 0);
+  TORCH_CHECK(words.size() * sizeof(int64_t) == sizeof d, "descriptor: expected ", sizeof d / sizeof(int64_t), " words");
+  std::memcpy(&d, words.data(), sizeof d);
+  return d;
+}
+// What the backward pass has to know travels with the node as its bytes.
 struct Kept {
   dw_dist_desc desc;
   int64_t dim, layout, list_layout;
 };
-void keep(AutogradContext* ctx, int64_t desc, int64_t dim, int64_t layout, int64_t list_layout) {
-  const Kept k{*reinterpret_cast<const dw_dist_desc*>(desc), dim, layout, list_layout};
+void keep(AutogradContext* ctx, const dw_dist_desc& desc, int64_t dim, int64_t layout, int64_t list_layout) {
+  const Kept k{desc, dim, layout, list_layout};
   ctx->saved_data["call"] = std::string(reinterpret_cast<const char*>(&k), sizeof k);
 }
 Kept kept(AutogradContext* ctx) {
@@ -107,8 +116,9 @@ Tensor once(Tensor grad) {
 
 struct LogProbs : torch::autograd::Function<LogProbs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& given,
-                               int64_t desc, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout,
+                               at::IntArrayRef words, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout,
                                bool train) {
+    const dw_dist_desc desc = descriptor(words);
     const Tensor x = in_place(logits, layout), index_in = given ? *given : Tensor(), index = contiguous(index_in);
     const c10::OptionalDeviceGuard guard(x.device());
     const auto f32 = x.options().dtype(at::kFloat).memory_format(std::nullopt);
@@ -123,7 +133,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
       top_idx = at::empty(with(rows, dim, top), f32.dtype(at::kInt));
     }
     const Tensor ws = workspace(x, nbytes);
-    check(lib.log_probs_fwd(reinterpret_cast<const dw_dist_desc*>(desc), data(x), data(index), data<float>(lp),
+    check(lib.log_probs_fwd(&desc, data(x), data(index), data<float>(lp),
                             data<float>(ent), data<float>(top_lp), data<int32_t>(top_idx), data<float>(stats), data(ws),
                             nbytes, stream_of(x)),
           "dw_log_probs_fwd");
@@ -164,8 +174,9 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
 
 struct Distill : torch::autograd::Function<Distill> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher_in, const Tensor& index_in,
-                        int64_t desc, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t layout, int64_t list_layout,
+                        at::IntArrayRef words, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t layout, int64_t list_layout,
                         bool train) {
+    const dw_dist_desc desc = descriptor(words);
     const Tensor x = in_place(logits, layout), teacher = in_place(teacher_in, list_layout),
                  index = in_place(index_in, list_layout);
     const c10::OptionalDeviceGuard guard(x.device());
@@ -173,7 +184,7 @@ struct Distill : torch::autograd::Function<Distill> {
     Tensor loss = at::empty(rows, f32), stats;
     if (train) stats = at::empty(with(rows, rows.size(), 4), f32);
     const Tensor ws = workspace(x, nbytes);
-    check(lib.distill_fwd(reinterpret_cast<const dw_dist_desc*>(desc), data(x), data(teacher), data(index),
+    check(lib.distill_fwd(&desc, data(x), data(teacher), data(index),
                           data<float>(loss), data<float>(stats), data(ws), nbytes, stream_of(x)),
           "dw_distill_fwd");
     if (train) {
@@ -201,12 +212,12 @@ struct Distill : torch::autograd::Function<Distill> {
 };
 
 // [log_prob if there is an index, entropy, and the two top lists if top > 0]
-std::vector<Tensor> log_probs(const Tensor& logits, const std::optional<Tensor>& index, int64_t desc, int64_t nbytes,
+std::vector<Tensor> log_probs(const Tensor& logits, const std::optional<Tensor>& index, at::IntArrayRef desc, int64_t nbytes,
                               at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout) {
   const bool train = logits.requires_grad() && at::GradMode::is_enabled();
   return LogProbs::apply(logits, index, desc, nbytes, rows, dim, top, layout, train);
 }
-Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, int64_t desc, int64_t nbytes,
+Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, at::IntArrayRef desc, int64_t nbytes,
                at::IntArrayRef rows, int64_t dim, int64_t layout, int64_t list_layout) {
   const bool train = logits.requires_grad() && at::GradMode::is_enabled();
   return Distill::apply(logits, teacher, index, desc, nbytes, rows, dim, layout, list_layout, train);
@@ -215,8 +226,8 @@ Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index,
 
 TORCH_LIBRARY_FRAGMENT(depthwarp, m) {
   m.def("_bind_distribution(int strerror, int lp_fwd, int lp_bwd, int ds_fwd, int ds_bwd) -> ()", &bind);
-  m.def("_log_probs_eager(Tensor logits, Tensor? index, int desc, int nbytes, int[] rows, int dim, int top, "
+  m.def("_log_probs_eager(Tensor logits, Tensor? index, int[] desc, int nbytes, int[] rows, int dim, int top, "
         "int layout) -> Tensor[]", &log_probs);
-  m.def("_distill_eager(Tensor logits, Tensor teacher, Tensor index, int desc, int nbytes, int[] rows, int dim, "
+  m.def("_distill_eager(Tensor logits, Tensor teacher, Tensor index, int[] desc, int nbytes, int[] rows, int dim, "
         "int layout, int list_layout) -> Tensor", &distill);
 }

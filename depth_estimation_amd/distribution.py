@@ -25,6 +25,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -66,6 +67,17 @@ def _eager():
     return torch.ops.depthwarp._log_probs_eager.default, torch.ops.depthwarp._distill_eager.default
 
 
+_PLAIN = (Tensor, torch.nn.Parameter)
+
+
+def _watched(*tensors: Optional[Tensor]) -> bool:
+    """Whether something records or replaces tensor operations (torch.compile, a dispatch mode such as make_fx's or a
+    FakeTensorMode, torch.jit.trace, tensors of another class): it has to see the registered operators."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._get_tracing_state() is not None
+            or any(type(t) not in _PLAIN for t in tensors if t is not None))
+
+
 def _call(device: torch.device, fn, *args) -> None:
     """One library call on the device's current stream (the library launches on the current device)."""
     with torch.cuda.device(device):
@@ -84,7 +96,7 @@ class _Plan(NamedTuple):
     dim: int
     rows: tuple        # shape without the class axis
     ref: object        # descriptor, for ctypes
-    address: int       # the same for C++
+    words: tuple       # the same for C++
     nbytes: int        # workspace
     top: int = 0
     list_layout: int = 0      # distillation: the same of the teacher's tensors (_COPY where they have no common order)
@@ -124,7 +136,7 @@ def _descriptor(workspace_of: str, shape, dim: int, last: bool, dtype, scale: fl
     nbytes = getattr(_lib.lib(), workspace_of)(ref)
     if nbytes < 0:
         _lib.check(int(nbytes), f"{workspace_of}(shape={tuple(shape)}, entries={entries}, scale={scale})")
-    return ref, C.addressof(d), nbytes
+    return ref, struct.unpack(f"{C.sizeof(d) // 8}q", bytes(d)), nbytes
 
 
 def _check_problem(shape, dtype, dim: int, scale: float) -> int:
@@ -173,8 +185,8 @@ def _make_lp_plan(shape, stride, dtype, index_dtype, index_shape, dim: int, scal
     dim = _lp_check(shape, dtype, index_dtype, index_shape, dim, scale, top)
     layout = _layout(shape, stride, dim)
     flags = 0 if index_dtype is None else _INDEX_FLAGS[index_dtype]
-    ref, address, nbytes = _descriptor("dw_log_probs_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, top, flags)
-    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, address, nbytes, top)
+    ref, words, nbytes = _descriptor("dw_log_probs_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, top, flags)
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, words, nbytes, top)
 
 
 _lp_plan = functools.lru_cache(maxsize=512)(_make_lp_plan)
@@ -231,7 +243,7 @@ def _lp_backward(logits: Tensor, index: Optional[Tensor], stats: Tensor, g_lp: O
     return grad
 
 
-# Torch operators with the same results, which is what torch.compile traces.  An operator always returns tensors:
+# Torch operators with the same results, which is what tracers record.  An operator always returns tensors:
 # without an index, log_prob is empty; the last result is for the backward pass.
 
 @torch.library.custom_op("depthwarp::log_probs", mutates_args=())
@@ -310,13 +322,13 @@ def log_probs(logits: Tensor, index: Optional[Tensor] = None, *, dim: int = 1, s
     if not logits.is_cuda or (index is not None and index.device != logits.device):
         _check_device(logits, index=index)
     scale, top = float(scale), int(top)
-    if torch.compiler.is_compiling():
+    if _watched(logits, index):
         dim = _lp_check(logits.shape, logits.dtype, None if index is None else index.dtype,
                         None if index is None else index.shape, dim, scale, top)
         lp, ent, top_lp, top_idx, _ = _log_probs_op(logits, index, dim, scale, top)
         return LogProbs(None if index is None else lp, ent, top_lp if top else None, top_idx if top else None)
     plan = _plan_of(logits, index, dim, scale, top)
-    out = _eager()[0](logits, index, plan.address, plan.nbytes, plan.rows, plan.dim, top, plan.layout)
+    out = _eager()[0](logits, index, plan.words, plan.nbytes, plan.rows, plan.dim, top, plan.layout)
     if index is None:
         return LogProbs(None, *out) if top else LogProbs(None, out[0], None, None)
     return LogProbs(*out) if top else LogProbs(*out, None, None)
@@ -347,8 +359,8 @@ def _make_ds_plan(shape, stride, dtype, t_shape, t_stride, t_dtype, i_shape, i_s
     strides = (k * inner, 1, k) if list_layout == _LAST else (k * inner, inner, 1)
     layout = _layout(shape, stride, dim)
     flags = _INDEX_FLAGS[i_dtype] | _TEACHER_FLAGS[t_dtype] | (_lib.DW_DIST_RENORMALISE if renormalise else 0)
-    ref, address, nbytes = _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k, flags, strides)
-    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, address, nbytes, list_layout=list_layout)
+    ref, words, nbytes = _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k, flags, strides)
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, words, nbytes, list_layout=list_layout)
 
 
 _ds_plan = functools.lru_cache(maxsize=512)(_make_ds_plan)
@@ -442,10 +454,10 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
     scale, renormalise = float(scale), bool(renormalise)
     if teacher.requires_grad and torch.is_grad_enabled():
         raise ValueError("teacher: no gradient flows to the teacher; pass teacher.detach()")
-    if torch.compiler.is_compiling():
+    if _watched(logits, teacher, teacher_index):
         dim = _ds_check(logits.shape, logits.dtype, teacher.shape, teacher.dtype, teacher_index.shape,
                         teacher_index.dtype, dim, scale)
         return _distill_op(logits, teacher, teacher_index, dim, scale, renormalise)[0]
     plan = _ds_plan_of(logits, teacher, teacher_index, dim, scale, renormalise)
-    return _eager()[1](logits, teacher, teacher_index, plan.address, plan.nbytes, plan.rows, plan.dim, plan.layout,
+    return _eager()[1](logits, teacher, teacher_index, plan.words, plan.nbytes, plan.rows, plan.dim, plan.layout,
                        plan.list_layout)

@@ -154,3 +154,58 @@ def test_python_refuses_cpu_tensors():
         log_probs(torch.zeros(2, 4), torch.zeros(2, dtype=torch.long))
     with pytest.raises(_lib.DepthwarpError):
         distill_loss(torch.zeros(2, 4), torch.zeros(2, 2), torch.zeros(2, 2, dtype=torch.long))
+
+
+# ------------------------------------------------------------------------------------ tracing
+
+def _fake_problem(mode, dtype=torch.float32):
+    with mode:
+        x = torch.empty(2, 20, 4, 6, device="cuda:0", dtype=dtype)
+        idx = torch.empty(2, 4, 6, device="cuda:0", dtype=torch.long)
+        t = torch.empty(2, 5, 4, 6, device="cuda:0")
+        ti = torch.empty(2, 5, 4, 6, device="cuda:0", dtype=torch.int32)
+    return x, idx, t, ti
+
+
+def test_calls_on_tensors_without_data_give_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    mode = FakeTensorMode()
+    x, idx, t, ti = _fake_problem(mode, torch.bfloat16)
+
+    def check():
+        out = log_probs(x, idx, top=3)
+        loss = distill_loss(x, t, ti)
+        assert out.log_prob.shape == out.entropy.shape == loss.shape == (2, 4, 6)
+        assert out.top_log_prob.shape == out.top_index.shape == (2, 3, 4, 6) and out.top_index.dtype == torch.int32
+        assert out.log_prob.dtype == loss.dtype == torch.float32 and out.entropy.device == x.device
+        bare = log_probs(x)
+        assert bare.log_prob is None and bare.top_index is None and bare.entropy.shape == (2, 4, 6)
+        with pytest.raises(TypeError):
+            log_probs(x, idx.float())
+        with pytest.raises(ValueError):
+            distill_loss(x, t, ti[:, :4])
+
+    with mode:
+        check()
+    check()   # the tensors' own class is enough
+
+
+def test_traced_graphs_hold_the_operators_and_what_decides_them():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+
+    def f(x, idx, t, ti):
+        o = log_probs(x, idx, scale=-2.0, top=3)
+        loss = distill_loss(x, t, ti, renormalise=True)
+        return o.log_prob, o.top_index, loss
+
+    mode = FakeTensorMode()
+    args = _fake_problem(mode)
+    with mode:
+        graph = make_fx(f)(*args)
+    calls = {n.target: n for n in graph.graph.nodes if n.op == "call_function"}
+    lp, ds = calls[torch.ops.depthwarp.log_probs.default], calls[torch.ops.depthwarp.distill_loss.default]
+    assert lp.args[2:] == (1, -2.0, 3) and ds.args[3:] == (1, 1.0, True)
+    assert not any("eager" in str(t) or "empty" in str(t) for t in calls)

@@ -874,6 +874,74 @@ def test_traced_calls_give_the_eager_results():
     assert torch.equal(want, got) and torch.equal(wi, gi) and torch.equal(gw, gg)
 
 
+def _run_of_both(x, idx, t, ti):
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    o = log_probs(x, idx, scale=-2.0, top=3)
+    return o.log_prob, o.entropy, o.top_log_prob, o.top_index, distill_loss(x, t, ti, scale=0.5, renormalise=True)
+
+
+def test_graphs_of_make_fx_compute_what_they_recorded():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    p = [v.detach() for v in _problem((2, 20, 4, 6), 0)]
+    graph = make_fx(_run_of_both)(*p)
+    assert any("depthwarp.log_probs" in str(n.target) for n in graph.graph.nodes)
+
+    def both_ways(x, idx, t, ti):
+        r = _run_of_both(x, idx, t, ti)
+        return torch.autograd.grad([r[0], r[1], r[4]], x, [torch.ones_like(r[0])] * 3)[0]
+
+    backward = make_fx(both_ways)(*_problem((2, 20, 4, 6), 0))
+    for seed in (1, 2):
+        p = _problem((2, 20, 4, 6), seed)
+        for got, want in zip(graph(*p), _run_of_both(*p)):
+            assert torch.equal(got, want)
+        assert torch.equal(backward(*p), both_ways(*p))
+
+
+def test_modules_of_jit_trace_hold_their_calls_by_value():
+    import io
+    from depth_estimation_amd import distribution
+    p = [v.detach() for v in _problem((2, 20, 4, 6), 0)]
+    traced = torch.jit.trace(_run_of_both, tuple(p), check_trace=False)
+    assert "_eager" not in str(traced.inlined_graph) and "depthwarp::log_probs" in str(traced.inlined_graph)
+    file = io.BytesIO()
+    torch.jit.save(traced, file)
+    file.seek(0)
+    loaded = torch.jit.load(file)
+    for seed in (1, 2):
+        distribution._lp_plan.cache_clear()
+        distribution._ds_plan.cache_clear()
+        p = _problem((2, 20, 4, 6), seed)
+        want = _run_of_both(*p)
+        wg, = torch.autograd.grad([want[0], want[1], want[4]], p[0], [torch.ones_like(want[0])] * 3)
+        for m in (traced, loaded):
+            got = m(*p)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+            gg, = torch.autograd.grad([got[0], got[1], got[4]], p[0], [torch.ones_like(want[0])] * 3)
+            assert torch.equal(gg, wg)
+
+
+def test_calls_under_a_dispatch_mode_give_the_same_results():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    p = [v.detach() for v in _problem((2, 20, 4, 6), 0)]
+    want = _run_of_both(*p)
+    n = torch._neg_view(-p[0])
+    with Watch():
+        got = _run_of_both(*p)
+        neg = _run_of_both(n, *p[1:])
+    assert "depthwarp.log_probs.default" in seen and "depthwarp.distill_loss.default" in seen
+    for a, b, c in zip(got, want, neg):
+        assert torch.equal(a, b) and torch.equal(c, b)
+
+
 @pytest.mark.parametrize("shape", [(9, 1 << 28), (2300000, 1000), (3, 2900, 512, 512)])
 def test_offsets_beyond_32_bits(shape):
     """More than 2^31 elements: the last rows come out as they do on their own."""
