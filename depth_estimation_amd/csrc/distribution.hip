@@ -34,6 +34,9 @@ constexpr float kLn2 = 0x1.62e43p-1f;      // fl(ln 2)
 constexpr float kLog2e = 0x1.715476p+0f;   // fl(log2 e)
 constexpr float kLog2eRest = 0x1.4ae0cp-26f;  // log2 e - fl(log2 e)
 constexpr float kFloor = -1e30f;           // stands in for an exponent of -inf where 0 * -inf would be NaN
+// The same in a gradient, where it is multiplied by an upstream value: 2^-1000 is 0 already, and the product stays finite
+// for upstream gradients up to 1e35
+constexpr float kGradFloor = -1000.f;
 constexpr int kMaxEntries = 64;
 
 // ---- element types -------------------------------------------------------------------------
@@ -924,7 +927,7 @@ __device__ __forceinline__ LpCoef lp_coef(const Prob& p, int64_t row, const void
 template <bool ENT>
 __device__ __forceinline__ float lp_grad(const LpCoef& r, float v, float c, float add) {
   const float t = (v - r.m) * c, e = exp2_(t);
-  return fmaf(e, ENT ? fmaf(vmax(t, kFloor), r.k1, r.k0) : r.k0, add);
+  return fmaf(e, ENT ? fmaf(vmax(t, kGradFloor), r.k1, r.k0) : r.k0, add);
 }
 
 // The rows' sums come from the forward pass, so this is one read and one write: dx_j = e_j (k0 + k1 t_j), and the

@@ -298,6 +298,30 @@ def test_rows_without_upstream_gradient_get_zeros_whatever_they_hold(layout):
     assert (grad == 0).all()
 
 
+# upstream gradients as a grown loss scale makes them: impossible and far classes still get 0
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["volume", "last", "rows", "many", "turned"])
+def test_large_gradients_of_the_entropy_leave_impossible_classes_alone(layout, dtype):
+    from depth_estimation_amd.distribution import log_probs
+    from oracle import distribution as ref
+    shape = {"rows": (24, 4500), "many": (8256, 40), "turned": (8256, 64)}.get(layout, (2, 70, 4, 6))
+    x, g = _make(layout, shape, dtype)
+    x.movedim(1, -1)[..., 5:] = -INF
+    x.movedim(1, -1)[..., 4] = torch.finfo(dtype).min
+    rows = shape[:1] + shape[2:]
+    idx = torch.zeros(rows, dtype=torch.long)
+    gl, gh = torch.randn(rows, generator=g) * 1e9, torch.randn(rows, generator=g) * 1e12
+    xg = _gpu(x, "last" if layout == "last" else "volume").requires_grad_(True)
+    out = log_probs(xg, idx.cuda())
+    grad, = torch.autograd.grad([out.log_prob, out.entropy], xg, [gl.cuda(), gh.cuda()])
+    got, xl = _last(grad.cpu()), _last(x)
+    assert (got[..., 4:] == 0).all()
+    want = ref.log_probs_grad(xl, idx, 1.0, gl, gh)
+    # each part of the gradient is at most (|gl| + |gh| (|log p| + H)) large; p (|log p|) <= 1/e, H <= ln 4 here
+    size = gl.double().abs() + 3 * gh.double().abs()
+    _close(got[..., :4], want[..., :4], _step(dtype)[0] * 1.01 * want[..., :4].abs() + 2 * _factor(4) * size[..., None], "grad")
+
+
 # ------------------------------------------------------------------------------- distillation
 
 def _teacher(rows, V, k, g, dtype=torch.float32, pad=True):
