@@ -267,11 +267,15 @@ __device__ __forceinline__ float wave_sum_all(float v) {
   return v;
 }
 
+// (x - m) scale + add, also where x - m alone leaves float32's range (halving is exact)
+__device__ __forceinline__ float scaled_difference(float x, float m, float scale, float add) {
+  return fmaf(0.5f * x - 0.5f * m, 2.f * scale, add);
+}
 // log p of a class of value x in a row of (m, ln s): -inf for an impossible class, also where the whole row
 // is impossible (ln s = -inf); NaN where the row holds NaN or z = +inf
 // (in base e: in base 2 the log-probability of a class at float32's lowest value would overflow)
 __device__ __forceinline__ float log_p(float x, float m, float ln_s, float scale) {
-  return (x * scale == -kInf && fabsf(x) == kInf && ln_s == ln_s) ? -kInf : fmaf(x - m, scale, -ln_s);
+  return (x * scale == -kInf && fabsf(x) == kInf && ln_s == ln_s) ? -kInf : scaled_difference(x, m, scale, -ln_s);
 }
 
 // ---- order keys --------------------------------------------------------------------------------
@@ -1004,7 +1008,7 @@ struct RowSums {
 };
 __device__ __forceinline__ float rest_term(const RowSums& r, float scale, float rr) {
   // log of the unlisted classes' probability
-  const float lp = fmaf(r.m_r - r.b, scale, logf(r.s_r) - r.ln_s);
+  const float lp = scaled_difference(r.m_r, r.b, scale, logf(r.s_r) - r.ln_s);
   return rr > 0.f ? rr * (logf(rr) - lp) : 0.f;
 }
 __device__ __forceinline__ float4 distill_stats(const RowSums& r, float c, float mass, float rr, bool alive) {
@@ -1999,6 +2003,9 @@ __global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S*
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------
+// Below 2^-120 a difference of two logits that leaves float32's range would not yet be a probability of 0; above 2^120
+// the factor of the exponents, scale log2 e, and twice the scale come near its end.
+constexpr float kLeastScale = 0x1p-120f, kMostScale = 0x1p120f;
 constexpr int64_t kMaxClasses = 1 << 28;   // the order keys hold 29 bits of index
 constexpr int64_t kMaxThreads = 0xffffffff; // of a launch
 constexpr int kWantWaves = 2048;           // 8 a compute unit: enough loads in flight
@@ -2032,7 +2039,7 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
                             : DW_DIST_INDEX64 | DW_DIST_LAST;
   if (d->flags & ~known) return DW_ERR_ARG;
   if ((d->flags & DW_DIST_TEACHER_BF16) && (d->flags & DW_DIST_TEACHER_F16)) return DW_ERR_ARG;
-  if (!(d->scale != 0.f) || !(d->scale - d->scale == 0.f)) return DW_ERR_ARG;  // zero, NaN, infinite
+  if (!(fabsf(d->scale) >= kLeastScale && fabsf(d->scale) <= kMostScale)) return DW_ERR_ARG;  // (nor NaN)
   const int64_t limit = (int64_t)1 << 40;
   if (d->outer > limit || d->inner > limit || (d->inner > 0 && d->outer > limit / d->inner)) return DW_ERR_SHAPE;
   if (d->outer * d->inner > ((int64_t)1 << 48) / d->classes) return DW_ERR_SHAPE;

@@ -12,7 +12,7 @@ They stand next to the disparity regression of `disparity.soft_argmin` (the refe
 
 Logits are float32, bfloat16 or float16; the class axis is `dim` (1, as in a (B, D, H, W) volume or a
 (rows, classes) matrix), and `scale * logits` are the log-weights: -1 for a cost volume, 1/T for a
-temperature.  Tensors in memory order, or with the class axis last in memory (torch's channels_last),
+temperature (of either sign, |scale| from 2^-120 to 2^120).  Tensors in memory order, or with the class axis last in memory (torch's channels_last),
 are read where they are; any other order is copied first.  Sums and results are float32, gradients
 have the type and the memory order of the logits.
 

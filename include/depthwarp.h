@@ -390,7 +390,7 @@ typedef struct dw_dist_desc {
   int64_t outer, classes, inner; /* 1 <= classes <= 2^28; outer or inner may be 0: nothing to do.  More rows than one
                                     launch takes (2^24 long ones, 2^32 of at most 2048 classes) are DW_ERR_SHAPE */
   int64_t entry_stride[3];       /* distillation: element strides of the teacher's list along outer, entry, inner */
-  float scale;                   /* finite, not 0 */
+  float scale;                   /* of either sign, 2^-120 <= |scale| <= 2^120; anything else is DW_ERR_ARG */
   int32_t dtype;                 /* of the logits and their gradient: DW_DTYPE_* */
   int32_t entries;               /* top classes wanted (0..64, at most classes) / entries of the teacher's list (1..64) */
   int32_t flags;                 /* DW_DIST_* */

@@ -107,6 +107,15 @@ def test_abi_refuses_bad_problems_before_touching_a_pointer(kw, code):
     assert lib.dw_distill_bwd(d, None, None, None, None, None, None, None) == code
 
 
+@pytest.mark.parametrize("scale", [3e38, -3e38, 2.0 ** 121, 2.0 ** -121, -1e-37, 1e-45])
+def test_abi_refuses_scales_whose_exponents_leave_float32(scale):
+    # (3e38 log2 e is infinite: every row's maximum would give 0 * inf)
+    test_abi_refuses_bad_problems_before_touching_a_pointer(dict(scale=scale), -5)
+    lib = _lib.lib()
+    for ok in (2.0 ** 120, -(2.0 ** -120)):
+        assert lib.dw_log_probs_workspace_bytes(_desc(scale=ok)) == 0 == lib.dw_distill_workspace_bytes(_desc(scale=ok))
+
+
 def test_abi_refuses_null_pointers_small_workspaces_and_misfit_lists():
     lib = _lib.lib()
     x = 256   # stands for a device pointer: nothing is launched

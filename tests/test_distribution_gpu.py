@@ -322,6 +322,42 @@ def test_large_gradients_of_the_entropy_leave_impossible_classes_alone(layout, d
     _close(got[..., :4], want[..., :4], _step(dtype)[0] * 1.01 * want[..., :4].abs() + 2 * _factor(4) * size[..., None], "grad")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V", [(4, 100), (4, 9000), (8256, 40), (8256, 64)])
+def test_logits_and_scales_at_the_ends_of_their_range(n, V, dtype):
+    """Differences of logits beyond float32, whose product with the scale lies within it."""
+    from depth_estimation_amd.distribution import distill_loss, log_probs
+    from oracle import distribution as ref
+    f = _factor(V)
+    for scale, big in ((0.5, 3e38), (-0.25, 3e38), (2.0 ** -120, 3e38), (-(2.0 ** 120), 1e-36)):
+        x, _ = _make("rows", (n, V), dtype, seed=V)
+        x = (x.float() * (abs(1 / scale) if abs(scale) < 1e-3 or abs(scale) > 1e3 else 1)).to(dtype)
+        x[0] = -big if scale > 0 else big                # far below the best class
+        x[0, 7] = -x[0, 0]
+        x[1] = x[0, 0]
+        x[1, 7:9] = x[0, 7]
+        idx = _index((n,), V, 1, holes=False)
+        idx[0], idx[1] = 3, 7
+        out = log_probs(x.cuda(), idx.cuda(), scale=scale, top=10)
+        want = ref.log_probs(x, idx, scale, 10)
+        z = x.double() * scale
+        t = z.amax(-1, keepdim=True) - z
+        near = torch.where(t < 40, t, 0.0).amax(-1)
+        _close(out.log_prob, want["log_prob"], f + 4 * U * t.gather(-1, idx[:, None])[:, 0], "log_prob")
+        _close(out.entropy, want["entropy"], (f + 4 * U * near) * (1 + want["entropy"]), "entropy")
+        assert torch.equal(out.top_index.cpu(), want["top_index"])
+        _close(out.top_log_prob, want["top_log_prob"], f + 4 * U * t.gather(-1, want["top_index"].long()), "top_log_prob")
+        # listed classes far below the best one, and a rest far below them
+        ti = torch.tensor([[3, 4], [7, 8]])[torch.arange(n) % 2].clone()
+        ti[0, 1] = 7
+        tv = torch.full((n, 2), math.log(0.25))
+        loss = distill_loss(x.cuda(), tv.cuda(), ti.cuda(), scale=scale)
+        w = ref.distill(x, tv, ti, scale)
+        t_rest = t.masked_fill(ref._listed(ti, torch.ones_like(ti, dtype=torch.bool), V), INF).amin(-1)
+        tol = (f + 12 * U) * w["size"] + 4 * U * (t.gather(-1, ti).amax(-1) + t_rest)
+        _close(loss, w["loss"], tol, "loss")
+
+
 # ------------------------------------------------------------------------------- distillation
 
 def _teacher(rows, V, k, g, dtype=torch.float32, pad=True):
