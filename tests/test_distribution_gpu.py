@@ -561,6 +561,11 @@ def test_a_teachers_list_trains_a_student(layout, dtype):
     assert disp.shape == loss.shape and disp.isfinite().all()
 
 
+def test_the_documented_loss():
+    from tests.test_distribution import check_documented_loss
+    check_documented_loss("cuda")
+
+
 # ------------------------------------------------------------- strides, refusals, bytes left alone
 
 def test_strided_inputs_equal_their_copies():
