@@ -939,6 +939,75 @@ def test_traced_calls_give_the_eager_results():
     assert torch.equal(want, got) and torch.equal(wi, gi) and torch.equal(gw, gg)
 
 
+# gradients of 128 MB and more of every family: flat tiles (rows of whole 16-byte pieces or not; the last tile overlaps
+# the one before), planes, rows.  Tiles store an aligned gradient past the caches, another one not; rows always.
+@pytest.mark.parametrize("shape,dtype", [((1, 193, 368101, 1), 2), ((1, 200, 368101, 1), 1), ((1, 97, 368101, 1), 0),
+                                         ((1, 100, 368101, 1), 0), ((3, 64, 192, 1024), 0), ((1100, 32771, 1, 1), 0)])
+def test_large_gradients_have_the_same_bits_however_they_are_stored(shape, dtype):
+    import ctypes as C
+    from depth_estimation_amd import _lib
+    from oracle import distribution as ref
+    lib = _lib.lib()
+    td = DTYPES[dtype]
+    last = shape[0] == 1
+    outer, V, inner = shape[0], shape[1], shape[2] * shape[3]
+    rows, k = outer * inner, 3
+    assert rows * V * td.itemsize >= 128 << 20
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(rows * V, generator=g, device="cuda").mul_(2).to(td)
+    idx = torch.randint(-1, V, (rows,), generator=g, device="cuda")
+    ti = torch.randint(-1, V, (rows * k,), generator=g, device="cuda")
+    tv = torch.randn(rows * k, generator=g, device="cuda") - 3
+    up = torch.rand(rows, generator=g, device="cuda") - 0.5
+    d = _lib.DwDistDesc(outer, V, inner, (k * inner, 1, k) if last else (k * inner, inner, 1), -1.0, dtype, k,
+                        _lib.DW_DIST_INDEX64 | (_lib.DW_DIST_LAST if last else 0))
+    lp_d = _lib.DwDistDesc(outer, V, inner, (0, 0, 0), -1.0, dtype, 0, d.flags)
+    st = torch.cuda.current_stream().cuda_stream
+    ent, s3, s4 = (torch.empty(rows * n, device="cuda") for n in (1, 3, 4))
+    loss = torch.empty(rows, device="cuda")
+    nb = max(lib.dw_log_probs_workspace_bytes(C.byref(lp_d)), lib.dw_distill_workspace_bytes(C.byref(d)))
+    ws = torch.empty(max(nb, 1), dtype=torch.uint8, device="cuda")
+    assert lib.dw_log_probs_fwd(C.byref(lp_d), x.data_ptr(), idx.data_ptr(), None, ent.data_ptr(), None, None, s3.data_ptr(),
+                                ws.data_ptr(), nb, st) == 0
+    assert lib.dw_distill_fwd(C.byref(d), x.data_ptr(), tv.data_ptr(), ti.data_ptr(), loss.data_ptr(), s4.data_ptr(),
+                              ws.data_ptr(), nb, st) == 0
+    guard = 256 // td.itemsize
+
+    def gradient(distill, shift):
+        out = torch.full((rows * V + 2 * guard,), 55.0, dtype=td, device="cuda")
+        at = out.data_ptr() + (guard + shift) * td.itemsize
+        assert (at % 128 == 0) == (shift == 0)
+        if distill:
+            rc = lib.dw_distill_bwd(C.byref(d), x.data_ptr(), tv.data_ptr(), ti.data_ptr(), s4.data_ptr(), up.data_ptr(), at, st)
+        else:
+            rc = lib.dw_log_probs_bwd(C.byref(lp_d), x.data_ptr(), idx.data_ptr(), s3.data_ptr(), up.data_ptr(), up.data_ptr(),
+                                      at, st)
+        assert rc == 0
+        assert (out[:guard + shift] == 55).all() and (out[guard + shift + rows * V:] == 55).all()
+        return out[guard + shift:guard + shift + rows * V]
+
+    # rows of both ends, as the oracle has them
+    near = torch.cat([torch.arange(70), torch.arange(rows - 70, rows)])
+    near_x, near_i = (x.view(rows, V) if last else x.view(outer, V, inner).movedim(1, -1).reshape(rows, V))[near].cpu(), idx[near].cpu()
+    view = (lambda t: t.view(rows, k)) if last else (lambda t: t.view(outer, k, inner).movedim(1, -1).reshape(rows, k))
+    u = up[near].cpu()
+    half, tiny = _step(td)
+    z = near_x.double() * -1.0
+    t = (z.amax(-1, keepdim=True) - z).clamp_max(60)
+    w_ds = ref.distill(near_x, view(tv)[near].cpu(), view(ti)[near].cpu(), -1.0)
+    w_lp = ref.log_probs_grad(near_x, near_i, -1.0, u, u)
+    for distill in (False, True):
+        a, b = gradient(distill, 0), gradient(distill, 3)
+        assert torch.equal(a, b)
+        want = w_ds["grad"] * u.double()[:, None] if distill else w_lp
+        # (the parts' sizes: (p Q + q + r p / P) |u|; (p + hit + p (|log p| + H + 2)) |u|, at most 4 |u|)
+        size = w_ds["grad_size"] if distill else torch.full_like(want, 4.0)
+        tol = half * 1.01 * want.abs() + 2 * (_factor(V) + 8 * U + 8 * U * t) * size * u.double().abs()[:, None] + tiny
+        got = (a.view(rows, V) if last else a.view(outer, V, inner).movedim(1, -1).reshape(rows, V))[near]
+        _close(got, want, tol, "grad")
+        del a, b, got
+
+
 def _run_of_both(x, idx, t, ti):
     from depth_estimation_amd.distribution import distill_loss, log_probs
     o = log_probs(x, idx, scale=-2.0, top=3)
