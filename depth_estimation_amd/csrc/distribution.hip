@@ -2008,13 +2008,22 @@ __global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S*
 constexpr float kLeastScale = 0x1p-120f, kMostScale = 0x1p120f;
 constexpr int64_t kMaxClasses = 1 << 28;   // the order keys hold 29 bits of index
 constexpr int64_t kMaxThreads = 0xffffffff; // of a launch
-constexpr int kWantWaves = 2048;           // 8 a compute unit: enough loads in flight
+// Waves a launch should have, 8 a compute unit: long rows are split, and the waves of a tile's block share its classes, until
+// there are so many.  For rows the second launch of a split is what decides (forward + backward, us; 1024 instead of 2048 in
+// brackets): 64 x 32768 bf16 top 5 12.3 + 4.4 (12.4 + 4.5, 512: 12.8 + 5.3), 600 x 32768 bf16 13.0 + 15.5 (13.2 + 15.5, 4096:
+// 17.2 + 14.2); it loses forward where 1024 leaves rows whole, 333 x 50001 bf16 17.3 + 16.9 (13.6 + 18.7),
+// 1500 x 4096 bf16 12.3 + 7.2 (7.5 + 7.9).
+constexpr int kWantWaves = 2048;
 // A gradient from this size on is stored past the caches.  It would fill half of the 256 MB last-level cache or
 // more, and what comes next would have to wait while that is written back: the next forward pass over 4096 x
 // 32768 bf16 takes 54 us instead of 80, over 4 x 256 x 192 x 640 bf16 66 instead of 86; the backward pass
-// itself 83 either way.  Smaller ones stay where the next operator finds them.  It takes whole 128-byte lines: rows
-// are written 1 KB at a time, flat tiles in one stretch, planes only where 64 pixels are whole lines (255 bins of 131 x 641
-// pixels bf16: 165 us instead of 96), turned rows never (193 classes f16: 45 instead of 29).
+// itself 83 either way.  Smaller ones stay where the next operator finds them.  Where a wave writes half a line and
+// the other half comes much later it costs more than it saves: planes take it only where 64 pixels are whole
+// lines (255 bins of 131 x 641 pixels bf16: 165 us instead of 96), turned rows never (193 classes f16: 45 instead of 29).
+// Flat tiles are written in one stretch.  So are rows, 1 KB at a time, and whether they begin and end with a line
+// decides little (backward alone, then forward and backward in turn; ordinary stores in brackets): 2048 x 49984 bf16, whole
+// lines, 85 (84), 115 (132); 2048 x 50001 95 (91), 130 (145); 1100 x 50001 f32 100 (97), 121 (146); 40000 x 3001 f16 109 (106),
+// 159 (164); 40000 x 3008 92 (90), 146 (145).
 constexpr int64_t kPastBytes = (int64_t)128 << 20;
 constexpr size_t kLdsBudget = 152 * 1024;  // of a block, of the compute unit's 160 KB
 constexpr int kMostFlat = 64 * 1024;       // of a flat tile
@@ -2063,6 +2072,12 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
   P.last = (d->flags & DW_DIST_LAST) || d->inner == 1;
   const int64_t tiles = P.last ? (p.rows + 63) / 64 : d->outer * ((d->inner + 63) / 64);
   const int esize = d->dtype == DW_DTYPE_F32 ? 4 : 2;
+  // Planes are tiles.  Rows are from 128 tiles on and up to 2048 classes (forward + backward, us; the other family in brackets).
+  // 8200 rows bf16: 40 classes 4.3 + 4.5 (12.4 + 11.5), with the top 8 6.1 + 4.5 (39.9 + 11.2), 512 classes 7.4 + 8.5 (12.5 + 12.1).
+  // 3000 classes are rows, 18.2 + 24.2 (21.8 + 40.7).  Between, the two are near each other forward and rows win backward: 16400 x
+  // 1000 bf16 17.3 + 22.8 (19.9 + 19.5), x 2048 26.0 + 40.5 (20.8 + 26.5; with the top 8 53.9, 43.7; distillation 34.7 + 41.3, 29.2
+  // + 29.2).  Fewer rows than that are rows though tiles of up to 512 classes take no longer: 4100 x 40 8.2 + 7.8 (4.2 + 4.5),
+  // top 8 24.4 (6.0), x 512 8.3 + 8.1 (7.0 + 7.4); 2100 x 1000 6.9 + 6.6 (10.1 + 11.2).
   P.tile = !P.last || (p.V <= 2048 && tiles * 4 >= kWantWaves / 4);
   if (P.tile) {
     const int row = p.V * esize;
@@ -2102,6 +2117,9 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
     P.grid = (unsigned)tiles;
     return DW_OK;
   }
+  // One wave a row up to 4096 classes, four above (forward + backward, us; the other in brackets): 4000 rows bf16 of 4000 classes
+  // 11.8 + 13.7 (17.5 + 17.5), 1000 rows 10.6 + 6.3 (7.8 + 7.9: one launch), 4000 of 8192 21.2 + 25.6 (18.3 + 27.1), f32
+  // 27.7 + 49.1 (29.2 + 52.6), 16000 of 6000 bf16 63.9 + 68.8 (45.2 + 81.2).
   P.nt = p.V <= 2 * kWaveTile ? 64 : 256;
   const int64_t block_tile = (int64_t)P.nt * 32;
   // few rows: several blocks share one, until the chip has its waves or a block is down to one tile
