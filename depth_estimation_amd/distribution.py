@@ -16,6 +16,10 @@ temperature (of either sign, |scale| from 2^-120 to 2^120).  Tensors in memory o
 are read where they are; any other order is copied first.  Sums and results are float32, gradients
 have the type and the memory order of the logits.
 
+A volume in memory order is read by a block for every 64 pixels.  One of few pixels and thousands of classes
+leaves most of the chip idle that way: give it with the class axis last in memory (1 x 32768 x 64 bfloat16: 148 us
+in memory order, 8 us that way, 11 us for the copy).
+
 Calls can be captured into a graph, backward passes with them; workspaces belong to the call, so graphs do
 not share them.  While a backward pass is captured, no eager graph of the same leaves may be alive (torch
 ends the process): drop the eager results first, or capture `torch.autograd.grad`.
