@@ -14,7 +14,7 @@ Logits are float32, bfloat16 or float16; the class axis is `dim` (1, as in a (B,
 (rows, classes) matrix), and `scale * logits` are the log-weights: -1 for a cost volume, 1/T for a
 temperature (of either sign, |scale| from 2^-120 to 2^120).  Tensors in memory order, or with the class axis last in memory (torch's channels_last),
 are read where they are; any other order is copied first.  Sums and results are float32, gradients
-have the type and the memory order of the logits.
+have the type and the memory order of the logits (memory order, where those were copied).
 
 A volume in memory order is read by a block for every 64 pixels.  One of few pixels and thousands of classes
 leaves most of the chip idle that way: give it with the class axis last in memory (1 x 32768 x 64 bfloat16: 148 us
@@ -451,7 +451,9 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
     Returns the loss of every row (the shape of `logits` without `dim`, float32), differentiable with
     respect to `logits`, once; the teacher is a constant and must not require a gradient.  A row
     without entries has loss and gradient 0.  A class listed twice counts with both entries.  The loss
-    is +inf where the teacher lists a class the student has at -inf.
+    is +inf where the teacher gives a listed class probability and the student has it at -inf.  The rest is
+    different: where the student has no possible class outside the list, the teacher's remaining
+    probability adds nothing to the loss and to the gradient, as if there were no further class.
     """
     if not (logits.is_cuda and teacher.device == logits.device == teacher_index.device):
         _check_device(logits, teacher=teacher, teacher_index=teacher_index)
