@@ -2006,7 +2006,9 @@ __global__ __launch_bounds__(NT, 4) void ds_row_bwd(Prob p, const typename T::S*
 // Below 2^-120 a difference of two logits that leaves float32's range would not yet be a probability of 0; above 2^120
 // the factor of the exponents, scale log2 e, and twice the scale come near its end.
 constexpr float kLeastScale = 0x1p-120f, kMostScale = 0x1p120f;
-constexpr int64_t kMaxClasses = 1 << 28;   // the order keys hold 29 bits of index
+// Bytes inside a row are counted in 32 bits (2^30 for float32), classes in an int, which also has to hold the ones a
+// block would step to behind the last.
+constexpr int64_t kMaxClasses = 1 << 28;
 constexpr int64_t kMaxThreads = 0xffffffff; // of a launch
 // Waves a launch should have, 8 a compute unit: long rows are split, and the waves of a tile's block share its classes, until
 // there are so many.  For rows the second launch of a split is what decides (forward + backward, us; 1024 instead of 2048 in
