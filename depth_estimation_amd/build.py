@@ -59,8 +59,8 @@ def build(force: bool = False, verbose: bool = True) -> Path:
     if not force and not stale():
         return LIB
     common = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-ffp-contract=off", "-fno-slp-vectorize",
-              # the packed fp32 instructions hipcc forms by itself have given wrong results on gfx950
-              # boards now and then: plain ones only
+              # a precaution: some forms of the packed fp32 instructions hipcc makes by itself are not trusted on
+              # gfx950, and tests would not show it reliably.  No kernel here is known to have gone wrong with them.
               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
               "-fPIC", "-fvisibility=hidden", "-DDW_BUILD", f"-I{ROOT / 'include'}", f"-I{CSRC}"]
     objdir = ROOT / "build" / "obj"

@@ -771,7 +771,8 @@ __device__ __forceinline__ void settle(float (&v)[32], float far, int n) {
 // A thread a row keeps the whole soft-max in its own registers: a block a row, as in the row kernels, would spend a
 // reduction over 64 lanes on every few hundred classes.  The waves of a block split the classes where there are
 // too few rows to fill the chip, and join through LDS.  Loads of the next 32 classes are issued before the ones at
-// hand are worked on.  12 x 64 x 96 x 320 bf16 (47 MB): 15.8 us, 3.0 TB/s, the vector pipe; 1 x 256 x 256 x 512 f32 with
+// hand are worked on.  12 x 64 x 96 x 320 bf16 (47 MB): 15.2 us, 3.1 TB/s, vector instructions in
+// 63 % of the busy cycles, so neither alone is the bound; 1 x 256 x 256 x 512 f32 with
 // the top 8 (134 MB): 34 us, 4.0 TB/s; 4 x 193 x 96 x 320 f16, classes last (47 MB): 18.1 us.
 // K: top classes kept in registers as keys of kind P (0: none).  More than K wanted: further passes over the data,
 // each for the next K below the last key of the pass before.
