@@ -5,7 +5,7 @@
 // training steps are bound by it: a node written in Python runs in the autograd engine's own thread, where the
 // interpreter's lock and cold caches took about half of such a step (80 to 90 us, 4 x 64 x 4 x 4).
 //
-// The library's functions come from Python as addresses, descriptors as their words: which build of the library is in
+// The library's functions come from Python as addresses, what a call has to know as a list of words: which build of the library is in
 // use, and what the shapes and types decide, is settled there (distribution.py).  These calls launch by pointer, so
 // nothing that records or replaces tensor operations sees more of them than their outputs being made: distribution.py
 // calls the registered operators wherever something of the kind watches.
@@ -82,27 +82,26 @@ std::vector<int64_t> with(at::IntArrayRef rows, int64_t at, int64_t n) {
   return s;
 }
 
-// A descriptor by value: a call that is kept for later holds no address of this process.
-dw_dist_desc descriptor(at::IntArrayRef words) {
-  dw_dist_desc d;
-  static_assert(sizeof d % sizeof(int64_t) == 0);
-  TORCH_CHECK(words.size() * sizeof(int64_t) == sizeof d, "descriptor: expected ", sizeof d / sizeof(int64_t), " words");
-  std::memcpy(&d, words.data(), sizeof d);
-  return d;
-}
-// What the backward pass has to know travels with the node as its bytes.
-struct Kept {
+// What a call has to know, by value (a call that is kept for later holds no address of this process): the words of this
+// struct.  They travel with the node to the backward pass.
+struct Call {
   dw_dist_desc desc;
-  int64_t dim, layout, list_layout;
+  int64_t nbytes, dim, top, layout, list_layout;
 };
-void keep(AutogradContext* ctx, const dw_dist_desc& desc, int64_t dim, int64_t layout, int64_t list_layout) {
-  const Kept k{desc, dim, layout, list_layout};
-  ctx->saved_data["call"] = std::string(reinterpret_cast<const char*>(&k), sizeof k);
+Call call_of(at::IntArrayRef words) {
+  Call c;
+  static_assert(sizeof c % sizeof(int64_t) == 0);
+  TORCH_CHECK(words.size() * sizeof(int64_t) == sizeof c, "expected ", sizeof c / sizeof(int64_t), " words, got ", words.size());
+  std::memcpy(&c, words.data(), sizeof c);
+  return c;
 }
-Kept kept(AutogradContext* ctx) {
-  Kept k;
-  std::memcpy(&k, ctx->saved_data["call"].toStringRef().data(), sizeof k);
-  return k;
+void keep(AutogradContext* ctx, const Call& c) {
+  ctx->saved_data["call"] = std::string(reinterpret_cast<const char*>(&c), sizeof c);
+}
+Call kept(AutogradContext* ctx) {
+  Call c;
+  std::memcpy(&c, ctx->saved_data["call"].toStringRef().data(), sizeof c);
+  return c;
 }
 // The gradients are differentiable once.  Where a pass builds a graph of itself, using that graph is an error.
 Tensor once(Tensor grad) {
@@ -116,26 +115,26 @@ Tensor once(Tensor grad) {
 
 struct LogProbs : torch::autograd::Function<LogProbs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& given,
-                               at::IntArrayRef words, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout,
-                               bool train) {
-    const dw_dist_desc desc = descriptor(words);
-    const Tensor x = in_place(logits, layout), index_in = given ? *given : Tensor(), index = contiguous(index_in);
+                               at::IntArrayRef words, at::IntArrayRef rows, bool train) {
+    const Call c = call_of(words);
+    const int64_t top = c.top;
+    const Tensor x = in_place(logits, c.layout), index_in = given ? *given : Tensor(), index = contiguous(index_in);
     const c10::OptionalDeviceGuard guard(x.device());
     const auto f32 = x.options().dtype(at::kFloat).memory_format(std::nullopt);
     Tensor ent = at::empty(rows, f32), lp, stats, top_lp, top_idx;
     if (index.defined()) lp = at::empty(rows, f32);
     if (train) stats = at::empty(with(rows, rows.size(), 3), f32);
-    if (top && layout == kLast) {  // the kernels write the list of a row together, too
-      top_lp = at::empty(with(rows, rows.size(), top), f32).movedim(-1, dim);
-      top_idx = at::empty(with(rows, rows.size(), top), f32.dtype(at::kInt)).movedim(-1, dim);
+    if (top && c.layout == kLast) {  // the kernels write the list of a row together, too
+      top_lp = at::empty(with(rows, rows.size(), top), f32).movedim(-1, c.dim);
+      top_idx = at::empty(with(rows, rows.size(), top), f32.dtype(at::kInt)).movedim(-1, c.dim);
     } else if (top) {
-      top_lp = at::empty(with(rows, dim, top), f32);
-      top_idx = at::empty(with(rows, dim, top), f32.dtype(at::kInt));
+      top_lp = at::empty(with(rows, c.dim, top), f32);
+      top_idx = at::empty(with(rows, c.dim, top), f32.dtype(at::kInt));
     }
-    const Tensor ws = workspace(x, nbytes);
-    check(lib.log_probs_fwd(&desc, data(x), data(index), data<float>(lp),
+    const Tensor ws = workspace(x, c.nbytes);
+    check(lib.log_probs_fwd(&c.desc, data(x), data(index), data<float>(lp),
                             data<float>(ent), data<float>(top_lp), data<int32_t>(top_idx), data<float>(stats), data(ws),
-                            nbytes, stream_of(x)),
+                            c.nbytes, stream_of(x)),
           "dw_log_probs_fwd");
     variable_list out;
     if (index.defined()) out.push_back(lp);
@@ -148,7 +147,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
       ctx->set_materialize_grads(false);
       if (top) ctx->mark_non_differentiable({top_lp, top_idx});
       ctx->save_for_backward({logits, index_in, stats});
-      keep(ctx, desc, dim, layout, kInOrder);
+      keep(ctx, c);
     }
     return out;
   }
@@ -158,13 +157,13 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     Tensor g_lp, g_ent;
     if (index.defined()) g_lp = contiguous(g[0]);
     g_ent = contiguous(g[index.defined() ? 1 : 0]);
-    variable_list out(9);
+    variable_list out(5);
     if (!g_lp.defined() && !g_ent.defined()) return out;
     const c10::OptionalDeviceGuard guard(saved[0].device());
-    const Kept k = kept(ctx);
-    const Tensor x = saved_in_place(saved[0], k.layout, k.dim);
+    const Call c = kept(ctx);
+    const Tensor x = saved_in_place(saved[0], c.layout, c.dim);
     Tensor grad = at::empty_like(x);
-    check(lib.log_probs_bwd(&k.desc, data(x), data(index), data<float>(stats), data<float>(g_lp), data<float>(g_ent),
+    check(lib.log_probs_bwd(&c.desc, data(x), data(index), data<float>(stats), data<float>(g_lp), data<float>(g_ent),
                             data(grad), stream_of(x)),
           "dw_log_probs_bwd");
     out[0] = once(grad);
@@ -174,36 +173,35 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
 
 struct Distill : torch::autograd::Function<Distill> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher_in, const Tensor& index_in,
-                        at::IntArrayRef words, int64_t nbytes, at::IntArrayRef rows, int64_t dim, int64_t layout, int64_t list_layout,
-                        bool train) {
-    const dw_dist_desc desc = descriptor(words);
-    const Tensor x = in_place(logits, layout), teacher = in_place(teacher_in, list_layout),
-                 index = in_place(index_in, list_layout);
+                        at::IntArrayRef words, at::IntArrayRef rows, bool train) {
+    const Call c = call_of(words);
+    const Tensor x = in_place(logits, c.layout), teacher = in_place(teacher_in, c.list_layout),
+                 index = in_place(index_in, c.list_layout);
     const c10::OptionalDeviceGuard guard(x.device());
     const auto f32 = x.options().dtype(at::kFloat).memory_format(std::nullopt);
     Tensor loss = at::empty(rows, f32), stats;
     if (train) stats = at::empty(with(rows, rows.size(), 4), f32);
-    const Tensor ws = workspace(x, nbytes);
-    check(lib.distill_fwd(&desc, data(x), data(teacher), data(index),
-                          data<float>(loss), data<float>(stats), data(ws), nbytes, stream_of(x)),
+    const Tensor ws = workspace(x, c.nbytes);
+    check(lib.distill_fwd(&c.desc, data(x), data(teacher), data(index),
+                          data<float>(loss), data<float>(stats), data(ws), c.nbytes, stream_of(x)),
           "dw_distill_fwd");
     if (train) {
       ctx->set_materialize_grads(false);
       ctx->save_for_backward({logits, teacher_in, index_in, stats});
-      keep(ctx, desc, dim, layout, list_layout);
+      keep(ctx, c);
     }
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    variable_list out(10);
+    variable_list out(6);
     if (!g[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard guard(saved[0].device());
-    const Kept k = kept(ctx);
-    const Tensor x = saved_in_place(saved[0], k.layout, k.dim), teacher = saved_in_place(saved[1], k.list_layout, k.dim),
-                 index = saved_in_place(saved[2], k.list_layout, k.dim), stats = contiguous(saved[3]), up = contiguous(g[0]);
+    const Call c = kept(ctx);
+    const Tensor x = saved_in_place(saved[0], c.layout, c.dim), teacher = saved_in_place(saved[1], c.list_layout, c.dim),
+                 index = saved_in_place(saved[2], c.list_layout, c.dim), stats = contiguous(saved[3]), up = contiguous(g[0]);
     Tensor grad = at::empty_like(x);
-    check(lib.distill_bwd(&k.desc, data(x), data(teacher), data(index), data<float>(stats), data<float>(up), data(grad),
+    check(lib.distill_bwd(&c.desc, data(x), data(teacher), data(index), data<float>(stats), data<float>(up), data(grad),
                           stream_of(x)),
           "dw_distill_bwd");
     out[0] = once(grad);
@@ -212,22 +210,19 @@ struct Distill : torch::autograd::Function<Distill> {
 };
 
 // [log_prob if there is an index, entropy, and the two top lists if top > 0]
-std::vector<Tensor> log_probs(const Tensor& logits, const std::optional<Tensor>& index, at::IntArrayRef desc, int64_t nbytes,
-                              at::IntArrayRef rows, int64_t dim, int64_t top, int64_t layout) {
+std::vector<Tensor> log_probs(const Tensor& logits, const std::optional<Tensor>& index, at::IntArrayRef call,
+                              at::IntArrayRef rows) {
   const bool train = logits.requires_grad() && at::GradMode::is_enabled();
-  return LogProbs::apply(logits, index, desc, nbytes, rows, dim, top, layout, train);
+  return LogProbs::apply(logits, index, call, rows, train);
 }
-Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, at::IntArrayRef desc, int64_t nbytes,
-               at::IntArrayRef rows, int64_t dim, int64_t layout, int64_t list_layout) {
+Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, at::IntArrayRef call, at::IntArrayRef rows) {
   const bool train = logits.requires_grad() && at::GradMode::is_enabled();
-  return Distill::apply(logits, teacher, index, desc, nbytes, rows, dim, layout, list_layout, train);
+  return Distill::apply(logits, teacher, index, call, rows, train);
 }
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(depthwarp, m) {
   m.def("_bind_distribution(int strerror, int lp_fwd, int lp_bwd, int ds_fwd, int ds_bwd) -> ()", &bind);
-  m.def("_log_probs_eager(Tensor logits, Tensor? index, int[] desc, int nbytes, int[] rows, int dim, int top, "
-        "int layout) -> Tensor[]", &log_probs);
-  m.def("_distill_eager(Tensor logits, Tensor teacher, Tensor index, int[] desc, int nbytes, int[] rows, int dim, "
-        "int layout, int list_layout) -> Tensor", &distill);
+  m.def("_log_probs_eager(Tensor logits, Tensor? index, int[] call, int[] rows) -> Tensor[]", &log_probs);
+  m.def("_distill_eager(Tensor logits, Tensor teacher, Tensor index, int[] call, int[] rows) -> Tensor", &distill);
 }

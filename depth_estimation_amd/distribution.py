@@ -72,14 +72,14 @@ def _eager():
 
 
 _PLAIN = (Tensor, torch.nn.Parameter)
+_modes, _is_tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
 
 
-def _watched(*tensors: Optional[Tensor]) -> bool:
+def _watched(a: Tensor, b: Optional[Tensor], c: Optional[Tensor] = None) -> bool:
     """Whether something records or replaces tensor operations (torch.compile, a dispatch mode such as make_fx's or a
     FakeTensorMode, torch.jit.trace, tensors of another class): it has to see the registered operators."""
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or torch._C._get_tracing_state() is not None
-            or any(type(t) not in _PLAIN for t in tensors if t is not None))
+    return (torch.compiler.is_compiling() or _modes() > 0 or _is_tracing() or type(a) not in _PLAIN
+            or (b is not None and type(b) not in _PLAIN) or (c is not None and type(c) not in _PLAIN))
 
 
 def _call(device: torch.device, fn, *args) -> None:
@@ -100,10 +100,16 @@ class _Plan(NamedTuple):
     dim: int
     rows: tuple        # shape without the class axis
     ref: object        # descriptor, for ctypes
-    words: tuple       # the same for C++
+    call: tuple        # for C++: the words of its Call -- descriptor, workspace, class axis, entries, layouts
     nbytes: int        # workspace
     top: int = 0
     list_layout: int = 0      # distillation: the same of the teacher's tensors (_COPY where they have no common order)
+
+
+def _plan(layout: int, dim: int, shape, descriptor, top: int = 0, list_layout: int = 0) -> _Plan:
+    ref, words, nbytes = descriptor
+    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref,
+                 words + (nbytes, dim, top, layout, list_layout), nbytes, top, list_layout)
 
 
 _IN_PLACE, _LAST, _COPY = 0, 1, 2
@@ -189,8 +195,8 @@ def _make_lp_plan(shape, stride, dtype, index_dtype, index_shape, dim: int, scal
     dim = _lp_check(shape, dtype, index_dtype, index_shape, dim, scale, top)
     layout = _layout(shape, stride, dim)
     flags = 0 if index_dtype is None else _INDEX_FLAGS[index_dtype]
-    ref, words, nbytes = _descriptor("dw_log_probs_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, top, flags)
-    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, words, nbytes, top)
+    return _plan(layout, dim, shape, _descriptor("dw_log_probs_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, top,
+                                                 flags), top)
 
 
 _lp_plan = functools.lru_cache(maxsize=512)(_make_lp_plan)
@@ -332,7 +338,7 @@ def log_probs(logits: Tensor, index: Optional[Tensor] = None, *, dim: int = 1, s
         lp, ent, top_lp, top_idx, _ = _log_probs_op(logits, index, dim, scale, top)
         return LogProbs(None if index is None else lp, ent, top_lp if top else None, top_idx if top else None)
     plan = _plan_of(logits, index, dim, scale, top)
-    out = _eager()[0](logits, index, plan.words, plan.nbytes, plan.rows, plan.dim, top, plan.layout)
+    out = _eager()[0](logits, index, plan.call, plan.rows)
     if index is None:
         return LogProbs(None, *out) if top else LogProbs(None, out[0], None, None)
     return LogProbs(*out) if top else LogProbs(*out, None, None)
@@ -363,8 +369,8 @@ def _make_ds_plan(shape, stride, dtype, t_shape, t_stride, t_dtype, i_shape, i_s
     strides = (k * inner, 1, k) if list_layout == _LAST else (k * inner, inner, 1)
     layout = _layout(shape, stride, dim)
     flags = _INDEX_FLAGS[i_dtype] | _TEACHER_FLAGS[t_dtype] | (_lib.DW_DIST_RENORMALISE if renormalise else 0)
-    ref, words, nbytes = _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k, flags, strides)
-    return _Plan(layout, dim, tuple(shape[:dim]) + tuple(shape[dim + 1:]), ref, words, nbytes, list_layout=list_layout)
+    return _plan(layout, dim, shape, _descriptor("dw_distill_workspace_bytes", shape, dim, layout == _LAST, dtype, scale, k,
+                                                 flags, strides), list_layout=list_layout)
 
 
 _ds_plan = functools.lru_cache(maxsize=512)(_make_ds_plan)
@@ -465,5 +471,4 @@ def distill_loss(logits: Tensor, teacher: Tensor, teacher_index: Tensor, *, dim:
                         teacher_index.dtype, dim, scale)
         return _distill_op(logits, teacher, teacher_index, dim, scale, renormalise)[0]
     plan = _ds_plan_of(logits, teacher, teacher_index, dim, scale, renormalise)
-    return _eager()[1](logits, teacher, teacher_index, plan.words, plan.nbytes, plan.rows, plan.dim, plan.layout,
-                       plan.list_layout)
+    return _eager()[1](logits, teacher, teacher_index, plan.call, plan.rows)
