@@ -1014,6 +1014,8 @@ __device__ __forceinline__ float4 distill_stats(const RowSums& r, float c, float
   if (r.s_r != 0.f) {
     st.x = r.m_r;
     st.y = mass * exp2_((r.m_r - r.b) * c) / r.s - rr / r.s_r;
+  } else {
+    st.y = 0.f * (r.s + mass);  // 0 for classes that are all impossible; NaN where a listed class or the list holds one
   }
   st.w = mass / r.s;
   return st;

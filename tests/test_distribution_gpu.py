@@ -481,6 +481,25 @@ def test_distill_lists_and_masks_that_go_to_the_limit(layout, dtype, renormalise
     _check_distill(-xs, vs, ids, lay, -1.0, renormalise)
 
 
+@pytest.mark.parametrize("layout", ["volume", "last", "rows", "many", "turned"])
+def test_nan_reaches_the_gradient_of_impossible_classes(layout):
+    # nothing unlisted is possible, and a listed class (or its teacher's value) is NaN: the whole row is
+    n, V, k = {"rows": (96, 4500, 3), "many": (8256, 40, 3), "turned": (8256, 64, 3)}.get(layout, (96, 70, 3))
+    x, g = _make(layout, (n, V), torch.float32)
+    val, idx = _teacher((n,), V, k, g, pad=False)
+    idx[:8] = torch.arange(k)
+    x[:8, k:] = -INF
+    x[0, 1] = float("nan")
+    x[1, 2] = INF
+    val[2, 0] = float("nan")
+    x[3, 0] = -INF
+    xs, vs, ids, lay = x, val, idx, "rows"
+    if layout in ("volume", "last"):
+        xs, vs, ids, lay = x.view(2, 6, 8, V).movedim(-1, 1).contiguous(), val.view(2, 6, 8, k), idx.view(2, 6, 8, k), layout
+    for renormalise in (False, True):
+        _check_distill(xs, vs, ids, lay, 1.0, renormalise)
+
+
 def test_duplicated_classes_sum_before_they_are_rounded():
     # the gradient of a class listed twice is p Q - (q1 + q2), rounded once: against the list with one entry
     from depth_estimation_amd.distribution import distill_loss
