@@ -773,7 +773,7 @@ __device__ __forceinline__ void settle(float (&v)[32], float far, int n) {
 // too few rows to fill the chip, and join through LDS.  Loads of the next 32 classes are issued before the ones at
 // hand are worked on.  12 x 64 x 96 x 320 bf16 (47 MB): 15.2 us, 3.1 TB/s, vector instructions in
 // 63 % of the busy cycles, so neither alone is the bound; 1 x 256 x 256 x 512 f32 with
-// the top 8 (134 MB): 34 us, 4.0 TB/s; 4 x 193 x 96 x 320 f16, classes last (47 MB): 18.1 us.
+// the top 8 (134 MB): 34 us, 4.0 TB/s; 4 x 193 x 96 x 320 f16, classes last (47 MB): 17.8 us.
 // K: top classes kept in registers as keys of kind P (0: none).  More than K wanted: further passes over the data,
 // each for the next K below the last key of the pass before.
 // Turning rows and keeping their lists takes up to 180 registers: those blocks have at most 8 waves, so that they get

@@ -20,6 +20,9 @@ A volume in memory order is read by a block for every 64 pixels.  One of few pix
 leaves most of the chip idle that way: give it with the class axis last in memory (1 x 32768 x 64 bfloat16: 148 us
 in memory order, 8 us that way, 11 us for the copy).
 
+Tracers and dispatch modes (torch.compile, make_fx, torch.export, torch.jit.trace, FakeTensorMode) see registered operators
+with the same results; functorch's transforms are refused.
+
 Calls can be captured into a graph, backward passes with them; workspaces belong to the call, so graphs do
 not share them.  While a backward pass is captured, no eager graph of the same leaves may be alive (torch
 ends the process): drop the eager results first, or capture `torch.autograd.grad`.
