@@ -1015,7 +1015,7 @@ __device__ __forceinline__ float4 distill_stats(const RowSums& r, float c, float
     st.x = r.m_r;
     st.y = mass * exp2_((r.m_r - r.b) * c) / r.s - rr / r.s_r;
   } else {
-    st.y = 0.f * (r.s + mass);  // 0 for classes that are all impossible; NaN where a listed class or the list holds one
+    st.y = fmaf(0.f, r.s, 0.f * mass);  // 0 for classes that are all impossible; NaN where a listed class or the list holds one
   }
   st.w = mass / r.s;
   return st;
@@ -2073,11 +2073,11 @@ int make_plan(const dw_dist_desc* d, bool distill, bool backward, Plan* out) {
   P.last = (d->flags & DW_DIST_LAST) || d->inner == 1;
   const int64_t tiles = P.last ? (p.rows + 63) / 64 : d->outer * ((d->inner + 63) / 64);
   const int esize = d->dtype == DW_DTYPE_F32 ? 4 : 2;
-  // Planes are tiles.  Rows are from 128 tiles on and up to 2048 classes (forward + backward, us; the other family in brackets).
-  // 8200 rows bf16: 40 classes 4.3 + 4.5 (12.4 + 11.5), with the top 8 6.1 + 4.5 (39.9 + 11.2), 512 classes 7.4 + 8.5 (12.5 + 12.1).
-  // 3000 classes are rows, 18.2 + 24.2 (21.8 + 40.7).  Between, the two are near each other forward and rows win backward: 16400 x
+  // Planes are tiles; so are rows of up to 2048 classes from 128 tiles on (forward + backward, us; the other family in
+  // brackets).  8200 rows bf16: 40 classes 4.3 + 4.5 (12.4 + 11.5), with the top 8 6.1 + 4.5 (39.9 + 11.2), 512 classes 7.4 + 8.5 (12.5 + 12.1).
+  // Rows of 3000 classes are not, 18.2 + 24.2 (21.8 + 40.7).  Between, the two are near each other forward and rows win backward: 16400 x
   // 1000 bf16 17.3 + 22.8 (19.9 + 19.5), x 2048 26.0 + 40.5 (20.8 + 26.5; with the top 8 53.9, 43.7; distillation 34.7 + 41.3, 29.2
-  // + 29.2).  Fewer rows than that are rows though tiles of up to 512 classes take no longer: 4100 x 40 8.2 + 7.8 (4.2 + 4.5),
+  // + 29.2).  Nor are fewer rows, though those of up to 512 classes would be faster as tiles: 4100 x 40 8.2 + 7.8 (4.2 + 4.5),
   // top 8 24.4 (6.0), x 512 8.3 + 8.1 (7.0 + 7.4); 2100 x 1000 6.9 + 6.6 (10.1 + 11.2).
   P.tile = !P.last || (p.V <= 2048 && tiles * 4 >= kWantWaves / 4);
   if (P.tile) {

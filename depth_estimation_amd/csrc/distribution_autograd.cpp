@@ -5,10 +5,10 @@
 // training steps are bound by it: a node written in Python runs in the autograd engine's own thread, where the
 // interpreter's lock and cold caches took about half of such a step (80 to 90 us, 4 x 64 x 4 x 4).
 //
-// The library's functions come from Python as addresses, what a call has to know as a list of words: which build of the library is in
-// use, and what the shapes and types decide, is settled there (distribution.py).  These calls launch by pointer, so
-// nothing that records or replaces tensor operations sees more of them than their outputs being made: distribution.py
-// calls the registered operators wherever something of the kind watches.
+// The library's functions come from Python as addresses, what a call has to know as a list of words: which build of
+// the library is in use, and what the shapes and types decide, is settled there (distribution.py).  These calls launch
+// by pointer, so nothing that records or replaces tensor operations sees more of them than their outputs being made:
+// distribution.py calls the registered operators wherever something of the kind watches.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>

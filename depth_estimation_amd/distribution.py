@@ -3,7 +3,7 @@ kernels: scoring (log-probability of a given class, entropy, top alternatives) a
 a teacher known by its top entries, both differentiable.
 
 They stand next to the disparity regression of `disparity.soft_argmin` (the reference's
-/root/reference/model/model.py:417-429, 454-456; the reference itself has neither operator):
+model/model.py:417-429, 454-456; the reference itself has neither operator):
 
     teacher = log_probs(teacher_cost, scale=-1.0, top=8)                    # 64 bytes a pixel instead of 4 D
     loss = distill_loss(student_cost, teacher.top_log_prob, teacher.top_index, scale=-1.0)   # (B, H, W)
@@ -12,16 +12,17 @@ They stand next to the disparity regression of `disparity.soft_argmin` (the refe
 
 Logits are float32, bfloat16 or float16; the class axis is `dim` (1, as in a (B, D, H, W) volume or a
 (rows, classes) matrix), and `scale * logits` are the log-weights: -1 for a cost volume, 1/T for a
-temperature (of either sign, |scale| from 2^-120 to 2^120).  Tensors in memory order, or with the class axis last in memory (torch's channels_last),
-are read where they are; any other order is copied first.  Sums and results are float32, gradients
-have the type and the memory order of the logits (memory order, where those were copied).
+temperature (of either sign, |scale| from 2^-120 to 2^120).  Tensors in memory order, or with the class
+axis last in memory (torch's channels_last), are read where they are; any other order is copied first.
+Sums and results are float32, gradients have the type and the order of the logits (memory order, where
+those were copied).
 
 A volume in memory order is read by a block for every 64 pixels.  One of few pixels and thousands of classes
 leaves most of the chip idle that way: give it with the class axis last in memory (1 x 32768 x 64 bfloat16: 148 us
 in memory order, 8 us that way, 11 us for the copy).
 
-Tracers and dispatch modes (torch.compile, make_fx, torch.export, torch.jit.trace, FakeTensorMode) see registered operators
-with the same results; functorch's transforms are refused.
+Tracers and dispatch modes (torch.compile, make_fx, torch.export, torch.jit.trace, FakeTensorMode) see
+registered operators with the same results; eager calls refuse functorch's transforms.
 
 Calls can be captured into a graph, backward passes with them; workspaces belong to the call, so graphs do
 not share them.  While a backward pass is captured, no eager graph of the same leaves may be alive (torch

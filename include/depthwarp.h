@@ -374,7 +374,7 @@ DW_API int dw_lidar_project(int32_t B, int32_t n_max, int32_t H, int32_t W, cons
 /* ---------------------------------------------------------------------------
  * Distributions over classes (disparity bins of a volume, or any other soft-max
  * axis): scoring and distillation.  Absent from the reference; they stand next
- * to its disparity regression (/root/reference/model/model.py:417-429, 454-456).
+ * to its disparity regression (model/model.py:417-429, 454-456).
  *
  * Logits are (outer, classes, inner) contiguous; with DW_DIST_LAST the classes
  * of a row lie together: (outer, inner, classes).  Rows are numbered outer *
